@@ -270,8 +270,10 @@ enum ptxstd_mx_type {
  * elements x * 2^-(scale-127) RN .satfinite (narrow.rs:125-130). q [rows, cols] bytes in the
  * tensor cores' operand layout for K = 32 MMAs (descriptor.rs:306-315): FP8 one code per byte;
  * FP6 16 six-bit codes packed little-endian in 12 bytes + 4 zero bytes per 16 elements; FP4 16
- * nibbles in 8 bytes + 8 zero bytes. sf_layout as ptxstd_quantize_mxfp8_layout. For E4M3 the
- * result equals ptxstd_quantize_mxfp8_layout's. */
+ * nibbles in 8 bytes + 8 zero bytes. sf_layout as ptxstd_quantize_mxfp8_layout, or 2: blocked for
+ * any number of rows and any cols % 32 == 0, padded with zero bytes to ceil(rows/128) x
+ * ceil(cols/128) tiles (layout 1 where that needs no padding). For E4M3 the result equals
+ * ptxstd_quantize_mxfp8_layout's. */
 PTXSTD_API int ptxstd_quantize_mx(const uint16_t* d_x, int64_t rows, int64_t cols, int elem_type,
                                   uint8_t* d_q, uint8_t* d_sf, int sf_layout,
                                   ptxstd_stream stream);
@@ -283,6 +285,101 @@ PTXSTD_API int ptxstd_quantize_mx(const uint16_t* d_x, int64_t rows, int64_t col
 PTXSTD_API int ptxstd_gemm_mx(const uint8_t* d_a, int a_type, const uint8_t* d_sfa,
                               const uint8_t* d_b, int b_type, const uint8_t* d_sfb, uint16_t* d_c,
                               int64_t M, int64_t N, int64_t K, ptxstd_stream stream);
+/* ---- feed-forward operators around the MX GEMM -------------------------------------------------
+ * No counterpart in the reference (it has no kernels): what a transformer block puts around the
+ * quantiser and the MX GEMM, fused into them. Common to all of them:
+ *   - MX operands are those of ptxstd_quantize_mx: one byte per element, UE8M0 scales per 32 in the
+ *     blocked layout. Any number of rows and any multiple of 32 columns is taken: the scale tensor
+ *     then has ceil(rows/128) x ceil(cols/128) tiles of 512 bytes, and where an operator writes
+ *     such a tensor it writes the padding as zero bytes. Padding that is read may hold anything.
+ *   - elem_type / out_type: PTXSTD_MX_E4M3 or PTXSTD_MX_E5M2 where the operator quantises. It
+ *     quantises the f32 result directly, with the scale and element rules of ptxstd_quantize_mx.
+ *   - Launched with programmatic dependent launch; caller memory is touched only after
+ *     griddepcontrol.wait. No workspace unless one is named. Results are bitwise reproducible.
+ *   - rows, M >= 1; sizes below 2^31; all pointers 16-byte aligned unless noted. Outputs must not
+ *     overlap inputs, unless noted. */
+enum ptxstd_act {
+    PTXSTD_ACT_NONE = 0,
+    PTXSTD_ACT_RELU = 1,
+    PTXSTD_ACT_SILU = 2,      /* x / (1 + exp(-x)) */
+    PTXSTD_ACT_GELU = 3,      /* x Phi(x), Phi the normal distribution function */
+    PTXSTD_ACT_GELU_TANH = 4, /* x / (1 + exp(-2 u)), u = sqrt(2/pi) (x + 0.044715 x^3) */
+};
+/* MX GEMM with an epilogue: pre = A B^T + bias; result = act(pre) + residual.
+ * A [M, K], B [N, K] as for ptxstd_gemm_mx (any pair of element types). bias: bf16 [N] or null.
+ * residual: bf16 [M, N] or null; it may be d_c itself. d_pre: bf16 [M, N] or null, receives pre
+ * (what the backward pass needs). The result goes to d_c (bf16 [M, N]), to d_q / d_sfq (MX of
+ * out_type) or to both; one of them is required. K % 32 == 0; N % 8 == 0, with d_q N % 32 == 0. */
+PTXSTD_API int ptxstd_gemm_mx_epilogue(const uint8_t* d_a, int a_type, const uint8_t* d_sfa,
+                                       const uint8_t* d_b, int b_type, const uint8_t* d_sfb,
+                                       const uint16_t* d_bias, int act, const uint16_t* d_residual,
+                                       uint16_t* d_c, uint16_t* d_pre, int out_type, uint8_t* d_q,
+                                       uint8_t* d_sfq, int64_t M, int64_t N, int64_t K,
+                                       ptxstd_stream stream);
+/* Gated feed-forward projection, both products in one kernel: gate = A Wg^T, up = A Wu^T,
+ * h = act(gate) * up. Wg, Wu [F, K] of element type w_type. h goes to d_h (bf16 [M, F]), to
+ * d_q / d_sfq (MX of out_type) or to both; one of them is required. d_gate, d_up: bf16 [M, F], both
+ * or neither, receive the projections for the backward pass. K % 32 == 0; F % 8 == 0, with d_q
+ * F % 32 == 0. */
+PTXSTD_API int ptxstd_gemm_mx_gated(const uint8_t* d_a, int a_type, const uint8_t* d_sfa,
+                                    const uint8_t* d_wg, const uint8_t* d_sfg, const uint8_t* d_wu,
+                                    const uint8_t* d_sfu, int w_type, int act, uint16_t* d_h,
+                                    uint16_t* d_gate, uint16_t* d_up, int out_type, uint8_t* d_q,
+                                    uint8_t* d_sfq, int64_t M, int64_t F, int64_t K,
+                                    ptxstd_stream stream);
+/* Gradient of an activation, quantised for both products that follow. Gated (d_up given):
+ * D = [dh * up * act'(gate) | dh * act(gate)], W = 2 cols columns; ungated (d_up null):
+ * D = dh * act'(gate), W = cols. dh, gate, up: bf16 [rows, cols], cols % 32 == 0. D is written as
+ * an MX operand along its rows (d_q [rows, W], d_sf: the operand of dX = D Wt^T) and along its
+ * columns (d_qt [W, R], d_sft, R = rows rounded up to 32, the added columns zero codes: the
+ * operand of dW = D^T X). d_dbias: f32 [W] or null, receives the column sums of D (before
+ * quantisation); it needs d_workspace of ptxstd_act_backward_mx_workspace_bytes (0 without it),
+ * 16-byte aligned, which stream-ordered calls may share. */
+PTXSTD_API size_t ptxstd_act_backward_mx_workspace_bytes(int64_t rows, int64_t cols, int gated,
+                                                         int with_dbias);
+PTXSTD_API int ptxstd_act_backward_mx(int act, const uint16_t* d_dh, const uint16_t* d_gate,
+                                      const uint16_t* d_up, int64_t rows, int64_t cols,
+                                      int elem_type, uint8_t* d_q, uint8_t* d_sf, uint8_t* d_qt,
+                                      uint8_t* d_sft, float* d_dbias, void* d_workspace,
+                                      size_t workspace_bytes, ptxstd_stream stream);
+/* Transposing MX quantiser: bf16 [rows, cols] (cols % 8 == 0) -> payload [cols, R] with blocks of 32
+ * along the rows of x, R = rows rounded up to 32 (the added columns zero codes), and the blocked
+ * scales of that operand. */
+PTXSTD_API int ptxstd_quantize_mx_t(const uint16_t* d_x, int64_t rows, int64_t cols, int elem_type,
+                                    uint8_t* d_qt, uint8_t* d_sft, ptxstd_stream stream);
+/* The norms between two blocks of a residual stream, with the gate and scale of the branch that
+ * joins it, per row of [rows, cols]:
+ *   p  = y * ry * w_post, ry = 1 / sqrt(mean(y^2) + eps)   (w_post null: p = y)
+ *   x' = bf16(x + scale * g * p)                           (y null: x' = x)
+ *   n  = x' * rx * w, rx = 1 / sqrt(mean(x'^2) + eps)      (of x' as it is stored)
+ * x, y bf16 [rows, cols]; w, w_post bf16 [cols]; gate bf16 [gate_rows, cols] with gate_rows 1 (one
+ * gate for all rows) or rows (one per row), or null (g = 1). d_x_out: bf16 [rows, cols], required
+ * with y (it may be d_x itself), null without. n goes to d_n (bf16), to d_q / d_sf (MX of out_type,
+ * sf_layout 0 row-major or 1 blocked and padded) or to both; one of them is required.
+ * d_rstd (rx) and d_rstd_post (ry): f32 [rows] or null, for the backward pass.
+ * cols % 8 == 0, with d_q cols % 32 == 0; cols <= 32768; eps >= 0. */
+PTXSTD_API int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
+                                       const uint16_t* d_w_post, const uint16_t* d_gate,
+                                       int64_t gate_rows, float scale, const uint16_t* d_w,
+                                       float eps, int64_t rows, int64_t cols, uint16_t* d_x_out,
+                                       uint16_t* d_n, int out_type, uint8_t* d_q, uint8_t* d_sf,
+                                       int sf_layout, float* d_rstd, float* d_rstd_post,
+                                       ptxstd_stream stream);
+/* Its gradient. dn, x_out (= x'), and, when the branch took part, y, w_post, gate, scale as in the
+ * forward pass with the statistics it wrote (d_rstd_post with w_post). d_dx_out: bf16 gradient
+ * that reaches x' by other paths, or null. Writes d_dx (bf16, also the gradient of x), d_dw (f32
+ * [cols]), with y d_dy (bf16), with w_post d_dw_post (f32 [cols]), with gate d_dgate (f32 [cols]
+ * for gate_rows 1, else bf16 [rows, cols]). d_dx may be d_dx_out. cols % 8 == 0, cols <= 16384.
+ * Workspace (per-block partial column sums, added in a fixed order): queried with the device
+ * current that will run the call; stream-ordered calls may share it. */
+PTXSTD_API size_t ptxstd_rmsnorm_residual_backward_workspace_bytes(int64_t rows, int64_t cols);
+PTXSTD_API int ptxstd_rmsnorm_residual_backward(
+    const uint16_t* d_dn, const uint16_t* d_dx_out, const uint16_t* d_x_out, const uint16_t* d_w,
+    const float* d_rstd, const uint16_t* d_y, const uint16_t* d_w_post, const float* d_rstd_post,
+    const uint16_t* d_gate, int64_t gate_rows, float scale, int64_t rows, int64_t cols,
+    uint16_t* d_dx, float* d_dw, uint16_t* d_dy, float* d_dw_post, void* d_dgate,
+    void* d_workspace, size_t workspace_bytes, ptxstd_stream stream);
+
 /* The decompressing shared-memory -> Tensor Memory copy (copy::<S128x256b, B6x16P32 | B4x16P64>,
  * src/tcgen05/copy.rs:32-46, :76-116), run over n_tiles tiles of 128 rows x 32 bytes: packed FP6
  * (elem_type PTXSTD_MX_E2M3 / E3M2: .b8x16.b6x16_p32) or FP4 (PTXSTD_MX_E2M1: .b8x16.b4x16_p64)

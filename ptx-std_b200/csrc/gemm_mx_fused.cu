@@ -1,0 +1,1083 @@
+// MX GEMMs with an epilogue, on the 5th-generation tensor cores:
+//   linear:  pre = A B^T + bias,  result = act(pre) + residual
+//   gated:   gate = A Wg^T, up = A Wu^T,  result = act(gate) * up   (one kernel, A read once)
+// Operands as for ptxstd_gemm_mx (kind::mxf8f6f4 block32, any pair of element types), results as
+// bf16, as an MX operand (E4M3 / E5M2 + blocked UE8M0 scales) for the next GEMM, or both. The f32
+// accumulator is biased, activated, multiplied and added to in f32 and rounded once, to bf16 or
+// straight to the 8-bit code (no bf16 step between).
+//
+// Two kernels share that contract:
+//
+// 1. wide_kernel, for many rows: the CTA-pair pipeline of gemm_mxfp8.cu (256 x 256 tiles of
+//    cta_group::2 MMAs, 6 stages of 128 K elements, eight epilogue warps per CTA). For the gated
+//    product the pair's 256 B rows are 128 rows of Wg (loaded by CTA 0) and the same 128 of Wu (by
+//    CTA 1), so the accumulator's columns 0..127 are gate and 128..255 up for the same 128
+//    features; an epilogue warp takes 64 columns of each, and the product needs no exchange. A
+//    lane holds one row, so the 32 elements of an MX block are in one thread's registers and the
+//    block's scale takes no shuffle.
+//    Ragged sizes: TMA fills rows and K elements outside the tensors with zeros and clips the
+//    stores; MMAs of a last K stage whose 32 elements lie outside are not issued, so padding
+//    scales (which may be NaN codes) never meet a product that is kept.
+//
+// 2. narrow_kernel, for few rows (serving): weight streaming, bound by HBM. The operands swap: 128
+//    weight rows are the M side of a cta_group::1 MMA and the tokens (up to 256, a multiple of 16)
+//    the N side, so a token costs one accumulator column instead of a padded row. K is split
+//    over a cluster; the CTAs' partial accumulators meet in distributed shared memory and are
+//    added in rank order, each CTA finishing every S-th token, so the split needs no workspace,
+//    no atomics and no second kernel, and the result is reproducible.
+//
+// Every device-side wait is bounded; a timeout records PTXSTD_ETIMEOUT.
+#include <atomic>
+
+#include "common.cuh"
+#include "data_types.cuh"
+#include "epilogue.cuh"
+#include "mx_block.cuh"
+#include "tcgen05.cuh"
+#include "tma_host.h"
+
+namespace {
+
+namespace t5 = ptxstd::tcgen05;
+namespace dt = ptxstd::data_types;
+namespace mx = ptxstd::mx;
+using ptxstd::mbar_wait;
+
+constexpr uint32_t BK = 128;            // K elements (= bytes) per stage
+constexpr uint32_t kMmaK = 32;          // K elements of one mxf8f6f4 MMA
+constexpr uint32_t kMmas = BK / kMmaK;  // 4 per stage, one scale byte each
+
+// What the epilogues read and write besides the tensor maps.
+struct Epi {
+    const uint16_t* bias;
+    const uint16_t* residual;
+    uint16_t* c;     // bf16 result, or null
+    uint16_t* pre;   // bf16 pre-activation (linear) / gate projection (gated), or null
+    uint16_t* up;    // bf16 up projection (gated), or null
+    uint8_t* q;      // MX payload, or null
+    uint8_t* sfq;
+    uint32_t q_type;
+    uint32_t act;
+};
+
+__device__ __forceinline__ float f(uint32_t r) { return __uint_as_float(r); }
+
+// ---------------------------------------------------------------------------------------------
+// Many rows: CTA pairs, 256-row tiles
+// ---------------------------------------------------------------------------------------------
+namespace wide {
+
+constexpr uint32_t P_BM = 256, P_BN = 256, P_HALF = 128;
+constexpr uint32_t STAGES = 6;
+constexpr uint32_t kEpiWarps = 8;
+constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kABytes = P_HALF * BK;
+constexpr uint32_t kBBytes = P_HALF * BK;
+constexpr uint32_t kSfaBytes = 512;
+constexpr uint32_t kSfbBytes = (P_BN / 128) * 512;
+constexpr uint32_t kCtaStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
+constexpr uint32_t kSlotCols = 4 + 4 * (P_BN / 128);
+constexpr uint32_t kSfBase = P_BN;
+constexpr uint32_t kTmemCols = 512;
+static_assert(kSfBase + STAGES * kSlotCols <= kTmemCols, "TMEM budget");
+constexpr uint32_t kGroupM = 8;
+constexpr uint32_t kCCols = 32;  // bf16 columns (or 64 MX bytes) per epilogue store
+using StageBox = ptxstd::epi::Box<kCCols>;
+
+struct alignas(1024) Smem {
+    uint8_t a[STAGES][kABytes];
+    uint8_t b[STAGES][kBBytes];
+    uint8_t sfa[STAGES][kSfaBytes];
+    uint8_t sfb[STAGES][kSfbBytes];
+    uint8_t cstage[kEpiWarps][StageBox::kBytes];
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t tfull;
+    uint64_t tempty;
+    uint64_t drain;
+    uint32_t tmem_base;
+    uint32_t abort;
+};
+constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory budget");
+
+enum : uint32_t { kDetailProducer = 0x3500, kDetailMma = 0x3600, kDetailEpilogue = 0x3700 };
+
+struct Maps {
+    CUtensorMap a, sfa;
+    CUtensorMap b, sfb;    // linear: B; gated: Wg
+    CUtensorMap b2, sfb2;  // gated: Wu
+    CUtensorMap c, pre, up, q;
+};
+
+__device__ __forceinline__ void tile_coords(uint32_t t, uint32_t num_m, uint32_t num_n,
+                                            uint32_t& mb, uint32_t& nb) {
+    const uint32_t group_tiles = kGroupM * num_n;
+    const uint32_t g = t / group_tiles;
+    const uint32_t first_m = g * kGroupM;
+    const uint32_t gm = min(num_m - first_m, kGroupM);
+    const uint32_t local = t - g * group_tiles;
+    mb = first_m + local % gm;
+    nb = local / gm;
+}
+
+__device__ __forceinline__ void fail(Smem& s, uint32_t* err, uint32_t detail) {
+    ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail);
+    *reinterpret_cast<volatile uint32_t*>(&s.abort) = 1u;
+}
+__device__ __forceinline__ bool aborted(Smem& s) {
+    return *reinterpret_cast<volatile uint32_t*>(&s.abort) != 0u;
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                         uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
+
+// One epilogue warp's 32 rows, leaving through its staging buffer.
+struct Out {
+    uint32_t stg, lane;
+    int32_t row0;
+    uint32_t row, M, N;  // this lane's row; the result's sizes
+
+    // 32 bf16 columns r[FIRST..] at col0 of `map`.
+    template <uint32_t FIRST, uint32_t L>
+    __device__ __forceinline__ void bf16(const CUtensorMap* map, const uint32_t (&r)[L],
+                                         uint32_t col0) const {
+        if (col0 >= N || static_cast<uint32_t>(row0) >= M) return;
+        ptxstd::epi::wait_staging(lane);
+        ptxstd::epi::stage_store<kCCols, FIRST>(map, stg, r, 1.0f, static_cast<int32_t>(col0),
+                                                row0, lane);
+    }
+    // Two MX blocks r[FIRST .. FIRST + 63] at col0; returns their scale codes (0 outside N or M).
+    template <uint32_t FIRST, uint32_t L>
+    __device__ __forceinline__ uint32_t mx2(const CUtensorMap* map, const uint32_t (&r)[L],
+                                            uint32_t col0, uint32_t type) const {
+        uint32_t codes = 0;
+        const bool any = col0 < N && static_cast<uint32_t>(row0) < M;
+        if (any) ptxstd::epi::wait_staging(lane);
+        const uint32_t emax = mx::emax_of(type);
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            uint32_t m = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) m = mx::amax_bits(m, f(r[FIRST + 32 * h + i]));
+            const uint32_t code = mx::scale_code(m, emax);
+            const float inv = dt::ue8m0_inverse(code);
+            if (row < M && col0 + 32 * h < N) codes |= code << (8 * h);
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c) {
+                uint32_t p[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t i = FIRST + 32 * h + 16 * c + 4 * k;
+                    p[k] = mx::pack4(type, f(r[i]), f(r[i + 1]), f(r[i + 2]), f(r[i + 3]), inv);
+                }
+                if (any)
+                    ptxstd::st_shared_v4(stg + StageBox::offset(lane, 2 * h + c), p[0], p[1], p[2],
+                                         p[3]);
+            }
+        }
+        if (any) {
+            ptxstd::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                ptxstd::tma_store_2d(map, stg, static_cast<int32_t>(col0), row0);
+                ptxstd::bulk_commit_group();
+            }
+        }
+        return codes;
+    }
+};
+
+template <uint32_t FIRST, uint32_t L>
+__device__ __forceinline__ void add_bias32(uint32_t (&r)[L], const uint16_t* bias, uint32_t col,
+                                           uint32_t N) {
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (col + 8 * c < N) w = __ldg(reinterpret_cast<const uint4*>(bias + col + 8 * c));
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t i = FIRST + 8 * c + 2 * k;
+            r[i] = __float_as_uint(f(r[i]) + dt::bf16_lo(v[k]));
+            r[i + 1] = __float_as_uint(f(r[i + 1]) + dt::bf16_hi(v[k]));
+        }
+    }
+}
+
+template <uint32_t FIRST, uint32_t L>
+__device__ __forceinline__ void act32(uint32_t (&r)[L], uint32_t kind) {
+    switch (kind) {  // one loop per kind: the choice is made once per 32 elements
+#define PTXSTD_CASE(K)                                                            \
+    case K:                                                                       \
+        _Pragma("unroll") for (uint32_t i = 0; i < 32; ++i)                       \
+            r[FIRST + i] = __float_as_uint(mx::act(K, f(r[FIRST + i])));          \
+        break;
+        PTXSTD_CASE(PTXSTD_ACT_RELU)
+        PTXSTD_CASE(PTXSTD_ACT_SILU)
+        PTXSTD_CASE(PTXSTD_ACT_GELU)
+        PTXSTD_CASE(PTXSTD_ACT_GELU_TANH)
+#undef PTXSTD_CASE
+    default: break;
+    }
+}
+
+// The linear epilogue of 32 accumulator columns r[FIRST..] at column `col` of the result.
+template <uint32_t FIRST, uint32_t L>
+__device__ __forceinline__ void linear32(uint32_t (&r)[L], const Out& o, const Epi& e,
+                                         const Maps& maps, uint32_t col) {
+    uint4 res[4];
+    if (e.residual) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            res[c] = make_uint4(0, 0, 0, 0);
+            if (o.row < o.M && col + 8 * c < o.N)
+                res[c] = *reinterpret_cast<const uint4*>(
+                    e.residual + static_cast<size_t>(o.row) * o.N + col + 8 * c);
+        }
+    }
+    if (e.bias) add_bias32<FIRST>(r, e.bias, col, o.N);
+    if (e.pre) o.bf16<FIRST>(&maps.pre, r, col);
+    act32<FIRST>(r, e.act);
+    if (e.residual) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            const uint32_t v[4] = {res[c].x, res[c].y, res[c].z, res[c].w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t i = FIRST + 8 * c + 2 * k;
+                r[i] = __float_as_uint(f(r[i]) + dt::bf16_lo(v[k]));
+                r[i + 1] = __float_as_uint(f(r[i + 1]) + dt::bf16_hi(v[k]));
+            }
+        }
+    }
+    if (e.c) o.bf16<FIRST>(&maps.c, r, col);
+}
+
+// h = act(gate) * up for 32 columns: gate r[FIRST..], up r[64 + FIRST..]; h replaces gate.
+template <uint32_t FIRST>
+__device__ __forceinline__ void gated32(uint32_t (&r)[128], const Out& o, const Epi& e,
+                                        const Maps& maps, uint32_t col) {
+    if (e.pre) {
+        o.bf16<FIRST>(&maps.pre, r, col);
+        o.bf16<64 + FIRST>(&maps.up, r, col);
+    }
+    act32<FIRST>(r, e.act);
+#pragma unroll
+    for (uint32_t i = 0; i < 32; ++i)
+        r[FIRST + i] = __float_as_uint(f(r[FIRST + i]) * f(r[64 + FIRST + i]));
+    if (e.c) o.bf16<FIRST>(&maps.c, r, col);
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+    wide_kernel(const __grid_constant__ Maps maps, uint32_t M, uint32_t N, uint32_t K,
+                uint32_t atype, uint32_t btype, const __grid_constant__ Epi e, uint32_t* err) {
+    constexpr uint32_t kTileN = GATED ? 128 : 256;  // result columns of a tile
+    extern __shared__ uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                       ~static_cast<uintptr_t>(1023));
+    const uint32_t warp = ptxstd::warp_id();
+    const uint32_t lane = ptxstd::lane_id();
+    const uint32_t rank = ptxstd::cluster_ctarank();
+    const uint32_t pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const uint32_t num_m = (M + P_BM - 1) / P_BM, num_n = (N + kTileN - 1) / kTileN;
+    const uint32_t num_tiles = num_m * num_n, num_k = (K + BK - 1) / BK;
+
+    if (warp == 0 && lane == 0) {
+        ptxstd::prefetch_tensormap(&maps.a);
+        ptxstd::prefetch_tensormap(&maps.b);
+        ptxstd::prefetch_tensormap(&maps.sfa);
+        ptxstd::prefetch_tensormap(&maps.sfb);
+        if (GATED) {
+            ptxstd::prefetch_tensormap(&maps.b2);
+            ptxstd::prefetch_tensormap(&maps.sfb2);
+        }
+        for (uint32_t i = 0; i < STAGES; ++i) {
+            ptxstd::mbar_init(&s.full[i], 1);
+            ptxstd::mbar_init(&s.empty[i], 1);
+        }
+        ptxstd::mbar_init(&s.tfull, 1);
+        ptxstd::mbar_init(&s.tempty, 2 * kEpiWarps);
+        ptxstd::mbar_init(&s.drain, 1);
+        s.abort = 0;
+        ptxstd::fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        t5::tmem_alloc_pair(&s.tmem_base, kTmemCols);
+        t5::tmem_relinquish_pair();
+    }
+    t5::fence_before_thread_sync();
+    ptxstd::cluster_sync();
+    t5::fence_after_thread_sync();
+    const uint32_t tmem = s.tmem_base;
+    // Only now, with this CTA's TMEM allocated: a dependent CTA on the same SM allocates its own
+    // before it waits for this grid, and must not be able to take what this one still needs.
+    ptxstd::pdl_launch_dependents();
+    ptxstd::pdl_wait();
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        if (ptxstd::elect_one()) {
+            const CUtensorMap* mb_ = GATED && rank == 1 ? &maps.b2 : &maps.b;
+            uint32_t stage = 0, phase = 0, issued = 0, issued_parity = 0;
+            for (uint32_t t = pair; t < num_tiles && !aborted(s); t += n_pairs) {
+                uint32_t mb, nb;
+                tile_coords(t, num_m, num_n, mb, nb);
+                const int32_t b_row =
+                    static_cast<int32_t>(GATED ? nb * 128 : nb * P_BN + rank * P_HALF);
+                for (uint32_t kb = 0; kb < num_k; ++kb) {
+                    if (!mbar_wait(&s.empty[stage], phase ^ 1u)) {
+                        fail(s, err, kDetailProducer | stage);
+                        break;
+                    }
+                    if (aborted(s)) break;
+                    const uint32_t fl = ptxstd::mapa_shared(ptxstd::smem_u32(&s.full[stage]), 0);
+                    if (rank == 0) ptxstd::mbar_arrive_expect_tx(&s.full[stage], 2 * kCtaStageBytes);
+                    ptxstd::tma_load_2d_pair(s.a[stage], &maps.a, fl, static_cast<int32_t>(kb * BK),
+                                             static_cast<int32_t>(mb * P_BM + rank * P_HALF));
+                    ptxstd::tma_load_2d_pair(s.b[stage], mb_, fl, static_cast<int32_t>(kb * BK),
+                                             b_row);
+                    ptxstd::tma_load_2d_pair(s.sfa[stage], &maps.sfa, fl, 0,
+                                             static_cast<int32_t>((mb * 2 + rank) * num_k + kb));
+                    if constexpr (GATED) {
+                        ptxstd::tma_load_2d_pair(s.sfb[stage], &maps.sfb, fl, 0,
+                                                 static_cast<int32_t>(nb * num_k + kb));
+                        ptxstd::tma_load_2d_pair(s.sfb[stage] + 512, &maps.sfb2, fl, 0,
+                                                 static_cast<int32_t>(nb * num_k + kb));
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < P_BN / 128; ++j)
+                            ptxstd::tma_load_2d_pair(
+                                s.sfb[stage] + j * 512, &maps.sfb, fl, 0,
+                                static_cast<int32_t>((nb * 2 + j) * num_k + kb));
+                    }
+                    issued |= 1u << stage;
+                    issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (aborted(s) && rank == 0) {
+                for (uint32_t i = 0; i < STAGES; ++i)
+                    if (issued & (1u << i)) mbar_wait(&s.full[i], (issued_parity >> i) & 1u);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (leader) ----------------
+        if (rank == 0 && ptxstd::elect_one()) {
+            uint32_t idesc0 = 0;
+            t5::idesc_mxf8f6f4(atype, btype, P_BM, P_BN, idesc0);
+            uint32_t idesc[kMmas];
+#pragma unroll
+            for (uint32_t j = 0; j < kMmas; ++j) {
+                uint32_t t0 = 0;
+                t5::idesc_with_field(idesc0, 29, 2, j, t0);   // scale-factor A id
+                t5::idesc_with_field(t0, 4, 2, j, idesc[j]);  // scale-factor B id
+            }
+            uint32_t stage = 0, phase = 0, acc_phase = 0;
+            for (uint32_t t = pair; t < num_tiles && !aborted(s); t += n_pairs) {
+                if (!mbar_wait(&s.tempty, acc_phase ^ 1u)) {
+                    fail(s, err, kDetailMma | 0x90);
+                    break;
+                }
+                t5::fence_after_thread_sync();
+                bool ok = true;
+                for (uint32_t kb = 0; kb < num_k; ++kb) {
+                    if (!mbar_wait(&s.full[stage], phase)) {
+                        fail(s, err, kDetailMma | 0x80 | stage);
+                        ok = false;
+                        break;
+                    }
+                    t5::fence_after_thread_sync();
+                    const uint64_t ad = t5::smem_desc_k128(ptxstd::smem_u32(s.a[stage]));
+                    const uint64_t bd = t5::smem_desc_k128(ptxstd::smem_u32(s.b[stage]));
+                    const uint32_t slot = tmem + kSfBase + stage * kSlotCols;
+                    t5::cp_32x128b_warpx4_pair(
+                        slot, t5::smem_desc_nosw(ptxstd::smem_u32(s.sfa[stage]), 0, 128));
+#pragma unroll
+                    for (uint32_t h = 0; h < P_BN / 128; ++h)
+                        t5::cp_32x128b_warpx4_pair(
+                            slot + 4 + 4 * h,
+                            t5::smem_desc_nosw(ptxstd::smem_u32(s.sfb[stage] + 512 * h), 0, 128));
+                    const uint32_t live = (K - kb * BK) / kMmaK;  // MMAs inside K
+#pragma unroll
+                    for (uint32_t j = 0; j < kMmas; ++j)
+                        if (j < live)
+                            mma_pair(tmem, ad + 2 * j, bd + 2 * j, idesc[j], slot, slot + 4,
+                                     (kb | j) != 0u);
+                    const uint32_t em = ptxstd::smem_u32(&s.empty[stage]);
+                    t5::commit_pair(em);
+                    t5::commit_pair(ptxstd::mapa_shared(em, 1));
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                const uint32_t fu = ptxstd::smem_u32(&s.tfull);
+                t5::commit_pair(fu);
+                t5::commit_pair(ptxstd::mapa_shared(fu, 1));
+                acc_phase ^= 1u;
+            }
+            t5::commit_pair(ptxstd::smem_u32(&s.drain));
+            mbar_wait(&s.drain, 0);
+        }
+    } else {
+        // ---------------- epilogue: warps 2..9 of both CTAs ----------------
+        const uint32_t q = warp & 3u;
+        const uint32_t half = (warp - 2u) >> 2;
+        uint32_t acc_phase = 0;
+        const uint32_t tempty_leader = ptxstd::mapa_shared(ptxstd::smem_u32(&s.tempty), 0);
+        const size_t q_tiles_k = mx::tiles_k(N / 32);
+        for (uint32_t t = pair; t < num_tiles; t += n_pairs) {
+            bool ok = !aborted(s) && mbar_wait(&s.tfull, acc_phase);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                if (lane == 0 && !aborted(s)) fail(s, err, kDetailEpilogue | 0x80);
+                break;
+            }
+            t5::fence_after_thread_sync();
+            // linear: accumulator columns 128 half .. + 127; gated: gate columns 64 half .. + 63,
+            // then up columns 128 + 64 half .. + 63
+            uint32_t r[128];
+            const uint32_t lo = tmem + ((32 * q) << 16) + half * (GATED ? 64 : 128);
+            const uint32_t hi = lo + (GATED ? 128 : 64);
+            {
+                uint32_t(&r0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&r[0]);
+                uint32_t(&r1)[32] = *reinterpret_cast<uint32_t(*)[32]>(&r[32]);
+                uint32_t(&r2)[32] = *reinterpret_cast<uint32_t(*)[32]>(&r[64]);
+                uint32_t(&r3)[32] = *reinterpret_cast<uint32_t(*)[32]>(&r[96]);
+                t5::ld_32x32b_x32(lo, r0);
+                t5::ld_32x32b_x32(lo + 32, r1);
+                t5::ld_32x32b_x32(hi, r2);
+                t5::ld_32x32b_x32(hi + 32, r3);
+                t5::wait_ld();
+            }
+            t5::fence_before_thread_sync();
+            __syncwarp();
+            if (lane == 0) ptxstd::mbar_arrive_cluster(tempty_leader);
+            acc_phase ^= 1u;
+
+            uint32_t mb, nb;
+            tile_coords(t, num_m, num_n, mb, nb);
+            Out o;
+            o.stg = ptxstd::smem_u32(s.cstage[warp - 2u]);
+            o.lane = lane;
+            o.row0 = static_cast<int32_t>(mb * P_BM + rank * P_HALF + 32 * q);
+            o.row = static_cast<uint32_t>(o.row0) + lane;
+            o.M = M;
+            o.N = N;
+            const uint32_t col0 = nb * kTileN + half * (GATED ? 64 : 128);
+            const bool in_tiles = o.row < mx::padded_rows(M);  // a row of the scale tiles
+            if constexpr (GATED) {
+                gated32<0>(r, o, e, maps, col0);
+                gated32<32>(r, o, e, maps, col0 + 32);
+                if (e.q) {
+                    const uint32_t codes = o.mx2<0>(&maps.q, r, col0, e.q_type);
+                    // the tile's four scale columns: this warp holds two of them
+                    if (in_tiles)
+                        *reinterpret_cast<uint16_t*>(
+                            e.sfq + mx::word_offset(o.row, nb, q_tiles_k) + 2 * half) =
+                            static_cast<uint16_t>(codes);
+                }
+            } else {
+                linear32<0>(r, o, e, maps, col0);
+                linear32<32>(r, o, e, maps, col0 + 32);
+                linear32<64>(r, o, e, maps, col0 + 64);
+                linear32<96>(r, o, e, maps, col0 + 96);
+                if (e.q) {
+                    uint32_t codes = o.mx2<0>(&maps.q, r, col0, e.q_type);
+                    codes |= o.mx2<64>(&maps.q, r, col0 + 64, e.q_type) << 16;
+                    if (in_tiles && col0 < N)
+                        *reinterpret_cast<uint32_t*>(
+                            e.sfq + mx::word_offset(o.row, nb * 2 + half, q_tiles_k)) = codes;
+                }
+            }
+        }
+        ptxstd::epi::drain(lane);
+    }
+
+    t5::fence_before_thread_sync();
+    ptxstd::cluster_sync();
+    t5::fence_after_thread_sync();
+    if (warp == 1) t5::tmem_dealloc_pair(tmem, kTmemCols);
+}
+
+}  // namespace wide
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: weights on the M side, tokens on the N side, K split over a cluster
+// ---------------------------------------------------------------------------------------------
+namespace narrow {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWBytes = 128 * BK;  // one weight tile of a stage
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMaxCluster = 8;
+
+enum : uint32_t { kDetailProducer = 0x3900, kDetailMma = 0x3A00, kDetailEpilogue = 0x3B00 };
+
+struct Maps {
+    CUtensorMap x, sfx;
+    CUtensorMap w, sfw;    // linear: B; gated: Wg
+    CUtensorMap w2, sfw2;  // gated: Wu
+};
+
+struct Shape {
+    uint32_t M, N, K;
+    uint32_t tokens;    // token columns of a CTA: a multiple of 16, up to 256
+    uint32_t stages;
+    uint32_t split;     // CTAs of a cluster = K slices
+    uint32_t tmem_cols;
+};
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+struct Bars {
+    uint64_t full[kMaxStages];
+    uint64_t empty[kMaxStages];
+    uint64_t done;
+    uint32_t tmem_base;
+    uint32_t abort;
+};
+
+template <bool GATED>
+__global__ void __launch_bounds__(kThreads)
+    narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape p,
+                  uint32_t wtype, uint32_t xtype, const __grid_constant__ Epi e, uint32_t* err) {
+    constexpr uint32_t G = GATED ? 2 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Bars b;
+    const uint32_t raw = ptxstd::smem_u32(smem_raw);
+    uint8_t* const base = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+    const uint32_t T = p.tokens, tok_tiles = (T + 127) / 128;
+    const uint32_t stage_bytes = G * kWBytes + T * BK;
+    const uint32_t sf_bytes = (G + tok_tiles) * 512;
+    uint8_t* const sf_base = base + p.stages * stage_bytes;
+    float* const part = reinterpret_cast<float*>(base);  // after the products: [G][T][128]
+
+    const uint32_t warp = ptxstd::warp_id(), lane = ptxstd::lane_id(), tid = threadIdx.x;
+    const uint32_t rank = p.split > 1 ? ptxstd::cluster_ctarank() : 0;
+    const uint32_t block = blockIdx.x / p.split;  // 128 weight rows
+    const uint32_t num_k = (p.K + BK - 1) / BK;
+    const uint32_t k_lo = static_cast<uint32_t>(static_cast<uint64_t>(num_k) * rank / p.split);
+    const uint32_t k_hi = static_cast<uint32_t>(static_cast<uint64_t>(num_k) * (rank + 1) / p.split);
+    const uint32_t tok0 = blockIdx.y * T;
+    volatile uint32_t* abort_flag = &b.abort;
+
+    if (tid == 0) {
+        ptxstd::prefetch_tensormap(&maps.x);
+        ptxstd::prefetch_tensormap(&maps.w);
+        ptxstd::prefetch_tensormap(&maps.sfx);
+        ptxstd::prefetch_tensormap(&maps.sfw);
+        for (uint32_t i = 0; i < p.stages; ++i) {
+            ptxstd::mbar_init(&b.full[i], 1);
+            ptxstd::mbar_init(&b.empty[i], 1);
+        }
+        ptxstd::mbar_init(&b.done, 1);
+        b.abort = 0;
+        ptxstd::fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        t5::tmem_alloc(&b.tmem_base, p.tmem_cols);
+        t5::tmem_relinquish();
+    }
+    t5::fence_before_thread_sync();
+    __syncthreads();
+    t5::fence_after_thread_sync();
+    const uint32_t tmem = b.tmem_base;
+    ptxstd::pdl_launch_dependents();  // after the TMEM allocation, as in the wide kernel
+    ptxstd::pdl_wait();
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        if (ptxstd::elect_one()) {
+            uint32_t stage = 0, phase = 0, issued = 0, issued_parity = 0;
+            for (uint32_t kb = k_lo; kb < k_hi; ++kb) {
+                if (!mbar_wait(&b.empty[stage], phase ^ 1u)) {
+                    ptxstd::record_error(err, PTXSTD_ETIMEOUT, kDetailProducer | stage);
+                    *abort_flag = 1u;
+                }
+                if (*abort_flag) break;
+                uint8_t* const st = base + stage * stage_bytes;
+                uint8_t* const sf = sf_base + stage * sf_bytes;
+                const int32_t k = static_cast<int32_t>(kb * BK);
+                ptxstd::mbar_arrive_expect_tx(&b.full[stage], stage_bytes + sf_bytes);
+                ptxstd::tma_load_2d(st, &maps.w, &b.full[stage], k,
+                                    static_cast<int32_t>(block * 128));
+                if constexpr (GATED)
+                    ptxstd::tma_load_2d(st + kWBytes, &maps.w2, &b.full[stage], k,
+                                        static_cast<int32_t>(block * 128));
+                ptxstd::tma_load_2d(st + G * kWBytes, &maps.x, &b.full[stage], k,
+                                    static_cast<int32_t>(tok0));
+                ptxstd::tma_load_2d(sf, &maps.sfw, &b.full[stage], 0,
+                                    static_cast<int32_t>(block * num_k + kb));
+                if constexpr (GATED)
+                    ptxstd::tma_load_2d(sf + 512, &maps.sfw2, &b.full[stage], 0,
+                                        static_cast<int32_t>(block * num_k + kb));
+                for (uint32_t j = 0; j < tok_tiles; ++j)
+                    ptxstd::tma_load_2d(sf + (G + j) * 512, &maps.sfx, &b.full[stage], 0,
+                                        static_cast<int32_t>((tok0 / 128 + j) * num_k + kb));
+                issued |= 1u << stage;
+                issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (*abort_flag) {
+                for (uint32_t i = 0; i < p.stages; ++i)
+                    if (issued & (1u << i)) mbar_wait(&b.full[i], (issued_parity >> i) & 1u);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (ptxstd::elect_one()) {
+            uint32_t idesc0 = 0;
+            t5::idesc_mxf8f6f4(wtype, xtype, 128, T, idesc0);
+            uint32_t idesc[kMmas];
+#pragma unroll
+            for (uint32_t j = 0; j < kMmas; ++j) {
+                uint32_t t0 = 0;
+                t5::idesc_with_field(idesc0, 29, 2, j, t0);
+                t5::idesc_with_field(t0, 4, 2, j, idesc[j]);
+            }
+            const uint32_t slot_cols = 4 * (G + tok_tiles);
+            uint32_t stage = 0, phase = 0;
+            for (uint32_t kb = k_lo; kb < k_hi; ++kb) {
+                if (!mbar_wait(&b.full[stage], phase)) {
+                    ptxstd::record_error(err, PTXSTD_ETIMEOUT, kDetailMma | stage);
+                    *abort_flag = 1u;
+                    break;
+                }
+                t5::fence_after_thread_sync();
+                const uint32_t st = ptxstd::smem_u32(base + stage * stage_bytes);
+                const uint32_t sf = ptxstd::smem_u32(sf_base + stage * sf_bytes);
+                const uint32_t slot = tmem + G * T + stage * slot_cols;
+                for (uint32_t j = 0; j < G + tok_tiles; ++j)
+                    t5::cp_32x128b_warpx4(slot + 4 * j,
+                                          t5::smem_desc_nosw(sf + 512 * j, 0, 128));
+                const uint64_t xd = t5::smem_desc_k128(st + G * kWBytes);
+                const uint32_t live = (p.K - kb * BK) / kMmaK;
+#pragma unroll
+                for (uint32_t g = 0; g < G; ++g) {
+                    const uint64_t wd = t5::smem_desc_k128(st + g * kWBytes);
+#pragma unroll
+                    for (uint32_t j = 0; j < kMmas; ++j)
+                        if (j < live)
+                            t5::mma_mxf8f6f4_block32(tmem + g * T, wd + 2 * j, xd + 2 * j,
+                                                     idesc[j], slot + 4 * g, slot + 4 * G,
+                                                     kb > k_lo || j > 0);
+                }
+                t5::commit(&b.empty[stage]);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            t5::commit(&b.done);
+        }
+    }
+    __syncwarp();
+
+    // ---------------- every warp: accumulators to shared memory, then the epilogue -----------
+    // `done` completes after the last MMA; by then every load has landed, so the ring's memory
+    // is free for the partial sums.
+    bool ok = mbar_wait(&b.done, 0);
+    if (!ok && lane == 0) ptxstd::record_error(err, PTXSTD_ETIMEOUT, kDetailEpilogue);
+    ok = __syncthreads_and(ok && !*abort_flag);
+    t5::fence_after_thread_sync();
+    if (ok) {
+        const uint32_t q = warp & 3u;
+        for (uint32_t c = (warp >> 2) * 8; c < G * T; c += 16) {
+            uint32_t r[8];
+            t5::ld_32x32b_x8(tmem + ((32 * q) << 16) + c, r);
+            t5::wait_ld();
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                part[(c + i) * 128 + 32 * q + lane] = k_hi > k_lo ? f(r[i]) : 0.0f;
+        }
+    }
+    t5::fence_before_thread_sync();
+    if (p.split > 1) ptxstd::cluster_sync();
+    else __syncthreads();
+    t5::fence_after_thread_sync();
+    if (warp == 1) t5::tmem_dealloc(tmem, p.tmem_cols);
+
+    if (ok) {
+        // 16 threads per token, 8 result columns (weight rows) each; CTA `rank` takes the tokens
+        // rank, rank + split, ... of the tile. With an MX result the padding rows of the last
+        // scale tile get zero codes.
+        const uint32_t c8 = (tid & 15u) * 8, col = block * 128 + c8;
+        const uint32_t live = min(T, p.M - tok0);
+        const bool last_y = blockIdx.y + 1 == gridDim.y;
+        const uint32_t upto =
+            e.q ? (last_y ? static_cast<uint32_t>(mx::padded_rows(p.M)) - tok0 : T) : live;
+        const bool col_ok = col < p.N;
+        const size_t q_tiles_k = mx::tiles_k(p.N / 32);
+        const uint32_t part_addr = ptxstd::smem_u32(part);
+        float bias[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) bias[i] = 0.0f;
+        if (!GATED && e.bias && col_ok) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(e.bias + col));
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                bias[2 * k] = dt::bf16_lo(v[k]);
+                bias[2 * k + 1] = dt::bf16_hi(v[k]);
+            }
+        }
+        // uniform trip count per warp (the shuffles below take all lanes)
+        for (uint32_t t0 = rank; t0 < upto; t0 += 16 * p.split) {
+            const uint32_t t = t0 + (tid >> 4) * p.split;
+            const bool on = t < live && col_ok;
+            const size_t at = static_cast<size_t>(tok0 + t) * p.N + col;
+            float v[G][8];
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g)
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) v[g][i] = 0.0f;
+            uint4 res = make_uint4(0, 0, 0, 0);
+            if (on) {
+                if (!GATED && e.residual) res = *reinterpret_cast<const uint4*>(e.residual + at);
+                for (uint32_t s = 0; s < p.split; ++s) {
+#pragma unroll
+                    for (uint32_t g = 0; g < G; ++g) {
+                        uint32_t a = part_addr + ((g * T + t) * 128 + c8) * 4;
+                        if (p.split > 1) a = ptxstd::mapa_shared(a, s);
+                        const float4 x = ld_cluster_v4(a), y = ld_cluster_v4(a + 16);
+                        v[g][0] += x.x;
+                        v[g][1] += x.y;
+                        v[g][2] += x.z;
+                        v[g][3] += x.w;
+                        v[g][4] += y.x;
+                        v[g][5] += y.y;
+                        v[g][6] += y.z;
+                        v[g][7] += y.w;
+                    }
+                }
+            }
+            auto store_bf16 = [&](uint16_t* dst, const float* x) {
+                uint4 o;
+                o.x = dt::bf16x2_from_f32(x[0], x[1]);
+                o.y = dt::bf16x2_from_f32(x[2], x[3]);
+                o.z = dt::bf16x2_from_f32(x[4], x[5]);
+                o.w = dt::bf16x2_from_f32(x[6], x[7]);
+                *reinterpret_cast<uint4*>(dst + at) = o;
+            };
+            float y[8];
+            if constexpr (GATED) {
+                if (on && e.pre) {
+                    store_bf16(e.pre, v[0]);
+                    store_bf16(e.up, v[1]);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) y[i] = mx::act(e.act, v[0][i]) * v[G - 1][i];
+            } else {
+                const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) v[0][i] += bias[i];
+                if (on && e.pre) store_bf16(e.pre, v[0]);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    y[i] = mx::act(e.act, v[0][i]);
+                    if (e.residual)
+                        y[i] += (i & 1) ? dt::bf16_hi(rw[i >> 1]) : dt::bf16_lo(rw[i >> 1]);
+                }
+            }
+            if (on && e.c) store_bf16(e.c, y);
+            if (e.q) {
+                uint32_t m = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) m = mx::amax_bits(m, y[i]);
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const uint32_t code = mx::scale_code(m, mx::emax_of(e.q_type));
+                const float inv = dt::ue8m0_inverse(code);
+                if (on)
+                    *reinterpret_cast<uint2*>(e.q + at) =
+                        make_uint2(mx::pack4(e.q_type, y[0], y[1], y[2], y[3], inv),
+                                   mx::pack4(e.q_type, y[4], y[5], y[6], y[7], inv));
+                if ((lane & 3u) == 0 && t < upto)
+                    e.sfq[mx::word_offset(tok0 + t, block, q_tiles_k) + ((tid & 15u) >> 2)] =
+                        on ? static_cast<uint8_t>(code) : 0;
+            }
+        }
+    }
+    // no CTA of the cluster leaves while another may still read its partial sums
+    if (p.split > 1) ptxstd::cluster_sync();
+}
+
+}  // namespace narrow
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+bool mx_type_ok(int t) { return t == 0 || t == 1 || t == 3 || t == 4 || t == 5; }
+
+struct Operand {
+    const uint8_t* data;
+    const uint8_t* sf;
+};
+
+int operand_maps(CUtensorMap* data, CUtensorMap* sf, Operand o, int64_t rows, int64_t K,
+                 uint32_t box_rows) {
+    const int st = ptxstd::make_tmap_2d(data, o.data, CU_TENSOR_MAP_DATA_TYPE_UINT8, K, rows, K, BK,
+                                        box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (st) return st;
+    return ptxstd::make_tmap_2d(sf, o.sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128,
+                                ((rows + 127) / 128) * ((K + 127) / 128), 512, 128, 1,
+                                CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <bool GATED>
+int launch_wide(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e, int64_t M,
+                int64_t N, int64_t K, cudaStream_t stream) {
+    using namespace wide;
+    Maps maps = {};
+    int st = operand_maps(&maps.a, &maps.sfa, a, M, K, P_HALF);
+    if (st) return st;
+    st = operand_maps(&maps.b, &maps.sfb, b, N, K, P_HALF);
+    if (st) return st;
+    if (GATED) {
+        st = operand_maps(&maps.b2, &maps.sfb2, b2, N, K, P_HALF);
+        if (st) return st;
+    }
+    if (e.c && (st = ptxstd::epi::make_store_map<kCCols>(&maps.c, e.c, M, N))) return st;
+    if (e.pre && (st = ptxstd::epi::make_store_map<kCCols>(&maps.pre, e.pre, M, N))) return st;
+    if (e.up && (st = ptxstd::epi::make_store_map<kCCols>(&maps.up, e.up, M, N))) return st;
+    if (e.q && (st = ptxstd::make_tmap_2d(&maps.q, e.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, N, M, N, 64,
+                                          ptxstd::epi::kRows, CU_TENSOR_MAP_SWIZZLE_64B)))
+        return st;
+    st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(wide_kernel<GATED>),
+                                      static_cast<int>(kSmemBytes));
+    if (st) return st;
+    uint32_t* err = ptxstd::device_error_word();
+    if (!err) return PTXSTD_ECUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static std::atomic<int> max_pairs[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return PTXSTD_ECUDA;
+    int resident = max_pairs[dev].load(std::memory_order_relaxed);
+    if (resident == 0) {
+        cfg.gridDim = dim3(2 * static_cast<uint32_t>(ptxstd::sm_count() / 2));
+        if (cudaOccupancyMaxActiveClusters(&resident, wide_kernel<GATED>, &cfg) != cudaSuccess ||
+            resident <= 0)
+            return PTXSTD_ECUDA;
+        max_pairs[dev].store(resident, std::memory_order_relaxed);
+    }
+    cfg.numAttrs = 2;
+    const int64_t tile_n = GATED ? 128 : 256;
+    const int64_t tiles = ((M + P_BM - 1) / P_BM) * ((N + tile_n - 1) / tile_n);
+    if (tiles >= (1ll << 31)) return PTXSTD_EINVAL;
+    cfg.gridDim = dim3(2 * static_cast<uint32_t>(tiles < resident ? tiles : resident));
+    if (cudaLaunchKernelEx(&cfg, wide_kernel<GATED>, maps, static_cast<uint32_t>(M),
+                           static_cast<uint32_t>(N), static_cast<uint32_t>(K),
+                           static_cast<uint32_t>(a_type), static_cast<uint32_t>(b_type), e,
+                           err) != cudaSuccess)
+        return PTXSTD_ECUDA;
+    return ptxstd::launch_status();
+}
+
+// Token columns of a narrow CTA. The accumulators (one, or two when gated) and the scale slots
+// share 512 TMEM columns, so a gated CTA takes up to 128 tokens, a linear one up to 256.
+uint32_t narrow_tokens(int64_t M, bool gated) {
+    const int64_t cap = gated ? 128 : 256;
+    const int64_t t = (M + 15) / 16 * 16;
+    return static_cast<uint32_t>(t < cap ? t : cap);
+}
+
+template <bool GATED>
+int launch_narrow(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e,
+                  int64_t M, int64_t N, int64_t K, cudaStream_t stream) {
+    using namespace narrow;
+    constexpr uint32_t G = GATED ? 2 : 1;
+    Shape p = {};
+    p.M = static_cast<uint32_t>(M);
+    p.N = static_cast<uint32_t>(N);
+    p.K = static_cast<uint32_t>(K);
+    p.tokens = narrow_tokens(M, GATED);
+    const uint32_t tok_tiles = (p.tokens + 127) / 128;
+    const uint32_t per_stage = G * kWBytes + p.tokens * BK + (G + tok_tiles) * 512;
+    // Two CTAs per SM where the ring allows it (each at most half of the SM's shared memory and
+    // 256 TMEM columns), so that one CTA's prologue and epilogue run beside the other's stream.
+    const uint32_t half_smem = 112 * 1024 - 1024, full_smem = 225 * 1024;
+    const uint32_t slot_cols = 4 * (G + tok_tiles);
+    p.stages = half_smem / per_stage;
+    const bool two = p.stages >= 2 && G * p.tokens + p.stages * slot_cols <= 256;
+    if (!two) p.stages = full_smem / per_stage;
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    const uint32_t cols = G * p.tokens + p.stages * slot_cols;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < cols) p.tmem_cols *= 2;
+    if (p.tmem_cols > 512) return PTXSTD_EINVAL;
+    if (two) p.tmem_cols = 256;
+    uint32_t smem = p.stages * per_stage + 1024;
+    const uint32_t part = G * p.tokens * 128 * 4 + 1024;
+    if (smem < part) smem = part;
+    // TMEM waits inside clusters must not be able to form a cycle, whatever else runs on the GPU
+    // (another stream's call, the next call's early start): a CTA with more than 256 columns takes
+    // all of its SM's shared memory, the others at least a third plus, so that two is the most
+    // an SM holds and their TMEM always fits.
+    if (p.tmem_cols > 256) smem = full_smem + 1024;
+    else if (smem < 78 * 1024) smem = 78 * 1024;
+
+    // K slices: the split that fills the resident CTA slots best, counting a fixed cost of a few
+    // stages for each CTA's start and end.
+    const int64_t blocks = (N + 127) / 128, ytiles = (M + p.tokens - 1) / p.tokens;
+    const int64_t num_k = (K + BK - 1) / BK;
+    const int64_t slots = static_cast<int64_t>(ptxstd::sm_count()) * (two ? 2 : 1);
+    double best = 0;
+    for (uint32_t s = 1; s <= kMaxCluster; s *= 2) {
+        if (s > 1 && num_k < 2 * s) break;
+        const int64_t ctas = blocks * ytiles * s;
+        const int64_t waves = (ctas + slots - 1) / slots;
+        const double cost = static_cast<double>(waves) *
+                            (static_cast<double>((num_k + s - 1) / s) + 6.0);
+        if (s == 1 || cost < best) {
+            best = cost;
+            p.split = s;
+        }
+    }
+
+    Maps maps = {};
+    int st = operand_maps(&maps.x, &maps.sfx, a, M, K, p.tokens);
+    if (st) return st;
+    st = operand_maps(&maps.w, &maps.sfw, b, N, K, 128);
+    if (st) return st;
+    if (GATED) {
+        st = operand_maps(&maps.w2, &maps.sfw2, b2, N, K, 128);
+        if (st) return st;
+    }
+    st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(narrow_kernel<GATED>),
+                                      227 * 1024 - 1024);
+    if (st) return st;
+    uint32_t* err = ptxstd::device_error_word();
+    if (!err) return PTXSTD_ECUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<uint32_t>(blocks * p.split), static_cast<uint32_t>(ytiles));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, narrow_kernel<GATED>, maps, p, static_cast<uint32_t>(b_type),
+                           static_cast<uint32_t>(a_type), e, err) != cudaSuccess)
+        return PTXSTD_ECUDA;
+    return ptxstd::launch_status();
+}
+
+// Rows up to which the narrow kernel runs: its 256 token columns read every weight once, while a
+// 256-row tile of the wide kernel would be padding for the most part.
+constexpr int64_t kNarrowRows = 256;
+
+template <bool GATED>
+int dispatch(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e, int64_t M,
+             int64_t N, int64_t K, cudaStream_t stream) {
+    if (M <= kNarrowRows)
+        return launch_narrow<GATED>(a, a_type, b, b2, b_type, e, M, N, K, stream);
+    return launch_wide<GATED>(a, a_type, b, b2, b_type, e, M, N, K, stream);
+}
+
+bool bad(const void* p) { return !p || !ptxstd::aligned16(p); }
+bool bad_or_null(const void* p) { return p && !ptxstd::aligned16(p); }
+
+int check_common(int a_type, int b_type, int act, int out_type, const Epi& e, int64_t M, int64_t N,
+                 int64_t K) {
+    if (!mx_type_ok(a_type) || !mx_type_ok(b_type)) return PTXSTD_EINVAL;
+    if (act < PTXSTD_ACT_NONE || act > PTXSTD_ACT_GELU_TANH) return PTXSTD_EINVAL;
+    if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 32) return PTXSTD_EINVAL;
+    if (M >= (1ll << 31) || N >= (1ll << 31) || K >= (1ll << 31)) return PTXSTD_EINVAL;
+    if (!e.c && !e.q) return PTXSTD_EINVAL;
+    if (bad_or_null(e.c) || bad_or_null(e.pre) || bad_or_null(e.up) || bad_or_null(e.bias) ||
+        bad_or_null(e.residual) || bad_or_null(e.q))
+        return PTXSTD_EINVAL;
+    if (e.q && (bad(e.sfq) || N % 32 || (out_type != PTXSTD_MX_E4M3 && out_type != PTXSTD_MX_E5M2)))
+        return PTXSTD_EINVAL;
+    return PTXSTD_OK;
+}
+
+}  // namespace
+
+extern "C" int ptxstd_gemm_mx_epilogue(const uint8_t* d_a, int a_type, const uint8_t* d_sfa,
+                                       const uint8_t* d_b, int b_type, const uint8_t* d_sfb,
+                                       const uint16_t* d_bias, int act, const uint16_t* d_residual,
+                                       uint16_t* d_c, uint16_t* d_pre, int out_type, uint8_t* d_q,
+                                       uint8_t* d_sfq, int64_t M, int64_t N, int64_t K,
+                                       ptxstd_stream stream) {
+    Epi e = {};
+    e.bias = d_bias;
+    e.residual = d_residual;
+    e.c = d_c;
+    e.pre = d_pre;
+    e.q = d_q;
+    e.sfq = d_sfq;
+    e.q_type = static_cast<uint32_t>(out_type);
+    e.act = static_cast<uint32_t>(act);
+    const int st = check_common(a_type, b_type, act, out_type, e, M, N, K);
+    if (st) return st;
+    if (bad(d_a) || bad(d_sfa) || bad(d_b) || bad(d_sfb)) return PTXSTD_EINVAL;
+    return dispatch<false>({d_a, d_sfa}, a_type, {d_b, d_sfb}, {nullptr, nullptr}, b_type, e, M, N,
+                           K, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ptxstd_gemm_mx_gated(const uint8_t* d_a, int a_type, const uint8_t* d_sfa,
+                                    const uint8_t* d_wg, const uint8_t* d_sfg, const uint8_t* d_wu,
+                                    const uint8_t* d_sfu, int w_type, int act, uint16_t* d_h,
+                                    uint16_t* d_gate, uint16_t* d_up, int out_type, uint8_t* d_q,
+                                    uint8_t* d_sfq, int64_t M, int64_t F, int64_t K,
+                                    ptxstd_stream stream) {
+    Epi e = {};
+    e.c = d_h;
+    e.pre = d_gate;
+    e.up = d_up;
+    e.q = d_q;
+    e.sfq = d_sfq;
+    e.q_type = static_cast<uint32_t>(out_type);
+    e.act = static_cast<uint32_t>(act);
+    const int st = check_common(a_type, w_type, act, out_type, e, M, F, K);
+    if (st) return st;
+    if (bad(d_a) || bad(d_sfa) || bad(d_wg) || bad(d_sfg) || bad(d_wu) || bad(d_sfu))
+        return PTXSTD_EINVAL;
+    if ((d_gate == nullptr) != (d_up == nullptr)) return PTXSTD_EINVAL;
+    return dispatch<true>({d_a, d_sfa}, a_type, {d_wg, d_sfg}, {d_wu, d_sfu}, w_type, e, M, F, K,
+                          static_cast<cudaStream_t>(stream));
+}

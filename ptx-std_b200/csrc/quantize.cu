@@ -62,7 +62,7 @@ enum : uint32_t { kDetailProducer = 0x2100, kDetailConsumer = 0x2200 };
 // scale of row r, column s sits at (r % 32) * 16 + ((r / 32) % 4) * 4 + s % 4, which is the
 // 32-lane x 16-byte source of one tcgen05.cp.32x128b.warpx4 (src/tcgen05/copy.rs:29-30).
 __device__ __forceinline__ size_t blocked_sf_offset(size_t r, size_t s, size_t sf_cols) {
-    const size_t tile = (r >> 7) * (sf_cols >> 2) + (s >> 2);
+    const size_t tile = (r >> 7) * ((sf_cols + 3) >> 2) + (s >> 2);
     return tile * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (s & 3);
 }
 
@@ -400,6 +400,8 @@ int launch_mx(const uint16_t* x, size_t n, uint8_t* q, uint8_t* sf, size_t sf_co
     return launch<DefaultCfg>(x, n, MxAny<false, T>{0.0f}, q, sf, sf_cols, s);
 }
 
+bool mx_type_ok(int t) { return t == 0 || t == 1 || t == 3 || t == 4 || t == 5; }
+
 }  // namespace
 
 extern "C" {
@@ -409,11 +411,18 @@ int ptxstd_quantize_mx(const uint16_t* d_x, int64_t rows, int64_t cols, int elem
     if (rows <= 0 || cols <= 0 || cols % 32 != 0) return PTXSTD_EINVAL;
     if (!d_x || !d_q || !d_sf || !ptxstd::aligned16(d_x) || !ptxstd::aligned16(d_q))
         return PTXSTD_EINVAL;
-    if (sf_layout != 0 && sf_layout != 1) return PTXSTD_EINVAL;
+    if (sf_layout < 0 || sf_layout > 2) return PTXSTD_EINVAL;
+    if (!mx_type_ok(elem_type)) return PTXSTD_EINVAL;
     if (sf_layout == 1 && (rows % 128 != 0 || cols % 128 != 0)) return PTXSTD_EINVAL;
     const size_t n = static_cast<size_t>(rows) * static_cast<size_t>(cols);
     const size_t sf_cols = static_cast<size_t>(cols) / 32;
     auto s = static_cast<cudaStream_t>(stream);
+    if (sf_layout == 2) {  // blocked and padded: the padding is zero
+        const size_t padded = (static_cast<size_t>(rows) + 127) / 128 * ((sf_cols + 3) / 4) * 512;
+        if (padded != static_cast<size_t>(rows) * sf_cols &&
+            cudaMemsetAsync(d_sf, 0, padded, s) != cudaSuccess)
+            return PTXSTD_ECUDA;
+    }
     switch (elem_type) {
     case 0: return launch_mx<0>(d_x, n, d_q, d_sf, sf_cols, sf_layout, s);
     case 1: return launch_mx<1>(d_x, n, d_q, d_sf, sf_cols, sf_layout, s);

@@ -128,6 +128,34 @@ _SIGS = {
     "ptxstd_gemm_mxfp8_sparse": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                            C.c_int64, C.c_void_p]),
+    "ptxstd_gemm_mx_epilogue": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                          C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64,
+                                          C.c_int64, C.c_int64, C.c_void_p]),
+    "ptxstd_gemm_mx_gated": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
+                                       C.c_int64, C.c_int64, C.c_int64, C.c_void_p]),
+    "ptxstd_act_backward_mx_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int,
+        C.c_int]),
+    "ptxstd_act_backward_mx": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                         C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                         C.c_void_p]),
+    "ptxstd_quantize_mx_t": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                       C.c_void_p, C.c_void_p]),
+    "ptxstd_rmsnorm_residual": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_int64, C.c_float, C.c_void_p, C.c_float, C.c_int64,
+                                          C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                          C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
+                                          C.c_void_p]),
+    "ptxstd_rmsnorm_residual_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "ptxstd_rmsnorm_residual_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                   C.c_void_p, C.c_int64, C.c_float, C.c_int64,
+                                                   C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                                   C.c_void_p]),
     "ptxstd_gemm_decode_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
     "ptxstd_gemm_decode": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                                      C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t,
@@ -219,10 +247,15 @@ from .kernels import (MX_E2M1, MX_E2M3, MX_E3M2, MX_E4M3, MX_E5M2,  # noqa: E402
                       gemm_decode, gemm_fp8, gemm_mx, gemm_mxfp8, gemm_mxfp8_sparse, gemm_nvfp4,
                       prune_24, quantize_mx, quantize_mxfp8, quantize_nvfp4,
                       tcgen05_cp_unpack)
+from .ffn import (act_backward_mx, gemm_mx_epilogue, gemm_mx_gated,  # noqa: E402
+                  gemm_mx_gated_backward, quantize_mx_t, rmsnorm_residual,
+                  rmsnorm_residual_backward)
 
 __all__ = ["lib", "check", "PtxStdError", "status_string", "last_device_error", "data_types",
            "tcgen05", "quantize_mxfp8", "quantize_nvfp4", "quantize_mx", "gemm_fp8",
            "gemm_mxfp8", "gemm_mx", "gemm_nvfp4", "gemm_decode", "gemm_mxfp8_sparse", "prune_24",
            "tcgen05_cp_unpack", "set_gemm_schedule", "get_gemm_schedule", "SCHEDULE_PERSISTENT",
-           "SCHEDULE_DYNAMIC",
+           "SCHEDULE_DYNAMIC", "rmsnorm_residual", "rmsnorm_residual_backward",
+           "gemm_mx_epilogue", "gemm_mx_gated", "gemm_mx_gated_backward", "act_backward_mx",
+           "quantize_mx_t",
            "MX_E4M3", "MX_E5M2", "MX_E2M3", "MX_E3M2", "MX_E2M1"]

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 from . import _dev, _stream, _torch, check, lib
 
-SF_ROWMAJOR, SF_BLOCKED = 0, 1
+SF_ROWMAJOR, SF_BLOCKED, SF_PADDED = 0, 1, 2
 
 
 def quantize_mxfp8(x, sf_layout: int = SF_ROWMAJOR, out=None, stream=None, seed=None):
@@ -79,7 +79,8 @@ def _mx_type(t) -> int:
 def quantize_mx(x, elem_type, sf_layout: int = 1, out=None, stream=None):
     """bf16 [rows, cols] -> (payload [rows, cols] uint8 in the tensor-core operand layout,
     UE8M0 scales per 32) for any MX element type ("e4m3", "e5m2", "e2m3", "e3m2", "e2m1" or the
-    MX_* code). FP6 / FP4 payloads are 16-element groups padded to 16 bytes."""
+    MX_* code). FP6 / FP4 payloads are 16-element groups padded to 16 bytes. sf_layout 2 is the
+    blocked layout for any number of rows and any cols % 32 == 0, padded with zeros (flat)."""
     torch = _torch()
     if x.dtype != torch.bfloat16 or x.dim() != 2:
         raise TypeError("expected a 2-D bfloat16 tensor")
@@ -87,7 +88,11 @@ def quantize_mx(x, elem_type, sf_layout: int = 1, out=None, stream=None):
     rows, cols = x.shape
     if out is None:
         q = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
-        sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
+        if sf_layout == SF_PADDED:
+            sf = torch.empty(-(-rows // 128) * -(-cols // 128) * 512, dtype=torch.uint8,
+                             device=x.device)
+        else:
+            sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
     else:
         q, sf = out
     check(lib().ptxstd_quantize_mx(_dev(x), rows, cols, t, _dev(q), _dev(sf), sf_layout,

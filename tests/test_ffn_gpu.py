@@ -1,0 +1,627 @@
+"""The feed-forward operators on a B200 against their 64-bit restatements (ffn_ref).
+
+Every stored value is held to an interval: the rounding of (exact - d) .. (exact + d). d counts the
+f32 arithmetic only: the tensor cores' accumulation (ffn_ref.acc_bound), and 2^-19 of a value for
+the chain of at most a dozen f32 operations and fast exponentials behind it (each within 2^-22).
+"""
+
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import ffn_ref as R
+
+pytestmark = pytest.mark.gpu
+
+CHAIN = 2.0 ** -19
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _bf(g, *shape, std=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * std).to(torch.bfloat16)
+
+
+def _mx(g, rows, cols, fmt="e4m3", std=1.0):
+    import ptxstd
+    return ptxstd.quantize_mx(_bf(g, rows, cols, std=std), fmt, sf_layout=2)
+
+
+def _ok():
+    import ptxstd
+    torch.cuda.synchronize()
+    code, detail = ptxstd.last_device_error()
+    assert code == 0, (code, hex(detail))
+
+
+def _pad_nan(sf, rows, cols):
+    """The same scales with NaN codes in the padding (which operators must not let through)."""
+    sf = sf.clone()
+    at = R.sf_offsets(rows, cols // 32, sf.device).reshape(-1)
+    keep = sf[at].clone()
+    sf.fill_(255)
+    sf[at] = keep
+    return sf
+
+
+# ---- padded scales ------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 96), (129, 160), (128, 128), (300, 416)])
+def test_quantize_padded_layout(cuda, oracle, rows, cols):
+    g = _gen(rows)
+    x = _bf(g, rows, cols)
+    import ptxstd
+    for fmt, t in (("e4m3", oracle.E4M3), ("e2m1", oracle.E2M1)):
+        q, sf = ptxstd.quantize_mx(x, fmt, sf_layout=2)
+        oq, osf = oracle.quantize_mx(x.view(torch.int16).cpu().numpy().view(np.uint16), t)
+        code, rest = R.sf_rowmajor(sf, rows, cols // 32)
+        assert np.array_equal(q.cpu().numpy(), oq) and np.array_equal(code.cpu().numpy(), osf)
+        assert not rest.any()
+
+
+# ---- GEMM with an epilogue ----------------------------------------------------------------------
+def _linear_case(M, N, K, act="none", bias=False, residual=False, out=None, at="e4m3", bt="e4m3",
+                 pre=False, seed=0):
+    import ptxstd
+    g = _gen(seed + M + 3 * N + 7 * K)
+    a, sfa = _mx(g, M, K, at)
+    b, sfb = _mx(g, N, K, bt, std=K ** -0.5)
+    sfa, sfb = _pad_nan(sfa, M, K), _pad_nan(sfb, N, K)
+    bi = _bf(g, N) if bias else None
+    re = _bf(g, M, N, std=4.0) if residual else None
+    r = ptxstd.gemm_mx_epilogue(a, at, sfa, b, bt, sfb, bias=bi, act=act, residual=re,
+                                elem_type=out, save_pre=pre)
+    _ok()
+    ref, mag = R.gemm(R.dequant(a, sfa, at), R.dequant(b, sfb, bt))
+    d = R.acc_bound(mag, K)
+    if bias:
+        ref, d = ref + bi.double(), d + CHAIN * bi.double().abs()
+    if pre:
+        r, p = r
+        R.check_bf16(p, ref, d + CHAIN * ref.abs(), "pre")
+    # every activation here is at most 1.13-Lipschitz; |act(x)| <= |x|
+    v = R.act(ref, act)
+    d = 1.13 * d + CHAIN * ref.abs()
+    if residual:
+        v, d = v + re.double(), d + CHAIN * re.double().abs()
+    if out is None:
+        R.check_bf16(r, v, d, "c")
+    else:
+        R.check_mx(*r, v, d, out, what="c")
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 64, 65, 127, 128, 129, 200, 255, 256, 257, 511])
+@pytest.mark.parametrize("N,K", [(8, 32), (136, 416), (384, 1056)])
+def test_linear_sizes(cuda, M, N, K):
+    _linear_case(M, N, K, bias=True, residual=True)
+
+
+@pytest.mark.parametrize("M", [3, 130, 700])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_linear_activations(cuda, M, act):
+    _linear_case(M, 288, 512, act=act, bias=True, pre=True)
+    _linear_case(M, 288, 512, act=act, bias=True, residual=True, out="e4m3", pre=True)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 32, 64), (33, 160, 96), (129, 4128, 2080), (256, 96, 4096),
+                                   (300, 32, 160), (513, 1184, 1504)])
+@pytest.mark.parametrize("out", ["e4m3", "e5m2"])
+def test_linear_mx_result(cuda, M, N, K, out):
+    _linear_case(M, N, K, out=out, at="e5m2", residual=True)
+
+
+@pytest.mark.parametrize("M", [7, 290])
+@pytest.mark.parametrize("at,bt", [("e5m2", "e4m3"), ("e2m3", "e3m2"), ("e2m1", "e4m3"),
+                                   ("e4m3", "e2m1")])
+def test_linear_element_types(cuda, oracle, M, at, bt):
+    """Every kind of payload, held to the oracle's f64 product of the decoded operands."""
+    import ptxstd
+    N, K = 72, 160
+    g = _gen(M)
+    T = {"e4m3": oracle.E4M3, "e5m2": oracle.E5M2, "e2m3": oracle.E2M3, "e3m2": oracle.E3M2,
+         "e2m1": oracle.E2M1}
+    xa, xb = _bf(g, M, K), _bf(g, N, K)
+    a, sfa = ptxstd.quantize_mx(xa, at, sf_layout=2)
+    b, sfb = ptxstd.quantize_mx(xb, bt, sf_layout=2)
+    c = ptxstd.gemm_mx_epilogue(a, at, sfa, b, bt, sfb)
+    _ok()
+    np16 = lambda t: t.view(torch.int16).cpu().numpy().view(np.uint16)  # noqa: E731
+    oa, osa = oracle.quantize_mx(np16(xa), T[at])
+    ob, osb = oracle.quantize_mx(np16(xb), T[bt])
+    r, col = np.meshgrid(np.arange(M), np.arange(N), indexing="ij")
+    ref, mag = oracle.gemm_mx_ref(oa, T[at], osa, ob, T[bt], osb, r.ravel(), col.ravel())
+    ref, mag = (torch.from_numpy(np.asarray(v, dtype=np.float64)).view(M, N) for v in (ref, mag))
+    R.check_bf16(c.cpu(), ref, R.acc_bound(mag, K))
+
+
+@pytest.mark.parametrize("M", [4, 300])
+def test_linear_both_results_and_residual_in_place(cuda, M):
+    """d_c and d_q of one call agree; the residual may be the output; guard bytes stay."""
+    import ptxstd
+    N, K = 160, 224
+    g = _gen(M)
+    a, sfa = _mx(g, M, K)
+    b, sfb = _mx(g, N, K, std=K ** -0.5)
+    res = _bf(g, M, N)
+    want = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb, residual=res)
+    wq, wsf = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb, residual=res,
+                                      elem_type="e4m3")
+    guard = 4096
+    c = torch.full((M * N + guard,), 7.0, dtype=torch.bfloat16, device="cuda")
+    c[:M * N] = res.reshape(-1)
+    q = torch.full((M * N + guard,), 77, dtype=torch.uint8, device="cuda")
+    sf = torch.full((wsf.numel() + guard,), 77, dtype=torch.uint8, device="cuda")
+    L = ptxstd.lib()
+    st = L.ptxstd_gemm_mx_epilogue(a.data_ptr(), 0, sfa.data_ptr(), b.data_ptr(), 0, sfb.data_ptr(),
+                                   None, 0, c.data_ptr(), c.data_ptr(), None, 0, q.data_ptr(),
+                                   sf.data_ptr(), M, N, K, torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    _ok()
+    assert torch.equal(c[:M * N].view(M, N), want) and (c[M * N:] == 7).all()
+    assert torch.equal(q[:M * N].view(M, N), wq) and (q[M * N:] == 77).all()
+    assert torch.equal(sf[:wsf.numel()], wsf) and (sf[wsf.numel():] == 77).all()
+
+
+@pytest.mark.parametrize("M", [20, 400])
+def test_nan_and_infinity_stay_in_their_row(cuda, M):
+    """A NaN scale in one row of A reaches that row of the result only, in bf16 and as MX codes
+    (scale 255, elements NaN); infinite biases give infinite columns."""
+    import ptxstd
+    N, K = 96, 256
+    g = _gen(3)
+    a, sfa = _mx(g, M, K)
+    b, sfb = _mx(g, N, K)
+    clean = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb)
+    bad = sfa.clone()
+    bad[R.sf_offsets(M, K // 32)[13, 5]] = 255
+    c = ptxstd.gemm_mx_epilogue(a, "e4m3", bad, b, "e4m3", sfb)
+    q, sf = ptxstd.gemm_mx_epilogue(a, "e4m3", bad, b, "e4m3", sfb, elem_type="e4m3")
+    bias = torch.zeros(N, dtype=torch.bfloat16, device="cuda")
+    bias[5] = -math.inf
+    ci = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb, bias=bias)
+    _ok()
+    rows = torch.arange(M, device="cuda") != 13
+    assert c[13].isnan().all() and torch.equal(c[rows], clean[rows])
+    code, rest = R.sf_rowmajor(sf, M, N // 32)
+    assert (code[13] == 255).all() and (code[rows] != 255).all() and not rest.any()
+    assert ((q[13] & 127) == 127).all()
+    cols = torch.arange(N, device="cuda") != 5
+    assert (ci[:, 5] == -math.inf).all() and torch.equal(ci[:, cols], clean[:, cols])
+
+
+def test_linear_long_k(cuda):
+    """The down projection of one token and of a few (a long K, split over a cluster)."""
+    _linear_case(1, 1024, 28672, residual=True)
+    _linear_case(16, 264, 28672 - 32, bias=True)
+
+
+# ---- gated projection ---------------------------------------------------------------------------
+def _gated_case(M, F, K, act="silu", out=None, save=False, seed=0):
+    import ptxstd
+    g = _gen(seed + M + 3 * F + 7 * K)
+    a, sfa = _mx(g, M, K)
+    wg, sfg = _mx(g, F, K, std=K ** -0.5)
+    wu, sfu = _mx(g, F, K, std=K ** -0.5)
+    sfa, sfg, sfu = _pad_nan(sfa, M, K), _pad_nan(sfg, F, K), _pad_nan(sfu, F, K)
+    r = ptxstd.gemm_mx_gated(a, "e4m3", sfa, wg, sfg, wu, sfu, "e4m3", act=act, elem_type=out,
+                             save=save)
+    _ok()
+    av = R.dequant(a, sfa, "e4m3")
+    gate, gm = R.gemm(av, R.dequant(wg, sfg, "e4m3"))
+    up, um = R.gemm(av, R.dequant(wu, sfu, "e4m3"))
+    dg, du = R.acc_bound(gm, K), R.acc_bound(um, K)
+    if save:
+        r, (sg, su) = r
+        R.check_bf16(sg, gate, dg, "gate")
+        R.check_bf16(su, up, du, "up")
+    f = R.act(gate, act)
+    df = 1.13 * dg + CHAIN * gate.abs()
+    d = f.abs() * du + up.abs() * df + df * du + CHAIN * (f * up).abs()
+    if out is None:
+        R.check_bf16(r, f * up, d, "h")
+    else:
+        R.check_mx(*r, f * up, d, out, what="h")
+
+
+@pytest.mark.parametrize("M", [1, 16, 31, 100, 128, 129, 250, 256, 257, 600])
+@pytest.mark.parametrize("F,K", [(32, 32), (160, 224), (416, 1056)])
+def test_gated_sizes(cuda, M, F, K):
+    _gated_case(M, F, K, save=True)
+    _gated_case(M, F, K, out="e4m3", save=M % 2 == 0)
+
+
+@pytest.mark.parametrize("M", [9, 300])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh"])
+def test_gated_activations(cuda, M, act):
+    _gated_case(M, 128, 256, act=act)
+    _gated_case(M, 128, 256, act=act, out="e5m2")
+
+
+@pytest.mark.parametrize("M", [6, 270])
+def test_gated_features_of_eight(cuda, M):
+    _gated_case(M, 8, 64)
+    _gated_case(M, 200, 96, save=True)
+
+
+# ---- gradient of the activation, transposing quantiser ------------------------------------------
+def _t(v):
+    rows, cols = v.shape
+    out = torch.zeros((cols, -(-rows // 32) * 32), dtype=v.dtype, device=v.device)
+    out[:, :rows] = v.t()
+    return out
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (31, 64), (32, 96), (129, 160), (300, 416),
+                                       (128, 2080)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_act_backward(cuda, rows, cols, gated, fmt):
+    import ptxstd
+    g = _gen(rows + cols)
+    for act in ("silu", "gelu", "gelu_tanh", "relu", "none"):
+        dh, gate = _bf(g, rows, cols, std=0.1), _bf(g, rows, cols, std=2.0)
+        up = _bf(g, rows, cols) if gated else None
+        row, col, db = ptxstd.act_backward_mx(dh, gate, up, act=act, elem_type=fmt, bias_grad=True)
+        row2, col2 = ptxstd.act_backward_mx(dh, gate, up, act=act, elem_type=fmt)
+        _ok()
+        x = gate.double()
+        df = torch.ones_like(x) if act == "none" else R.act_grad(x, act)
+        d = dh.double() * df
+        # f' is a sum of terms up to 1.2 in size, each within CHAIN
+        e = 4 * CHAIN * dh.double().abs()
+        if gated:
+            u, f = up.double(), dh.double() * R.act(x, act)
+            d, e = torch.cat([d * u, f], 1), torch.cat([e * u.abs(), e * x.abs()], 1)
+        R.check_mx(*row, d, e, fmt, what=f"{act} rows")
+        R.check_mx(*col, _t(d), _t(e), fmt, what=f"{act} columns")
+        lim = e.sum(0) + d.abs().sum(0) * 2.0 ** -18
+        assert ((db.double() - d.sum(0)).abs() <= lim).all()
+        for p, q in zip(row + col, row2 + col2):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 8), (32, 32), (33, 72), (200, 264), (1000, 136)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_quantize_transposed(cuda, rows, cols, fmt):
+    """Bit-exact: bf16 values times powers of two have one rounding."""
+    import ptxstd
+    x = _bf(_gen(rows), rows, cols, std=3.0)
+    x[0, 0] = 0
+    qt, sft = ptxstd.quantize_mx_t(x, fmt)
+    _ok()
+    R.check_mx(qt, sft, _t(x.double()), 0.0, fmt)
+    if rows % 32 == 0:
+        q, sf = ptxstd.quantize_mx(x.t().contiguous(), fmt, sf_layout=2)
+        assert torch.equal(q, qt) and torch.equal(sf, sft)
+
+
+def test_activation_extremes(cuda):
+    """Saturated, tiny and infinite pre-activations: no NaN where the limit is finite."""
+    import ptxstd
+    v = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 30.0, -30.0, 90.0, -90.0, 1e4, -1e4, 1e20, -1e20,
+                      3e38, -3e38] + [0.5] * 18, device="cuda").to(torch.bfloat16)
+    gate = v.repeat(4, 1)
+    dh = torch.ones_like(gate)
+    for act in ("relu", "silu", "gelu", "gelu_tanh"):
+        (q, sf), _ = ptxstd.act_backward_mx(dh, gate, act=act, elem_type="e4m3")
+        _ok()
+        got = R.dequant(q, sf, "e4m3")
+        want = torch.where(gate.double() > 20, 1.0, 0.0)
+        big = gate.double().abs() > 20
+        assert torch.equal(got[big], want[big]), act
+        assert got.isfinite().all()
+
+
+# ---- norms --------------------------------------------------------------------------------------
+def _norm_inputs(rows, cols, post, gate, seed=0):
+    g = _gen(seed + rows + cols)
+    x, y = _bf(g, rows, cols, std=2.0), _bf(g, rows, cols, std=0.7)
+    x[:, ::17] *= 8
+    w = (1 + 0.2 * torch.randn(cols, generator=g, device="cuda")).to(torch.bfloat16)
+    wp = (1 + 0.2 * torch.randn(cols, generator=g, device="cuda")).to(torch.bfloat16) if post \
+        else None
+    gt = {"none": None, "vector": _bf(g, cols), "row": _bf(g, rows, cols)}[gate]
+    return g, x, y, w, wp, gt
+
+
+def _d(t):
+    return None if t is None else t.double()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 8192), (3, 256), (5, 480), (130, 1024),
+                                       (7, 1056), (300, 2080), (2, 16384 + 32), (2, 32768)])
+@pytest.mark.parametrize("post,gate", [(False, "none"), (True, "vector"), (True, "row"),
+                                       (False, "vector")])
+def test_norm_forward(cuda, rows, cols, post, gate):
+    import ptxstd
+    _, x, y, w, wp, gt = _norm_inputs(rows, cols, post, gate)
+    eps, s = 1e-5, 0.5
+    for fmt, layout in ((None, 1), ("e4m3", 1), ("e5m2", 0)):
+        xo, n, (r, rp) = ptxstd.rmsnorm_residual(x, w, y=y, w_post=wp, gate=gt, scale=s, eps=eps,
+                                                 elem_type=fmt, sf_layout=layout)
+        _ok()
+        ref, mag, ry = R.norm_forward(_d(x), _d(y), _d(wp), _d(gt), s, eps)
+        R.check_bf16(xo, ref, CHAIN * mag, "x'")
+        ref, rx = R.norm_result(xo.double(), _d(w), eps)
+        assert ((r.double() - rx).abs() <= CHAIN * rx).all()
+        assert (rp is None) == (not post)
+        if post:
+            assert ((rp.double() - ry).abs() <= CHAIN * ry).all()
+        if fmt is None:
+            R.check_bf16(n, ref, CHAIN * ref.abs(), "n")
+        else:
+            R.check_mx(*n, ref, CHAIN * ref.abs(), fmt, padded=layout == 1, what="n")
+
+
+def test_norm_without_branch(cuda):
+    """No y: x' is x; columns that are not a multiple of 32 in bf16; a zero row stays zero."""
+    import ptxstd
+    _, x, _, w, _, _ = _norm_inputs(70, 40, False, "none")
+    x[3] = 0
+    xo, n, (r, rp) = ptxstd.rmsnorm_residual(x, w, eps=1e-6)
+    _ok()
+    assert xo is x and rp is None and not n[3].any() and float(r[3]) == pytest.approx(1e3, rel=1e-5)
+    R.check_bf16(n, R.norm_result(_d(x), _d(w), 1e-6)[0], CHAIN * 200.0, "n")
+    with pytest.raises(ptxstd.PtxStdError):
+        ptxstd.rmsnorm_residual(x, w, elem_type="e4m3")  # 40 % 32
+    # NaN stays in its row
+    x[5, 7] = math.nan
+    n2 = ptxstd.rmsnorm_residual(x, w, eps=1e-6)[1]
+    keep = torch.arange(70, device="cuda") != 5
+    assert n2[5].isnan().all() and torch.equal(n2[keep], n[keep])
+
+
+def test_norm_in_place(cuda):
+    """x' may be written over x (C ABI)."""
+    import ptxstd
+    _, x, y, w, wp, gt = _norm_inputs(9, 512, True, "vector")
+    want = ptxstd.rmsnorm_residual(x, w, y=y, w_post=wp, gate=gt, scale=2.0)
+    n = torch.empty_like(x)
+    st = ptxstd.lib().ptxstd_rmsnorm_residual(
+        x.data_ptr(), y.data_ptr(), wp.data_ptr(), gt.data_ptr(), 1, 2.0, w.data_ptr(), 1e-6, 9,
+        512, x.data_ptr(), n.data_ptr(), 0, None, None, 1, None, None,
+        torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    _ok()
+    assert torch.equal(x, want[0]) and torch.equal(n, want[1])
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (2, 40), (5, 480), (300, 1056), (1200, 256),
+                                       (9, 4096 + 32), (160, 8192), (5, 8192 + 32), (3, 16384)])
+@pytest.mark.parametrize("post,gate,du", [(False, "none", True), (True, "vector", True),
+                                          (True, "row", False), (False, "row", True)])
+def test_norm_backward(cuda, rows, cols, post, gate, du):
+    import ptxstd
+    g, xo, y, w, wp, gt = _norm_inputs(rows, cols, post, gate)
+    dn = _bf(g, rows, cols, std=0.3)
+    dxo = _bf(g, rows, cols, std=0.3) if du else None
+    rx = torch.rsqrt(xo.double().square().mean(1) + 1e-6).float()
+    ry = torch.rsqrt(y.double().square().mean(1) + 1e-6).float() if post else None
+    dx, dw, dy, dwp, dg = ptxstd.rmsnorm_residual_backward(
+        dn, xo, w, (rx, ry), dx_out=dxo, y=y, w_post=wp, gate=gt, scale=0.5)
+    again = ptxstd.rmsnorm_residual_backward(
+        dn, xo, w, (rx, ry), dx_out=dxo, y=y, w_post=wp, gate=gt, scale=0.5)
+    _ok()
+    ref = R.norm_backward(_d(dn), _d(dxo), _d(xo), _d(w), _d(rx), _d(y), _d(wp), _d(ry), _d(gt),
+                          0.5)
+    # the f32 sums over a row add at most 32 terms per thread, then over at most 512 threads in a
+    # tree: 41 roundings of 2^-24, under CHAIN of the terms' magnitudes; column sums over at most
+    # rows / CTAs + CTAs / 8 + 8 terms, 2^-24 each
+    R.check_bf16(dx, ref["dx"][0], CHAIN * ref["dx"][1], "dx")
+    R.check_bf16(dy, ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
+    terms = CHAIN + (rows / 148 + 200) * 2.0 ** -24
+    for name, got in (("dw", dw), ("dw_post", dwp)):
+        if got is None:
+            assert name not in ref
+            continue
+        assert got.dtype == torch.float32
+        assert ((got.double() - ref[name][0]).abs() <= 4 * terms * ref[name][1]).all(), name
+    if gate == "vector":
+        assert dg.dtype == torch.float32
+        assert ((dg.double() - ref["dgate"][0]).abs() <= 4 * terms * ref["dgate"][1]).all()
+    elif gate == "row":
+        if rows == 1:  # through the column sum, then rounded
+            ref["dgate"] = (ref["dgate"][0].view(1, -1), ref["dgate"][1].view(1, -1))
+        R.check_bf16(dg, ref["dgate"][0], 4 * CHAIN * ref["dgate"][1], "dgate")
+    else:
+        assert dg is None
+    for p, q in zip((dx, dw, dy, dwp, dg), again):
+        assert p is q is None or torch.equal(p, q)
+
+
+def test_norm_gradient_against_differences(cuda):
+    """The kernels' gradients along a direction against the central difference of the 64-bit
+    forward pass: they differ by the gradients' bf16 rounding, 2^-8 of each entry."""
+    import ptxstd
+    rows, cols, s, eps = 4, 512, 0.5, 1e-6
+    g, x, y, w, wp, gt = _norm_inputs(rows, cols, True, "vector")
+    dn, du = _bf(g, rows, cols, std=0.3), _bf(g, rows, cols, std=0.3)
+    # the stored x' is the point of expansion, so start from an x for which x' needs no rounding
+    p, _, ry = R.norm_forward(torch.zeros_like(_d(x)), _d(y), _d(wp), _d(gt), s, eps)
+    xo = x
+    x64 = _d(xo) - p
+    rx = R.norm_result(_d(xo), _d(w), eps)[1]
+    got = ptxstd.rmsnorm_residual_backward(dn, xo, w, (rx.float(), ry.float()), dx_out=du, y=y,
+                                           w_post=wp, gate=gt, scale=s)
+    args = [x64, _d(w), _d(y), _d(wp), _d(gt)]
+
+    def loss(x, w, y, wp, gt):
+        o = R.norm_forward(x, y, wp, gt, s, eps)[0]
+        return (R.norm_result(o, w, eps)[0] * _d(dn)).sum() + (o * _d(du)).sum()
+
+    for k in range(5):
+        v = torch.randn(args[k].shape, generator=g, device="cuda", dtype=torch.float64)
+        h = 1e-6
+        up, down = list(args), list(args)
+        up[k], down[k] = args[k] + h * v, args[k] - h * v
+        d = float(loss(*up) - loss(*down)) / (2 * h)
+        e = float((got[k].double() * v).sum())
+        assert abs(d - e) <= 2.0 ** -8 * float((got[k].double() * v).abs().sum()) + 1e-4 * abs(d)
+
+
+# ---- together -----------------------------------------------------------------------------------
+class Block:
+    """norm -> gated projection -> down projection onto the residual stream, and its backward."""
+
+    def __init__(self, M, D, F, seed=1):
+        import ptxstd
+        g = _gen(seed)
+        self.P, self.M, self.D, self.F = ptxstd, M, D, F
+        self.x, self.y = _bf(g, M, D, std=2.0), _bf(g, M, D)
+        self.w, self.wp, self.gate = _bf(g, D), _bf(g, D), _bf(g, D)
+        self.wg = _bf(g, F, D, std=D ** -0.5)
+        self.wu = _bf(g, F, D, std=D ** -0.5)
+        self.wd = _bf(g, D, F, std=F ** -0.5)
+        q = lambda t: ptxstd.quantize_mx(t, "e4m3", sf_layout=2)  # noqa: E731
+        self.qg, self.qu, self.qd = q(self.wg), q(self.wu), q(self.wd)
+        self.gut = q(torch.cat([self.wg, self.wu]).t().contiguous())
+        self.dt = q(self.wd.t().contiguous())
+        self.dout = _bf(g, M, D, std=0.1)
+
+    def forward(self):
+        P = self.P
+        xo, n, st = P.rmsnorm_residual(self.x, self.w, y=self.y, w_post=self.wp, gate=self.gate,
+                                       scale=0.5, elem_type="e4m3")
+        h, (g, u) = P.gemm_mx_gated(n[0], "e4m3", n[1], self.qg[0], self.qg[1], self.qu[0],
+                                    self.qu[1], "e4m3", elem_type="e4m3", save=True)
+        out = P.gemm_mx_epilogue(h[0], "e4m3", h[1], self.qd[0], "e4m3", self.qd[1], residual=xo)
+        return xo, n, st, h, g, u, out
+
+    def backward(self, xo, n, st, h, g, u, out):
+        P = self.P
+        dq, dsf = P.quantize_mx(self.dout, "e5m2", sf_layout=2)
+        dh = P.gemm_mx_epilogue(dq, "e5m2", dsf, self.dt[0], "e4m3", self.dt[1])
+        nb = P.rmsnorm_residual(xo, self.w)[1]
+        nt, sfnt = P.quantize_mx_t(nb, "e4m3")
+        dn, dw = P.gemm_mx_gated_backward(dh, g, u, nt, "e4m3", sfnt, self.gut[0], "e4m3",
+                                          self.gut[1])
+        return (dh, dn, dw) + P.rmsnorm_residual_backward(
+            dn, xo, self.w, st, dx_out=self.dout, y=self.y, w_post=self.wp, gate=self.gate,
+            scale=0.5)
+
+
+def _flat(v):
+    return [t for x in v for t in (_flat(x) if isinstance(x, (tuple, list)) else [x])
+            if t is not None]
+
+
+@pytest.mark.parametrize("M", [1, 40, 333])
+def test_block_stage_by_stage(cuda, M):
+    """A whole feed-forward block forward and backward, launched without a wait in between; every
+    stage is then held to its restatement on the stage's own stored inputs."""
+    b = Block(M, 256, 416)
+    f = b.forward()
+    xo, n, st, h, g, u, out = f
+    dh, dn, dw, dx, dnw, dy, dwp, dgate = b.backward(*f)
+    _ok()
+    D, F = b.D, b.F
+    a = R.dequant(*n, "e4m3")
+    gate, gm = R.gemm(a, R.dequant(*b.qg, "e4m3"))
+    R.check_bf16(g, gate, R.acc_bound(gm, D), "gate")
+    c, cm = R.gemm(R.dequant(*h, "e4m3"), R.dequant(*b.qd, "e4m3"))
+    R.check_bf16(out, c + _d(xo), R.acc_bound(cm, F) + CHAIN * _d(xo).abs(), "out")
+    # backward: the quantised gradient follows from the stored dh, gate, up
+    (q, sf), (qt, sft) = b.P.act_backward_mx(dh, g, u)
+    c, cm = R.gemm(R.dequant(q, sf, "e5m2"), R.dequant(*b.gut, "e4m3"))
+    R.check_bf16(dn, c, R.acc_bound(cm, 2 * F), "dn")
+    nt = b.P.quantize_mx_t(b.P.rmsnorm_residual(xo, b.w)[1], "e4m3")
+    c, cm = R.gemm(R.dequant(qt, sft, "e5m2"), R.dequant(*nt, "e4m3"))
+    R.check_bf16(dw, c, R.acc_bound(cm, -(-M // 32) * 32), "dw")
+    ref = R.norm_backward(_d(dn), _d(b.dout), _d(xo), _d(b.w), _d(st[0]), _d(b.y), _d(b.wp),
+                          _d(st[1]), _d(b.gate), 0.5)
+    R.check_bf16(dx, ref["dx"][0], CHAIN * ref["dx"][1], "dx")
+    R.check_bf16(dy, ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
+
+
+def test_block_gradients_follow_the_exact_ones(cuda):
+    """End to end against autograd of the unquantised block in 64 bits. A check of signs and factors,
+    not of rounding: E4M3 / E5M2 operands carry up to 2^-4 and 2^-3 of relative rounding each
+    (and 2^-3 where a block saturates), independent over the entries of each product, so the
+    gradients keep a cosine well above 0.99 to the exact ones and a norm within 5 %."""
+    b = Block(256, 256, 512, seed=5)
+    f = b.forward()
+    dh, dn, dw, dx, dnw, dy, dwp, dgate = b.backward(*f)
+    _ok()
+    v = {k: _d(getattr(b, k)).requires_grad_(True)
+         for k in ("x", "y", "w", "wp", "gate", "wg", "wu", "wd")}
+    xo = R.norm_forward(v["x"], v["y"], v["wp"], v["gate"], 0.5, 1e-6)[0]
+    n = R.norm_result(xo, v["w"], 1e-6)[0]
+    out = xo + (R.act(n @ v["wg"].t(), "silu") * (n @ v["wu"].t())) @ v["wd"].t()
+    out.backward(_d(b.dout))
+    want = {"dx": v["x"].grad, "dy": v["y"].grad, "dw": v["w"].grad, "dwp": v["wp"].grad,
+            "dgate": v["gate"].grad, "dwgu": torch.cat([v["wg"].grad, v["wu"].grad])}
+    got = {"dx": dx, "dy": dy, "dw": dnw, "dwp": dwp, "dgate": dgate, "dwgu": dw}
+    for k, w in want.items():
+        p, q = got[k].double().reshape(-1), w.reshape(-1)
+        cos = float(p @ q / (p.norm() * q.norm()))
+        assert cos > 0.99 and abs(float(p.norm() / q.norm()) - 1) < 0.05, (k, cos)
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_captured_and_replayed(cuda, M):
+    """Forward and backward captured into one CUDA graph; replays on changed inputs equal eager
+    calls on them, bit for bit."""
+    b = Block(M, 256, 416, seed=9)
+    b.backward(*b.forward())
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(graph, stream=s):
+            f = b.forward()
+            r = b.backward(*f)
+    torch.cuda.current_stream().wait_stream(s)
+    for k in range(2):
+        b.x.copy_(_bf(_gen(50 + k), M, b.D, std=2.0))
+        b.dout.copy_(_bf(_gen(60 + k), M, b.D, std=0.1))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in _flat((f, r))]
+        ef = b.forward()
+        eager = _flat((ef, b.backward(*ef)))
+        _ok()
+        for p, q in zip(replayed, eager):
+            assert torch.equal(p, q)
+
+
+def test_two_streams_at_once(cuda):
+    """Blocks of both kernels (few rows, many rows) running on two streams give the results that
+    they give alone."""
+    blocks = [Block(5, 512, 1024, seed=3), Block(300, 512, 1024, seed=4),
+              Block(140, 512, 1024, seed=6)]
+    alone = []
+    for b in blocks:
+        f = b.forward()
+        alone.append([t.clone() for t in _flat((f, b.backward(*f)))])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in blocks]
+    got = [None] * len(blocks)
+    for _ in range(5):
+        for i, (b, s) in enumerate(zip(blocks, streams)):
+            with torch.cuda.stream(s):
+                f = b.forward()
+                got[i] = _flat((f, b.backward(*f)))
+    _ok()
+    for want, have in zip(alone, got):
+        for p, q in zip(want, have):
+            assert torch.equal(p, q)
+
+
+def test_device_refusals(cuda):
+    import ptxstd
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(64, dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="CUDA"):
+        ptxstd.rmsnorm_residual(x, w)
+    with pytest.raises(ValueError, match="contiguous"):
+        ptxstd.rmsnorm_residual(torch.zeros((64, 4), dtype=torch.bfloat16, device="cuda").t(),
+                                w.cuda())
+    flat = torch.zeros(4 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ptxstd.PtxStdError):  # 2-byte offset: not 16-byte aligned
+        ptxstd.rmsnorm_residual(flat[1:257].view(4, 64), w.cuda())
+    assert C.sizeof(C.c_void_p) == 8
