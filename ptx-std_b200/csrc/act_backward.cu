@@ -55,12 +55,7 @@ __device__ __forceinline__ void put8(float* row, uint32_t l, const float (&v)[8]
 // One row block (four lanes) of D at (row, first column col of this lane's eight values).
 __device__ __forceinline__ void row_block(const Params& p, const float (&v)[8], uint32_t row,
                                           uint32_t col, bool on, bool in_tiles, uint32_t lane) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = mx::amax_bits(m, v[k]);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t code = mx::scale_code(m, mx::emax_of(p.type));
+    const uint32_t code = mx::scale_code(mx::amax_quad(mx::amax_of(v)), mx::emax_of(p.type));
     const float inv = dt::ue8m0_inverse(code);
     if (on)
         *reinterpret_cast<uint2*>(p.q + static_cast<size_t>(row) * p.W + col) =
@@ -161,15 +156,13 @@ __global__ void __launch_bounds__(kThreads)
     for (int h = 0; h < kTiles; ++h) {
         const float* src = tile + (h * kRows + 32 * b) * kCols + f;
         float v[32];
-        uint32_t m = 0;
         float sum = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < 32; ++i) {
             v[i] = src[i * kCols];
-            m = mx::amax_bits(m, v[i]);
             sum += v[i];
         }
-        const uint32_t code = mx::scale_code(m, emax);
+        const uint32_t code = mx::scale_code(mx::amax_of(v), emax);
         const float inv = dt::ue8m0_inverse(code);
         const uint32_t feature = h * p.cols + col0 + f;
         if (col0 + f < p.cols) {

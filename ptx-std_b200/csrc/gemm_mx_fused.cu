@@ -165,9 +165,10 @@ struct Out {
         const uint32_t emax = mx::emax_of(type);
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
-            uint32_t m = 0;
+            float m = 0.0f;
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) m = mx::amax_bits(m, f(r[FIRST + 32 * h + i]));
+            for (uint32_t i = 0; i < 32; i += 2)
+                m = mx::amax(m, f(r[FIRST + 32 * h + i]), f(r[FIRST + 32 * h + i + 1]));
             const uint32_t code = mx::scale_code(m, emax);
             const float inv = dt::ue8m0_inverse(code);
             if (row < M && col0 + 32 * h < N) codes |= code << (8 * h);
@@ -806,12 +807,7 @@ __global__ void __launch_bounds__(kThreads)
             }
             if (on && e.c) store_bf16(e.c, y);
             if (e.q) {
-                uint32_t m = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) m = mx::amax_bits(m, y[i]);
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const uint32_t code = mx::scale_code(m, mx::emax_of(e.q_type));
+                const uint32_t code = mx::scale_code(mx::amax_quad(mx::amax_of(y)), mx::emax_of(e.q_type));
                 const float inv = dt::ue8m0_inverse(code);
                 if (on)
                     *reinterpret_cast<uint2*>(e.q + at) =

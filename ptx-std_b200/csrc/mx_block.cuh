@@ -37,23 +37,51 @@ __host__ __device__ __forceinline__ size_t word_offset(size_t r, size_t t, size_
 // Element types an operator can write: the one-byte ones, by their F8f6f4ElementType code.
 constexpr uint32_t kE4m3 = 0, kE5m2 = 1;
 
-// |x| and |y| folded into a running block maximum of magnitude bits: for non-negative f32
-// patterns the integer order is the float order and every NaN sorts above infinity, so the
-// maximum propagates NaN as the quantisers of bf16 do.
-__device__ __forceinline__ uint32_t amax_bits(uint32_t m, float x) {
-    return max(m, __float_as_uint(x) & 0x7FFFFFFFu);
+// Running block maximum of magnitudes, NaN-propagating like the quantisers of bf16; the pair form
+// is one three-input maximum.
+__device__ __forceinline__ float amax(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
 }
-// Scale code of a block from its magnitude bits: floor-pow2 (TowardZero, SaturateFinite) minus
+__device__ __forceinline__ float amax(float m, float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x)), "f"(fabsf(y)));
+    return r;
+}
+template <uint32_t L>
+__device__ __forceinline__ float amax_of(const float (&v)[L]) {
+    float m = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < L; i += 2) m = amax(m, v[i], v[i + 1]);
+    return m;
+}
+// The maximum over the four lanes that hold a block of 32 (eight values each).
+__device__ __forceinline__ float amax_quad(float m) {
+    m = amax(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return amax(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+// Scale code of a block from its largest magnitude: floor-pow2 (TowardZero, SaturateFinite) minus
 // the format's emax (E4M3 8, E5M2 15), clamped at 0; NaN stays NaN.
-__device__ __forceinline__ uint32_t scale_code(uint32_t bits, uint32_t emax) {
-    const uint32_t u = data_types::ue8m0_from_f32<false, true>(__uint_as_float(bits));
+__device__ __forceinline__ uint32_t scale_code(float amax, uint32_t emax) {
+    const uint32_t u = data_types::ue8m0_from_f32<false, true>(amax);
     return u == 0xFFu ? 0xFFu : (u > emax ? u - emax : 0u);
+}
+// (a s, b s): one packed multiply, two IEEE products.
+__device__ __forceinline__ float2 mul2(float a, float b, float s) {
+    const uint64_t x = (static_cast<uint64_t>(__float_as_uint(b)) << 32) | __float_as_uint(a);
+    const uint64_t y = (static_cast<uint64_t>(__float_as_uint(s)) << 32) | __float_as_uint(s);
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return make_float2(__uint_as_float(static_cast<uint32_t>(r)),
+                       __uint_as_float(static_cast<uint32_t>(r >> 32)));
 }
 // Two values times 2^-(code-127) (exact but for subnormal results) as a code pair.
 template <uint32_t T>
 __device__ __forceinline__ uint32_t pack2(float a, float b, float inv) {
-    return T == kE4m3 ? data_types::e4m3x2_from_f32<false>(a * inv, b * inv)
-                      : data_types::e5m2x2_from_f32<false>(a * inv, b * inv);
+    const float2 v = mul2(a, b, inv);
+    return T == kE4m3 ? data_types::e4m3x2_from_f32<false>(v.x, v.y)
+                      : data_types::e5m2x2_from_f32<false>(v.x, v.y);
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t type, float a, float b, float c, float d,
                                           float inv) {
@@ -65,17 +93,44 @@ __host__ __device__ __forceinline__ uint32_t emax_of(uint32_t type) {
 }
 
 // ---- activations ------------------------------------------------------------------------------
-// sigmoid with the fast exponential and divide (each within a few ulp of f32; every caller rounds
-// the result to bf16 or to an 8-bit float). z -> -inf gives 0 through 1 / inf.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// Hardware reciprocal (1 ulp): 1 / inf is 0.
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// sigmoid with the fast exponential and reciprocal (each within a few ulp of f32; every caller
+// rounds the result to bf16 or to an 8-bit float). z -> -inf gives 0 through 1 / inf.
+__device__ __forceinline__ float sigmoid(float z) { return rcp(1.0f + __expf(-z)); }
 
-// 2 sqrt(2 / pi) and its product with 3 * 0.044715: gelu_tanh(x) = x sigmoid(kG (x + c x^3)).
+// 2 sqrt(2 / pi) and the cubic's factor: gelu_tanh(x) = x sigmoid(kG (x + kC x^3)).
 constexpr float kG = 1.5957691216057308f;
 constexpr float kC = 0.044715f;
 
-// Normal distribution function, accurate in the lower tail (1 + erf would cancel there).
+// Normal distribution function Phi(x) and exp(-x^2 / 2). For x <= 0,
+// Phi(x) = 0.5 erfcx(|x| / sqrt(2)) exp(-x^2 / 2), which keeps the lower tail's relative accuracy
+// (1 + erf would cancel there). erfcx(z) = exp(z^2) erfc(z) is a degree-8 polynomial without
+// constant term in t = 1 / (1 + 0.33 z) (the form of Abramowitz and Stegun 7.1.26), its
+// coefficients fitted here for the least largest relative error on 0 <= z <= 9.6: 8.2e-8. Beyond,
+// the exponential is below the smallest normal float. erfcf instead took act_backward_mx with
+// GELU from 79 to 192 us at 4096 x 16384.
+__device__ __forceinline__ float phi_cdf(float x, float& e) {
+    const float t = rcp(fmaf(fabsf(x), 0.33f * 0.70710678f, 1.0f));
+    e = __expf(-0.5f * x * x);
+    float p = -0.067971688f;
+    p = fmaf(p, t, 0.23137758f);
+    p = fmaf(p, t, -0.17778363f);
+    p = fmaf(p, t, 0.20633723f);
+    p = fmaf(p, t, 0.022465308f);
+    p = fmaf(p, t, 0.10097591f);
+    p = fmaf(p, t, 0.091415916f);
+    p = fmaf(p, t, 0.093183258f);
+    const float q = p * t * e;
+    return x > 0.0f ? 1.0f - q : q;
+}
 __device__ __forceinline__ float phi_cdf(float x) {
-    return 0.5f * erfcf(-0.7071067811865476f * x);
+    float e;
+    return phi_cdf(x, e);
 }
 
 __device__ __forceinline__ float act(uint32_t kind, float x) {
@@ -101,9 +156,10 @@ __device__ __forceinline__ void act_grad(uint32_t kind, float x, float& f, float
         break;
     }
     case PTXSTD_ACT_GELU: {
-        const float t = phi_cdf(x);
+        float e;
+        const float t = phi_cdf(x, e);
         f = x * t;
-        df = t + x * (0.3989422804014327f * __expf(-0.5f * x * x));
+        df = fmaf(x * 0.3989422804014327f, e, t);
         break;
     }
     case PTXSTD_ACT_GELU_TANH: {

@@ -164,12 +164,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
         if (p.q) {
             // a block of 32 is the vectors of four neighbouring lanes (cols % 32 == 0, so a block
             // is inside the row or outside it as a whole); lanes outside hold zeros
-            uint32_t m = 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) m = mx::amax_bits(m, a[k]);
-            if (!on) m = 0;  // 0 * rx is NaN when rx is
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float m = mx::amax_quad(mx::amax_of(a));  // every lane takes part
             const uint32_t code = on ? mx::scale_code(m, emax) : 0u;
             const float inv = dt::ue8m0_inverse(code);
             if (on)
