@@ -277,7 +277,8 @@ extern "C" int ptxstd_act_backward_mx(int act, const uint16_t* d_dh, const uint1
     ptxstd::Reduce r = {};
     r.partial = p.partial;
     r.P = (p.rows + kRows - 1) / kRows;
-    r.cols = r.split0 = r.split1 = p.W;
+    r.sums = 1;
+    r.cols = p.W;
     r.o0 = d_dbias;
     return ptxstd::launch_reduce(r, s);
 }

@@ -19,6 +19,61 @@ __device__ __forceinline__ void pdl_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// ---- packed f32 pairs --------------------------------------------------------------------------
+// sm_100's two-wide f32 instructions (two IEEE operations per issue slot); element 0 in the low
+// half.
+using f32x2 = uint64_t;
+__device__ __forceinline__ f32x2 pack2f(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float hsum2(f32x2 v) {
+    const float2 f = unpack2(v);
+    return f.x + f.y;
+}
+// Eight bf16 values of a 16-byte vector as four pairs, and back (round to nearest even).
+struct Oct {
+    f32x2 v[4];
+};
+__device__ __forceinline__ Oct widen(const uint4& w) {
+    Oct o;
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        o.v[k] = pack2f(data_types::bf16_lo(x[k]), data_types::bf16_hi(x[k]));
+    return o;
+}
+__device__ __forceinline__ uint4 narrow(const Oct& o) {
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2(o.v[k]);
+        x[k] = data_types::bf16x2_from_f32(f.x, f.y);
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 namespace mx {
 
 // ---- blocked scales, padded ------------------------------------------------------------------
@@ -67,19 +122,10 @@ __device__ __forceinline__ uint32_t scale_code(float amax, uint32_t emax) {
     const uint32_t u = data_types::ue8m0_from_f32<false, true>(amax);
     return u == 0xFFu ? 0xFFu : (u > emax ? u - emax : 0u);
 }
-// (a s, b s): one packed multiply, two IEEE products.
-__device__ __forceinline__ float2 mul2(float a, float b, float s) {
-    const uint64_t x = (static_cast<uint64_t>(__float_as_uint(b)) << 32) | __float_as_uint(a);
-    const uint64_t y = (static_cast<uint64_t>(__float_as_uint(s)) << 32) | __float_as_uint(s);
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return make_float2(__uint_as_float(static_cast<uint32_t>(r)),
-                       __uint_as_float(static_cast<uint32_t>(r >> 32)));
-}
 // Two values times 2^-(code-127) (exact but for subnormal results) as a code pair.
 template <uint32_t T>
 __device__ __forceinline__ uint32_t pack2(float a, float b, float inv) {
-    const float2 v = mul2(a, b, inv);
+    const float2 v = unpack2(mul2(pack2f(a, b), pack2f(inv, inv)));
     return T == kE4m3 ? data_types::e4m3x2_from_f32<false>(v.x, v.y)
                       : data_types::e5m2x2_from_f32<false>(v.x, v.y);
 }

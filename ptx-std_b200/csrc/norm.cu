@@ -15,9 +15,14 @@
 //   dy = ry b - y ry^3 mean(b y),          dw_post = sum_rows dp y ry.
 // mean(b y) needs dx, hence mean(a x'). Substituting dx gives, with t = scale g w_post y,
 //   sum(b y) = sum(t du) + rx sum(t a) - (rx^3 mean(a x')) sum(t x'),
-// so one exchange of four sums serves both means. Each thread keeps its columns for all rows of
-// the CTA and accumulates the column sums in f32 registers; the CTAs' partial sums go through a
-// workspace and are added in CTA order by a second kernel (reproducible, no atomics).
+// so one exchange of four sums serves both means. With one gate for all rows both dg and dw_post
+// are column factors times the same sum, S = sum_rows dx y ry: dg = scale w_post S,
+// dw_post = scale g S; with a gate per row dg needs no sum and S takes g inside. So there are two
+// column sums at most. Each thread keeps its columns for all rows of its group and accumulates
+// them in f32; the partial sums go through a workspace and are added in order by a second kernel
+// (reproducible, no atomics), which applies the factors.
+//
+// Both directions are near the issue rate as well as the HBM rate, hence the packed f32 pairs.
 #include "common.cuh"
 #include "data_types.cuh"
 #include "mx_block.cuh"
@@ -28,18 +33,17 @@ namespace {
 namespace dt = ptxstd::data_types;
 namespace mx = ptxstd::mx;
 
-__device__ __forceinline__ void unpack8(const uint4& v, float (&o)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        o[2 * k] = dt::bf16_lo(w[k]);
-        o[2 * k + 1] = dt::bf16_hi(w[k]);
-    }
-}
-__device__ __forceinline__ uint4 pack8(const float (&o)[8]) {
-    return make_uint4(dt::bf16x2_from_f32(o[0], o[1]), dt::bf16x2_from_f32(o[2], o[3]),
-                      dt::bf16x2_from_f32(o[4], o[5]), dt::bf16x2_from_f32(o[6], o[7]));
-}
+using ptxstd::add2;
+using ptxstd::f32x2;
+using ptxstd::fma2;
+using ptxstd::hsum2;
+using ptxstd::mul2;
+using ptxstd::narrow;
+using ptxstd::Oct;
+using ptxstd::pack2f;
+using ptxstd::unpack2;
+using ptxstd::widen;
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -68,6 +72,83 @@ struct Fwd {
     size_t gate_stride;  // 0: one gate for all rows
 };
 
+__device__ __forceinline__ f32x2 square_sum(const uint4& v, f32x2 s) {
+    const Oct a = widen(v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s = fma2(a.v[k], a.v[k], s);
+    return s;
+}
+
+// bf16(x + scale gate (y ry w_post)) of eight columns; w_post and gate may be null.
+__device__ __forceinline__ uint4 join8(const uint4& xv, const uint4& yv, const uint4* w_post,
+                                       const uint4* gate, float ry, float scale) {
+    Oct a = widen(yv), x = widen(xv);
+    if (w_post) {
+        const Oct w = widen(*w_post);
+        const f32x2 r = pack2f(ry, ry);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.v[k] = mul2(mul2(a.v[k], r), w.v[k]);
+    }
+    if (gate) {
+        const Oct w = widen(*gate);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.v[k] = mul2(a.v[k], w.v[k]);
+    }
+    const f32x2 s = pack2f(scale, scale);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x.v[k] = fma2(s, a.v[k], x.v[k]);
+    return narrow(x);
+}
+
+// n = x' rx w of eight columns (vector i of the row), stored as bf16 and / or quantised. Every
+// lane of the warp calls it; lanes outside the row pass on = false and zeros. A block of 32 is the
+// vectors of four neighbouring lanes (cols % 32 == 0, so a block is inside the row or outside it
+// as a whole).
+__device__ __forceinline__ void finish8(const Fwd& p, const uint4& xv, const uint4& wv, float rx,
+                                        uint32_t row, size_t base, uint32_t i, bool on,
+                                        uint32_t lane, size_t k_tiles) {
+    Oct n = widen(xv);
+    const Oct w = widen(wv);
+    const f32x2 r = pack2f(rx, rx);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n.v[k] = mul2(mul2(n.v[k], r), w.v[k]);
+    if (p.n && on) *reinterpret_cast<uint4*>(p.n + base + 8 * i) = narrow(n);
+    if (!p.q) return;
+    float a[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2(n.v[k]);
+        a[2 * k] = f.x;
+        a[2 * k + 1] = f.y;
+    }
+    const float m = mx::amax_quad(mx::amax_of(a));
+    const uint32_t code = on ? mx::scale_code(m, mx::emax_of(p.q_type)) : 0u;
+    const float inv = dt::ue8m0_inverse(code);
+    if (on)
+        *reinterpret_cast<uint2*>(p.q + base + 8 * i) =
+            make_uint2(mx::pack4(p.q_type, a[0], a[1], a[2], a[3], inv),
+                       mx::pack4(p.q_type, a[4], a[5], a[6], a[7], inv));
+    if (p.blocked) {
+        // four blocks' codes (16 lanes) as one word of the scale tile
+        uint32_t c = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;
+        c |= __shfl_down_sync(0xffffffffu, c, 8) << 16;
+        if ((lane & 15u) == 0 && on)
+            *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, i >> 4, k_tiles)) = c;
+    } else if ((lane & 3u) == 0 && on) {
+        p.sf[static_cast<size_t>(row) * (p.cols / 32) + (i >> 2)] = static_cast<uint8_t>(code);
+    }
+}
+
+// The blocked scales' padding rows: zero.
+__device__ __forceinline__ void pad_row(const Fwd& p, uint32_t row, uint32_t tid, uint32_t stride,
+                                        size_t k_tiles) {
+    if (p.q && p.blocked && row < mx::padded_rows(p.rows))
+        for (size_t t = tid; t < k_tiles; t += stride)
+            *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, t, k_tiles)) = 0;
+}
+
+// One row per warp or per block, straight from global memory: for few rows (a single row's
+// latency), short rows and the longest ones.
 constexpr uint32_t kWarpRows = 4;  // rows of a CTA when a warp holds a row
 
 template <int V, bool WARP_ROW>
@@ -83,13 +164,14 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
 
     ptxstd::pdl_launch_dependents();
     ptxstd::pdl_wait();
-    if (row >= p.rows) {  // padding rows of the blocked scales
-        if (p.q && p.blocked && row < mx::padded_rows(p.rows))
-            for (size_t t = tid; t < k_tiles; t += stride)
-                *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, t, k_tiles)) = 0;
+    if (row >= p.rows) {
+        pad_row(p, row, tid, stride, k_tiles);
         return;
     }
     const size_t base = static_cast<size_t>(row) * p.cols;
+    const uint4* const w_post = reinterpret_cast<const uint4*>(p.w_post);
+    const uint4* const gate =
+        p.gate ? reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride) : nullptr;
     uint4 xv[V], yv[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -103,84 +185,219 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
     const float inv_d = 1.0f / static_cast<float>(p.cols);
     if (p.y) {
         float ry = 1.0f;
-        if (p.w_post) {
-            float s = 0.0f;
+        if (w_post) {
+            f32x2 s = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float a[8];
-                unpack8(yv[j], a);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) s = fmaf(a[k], a[k], s);
-            }
-            ry = rsqrtf(row_sum<WARP_ROW>(s, red[0]) * inv_d + p.eps);
+            for (int j = 0; j < V; ++j) s = square_sum(yv[j], s);
+            ry = rsqrtf(row_sum<WARP_ROW>(hsum2(s), red[0]) * inv_d + p.eps);
             if (p.rstd_post && tid == 0) p.rstd_post[row] = ry;
         }
-        const uint16_t* gate = p.gate ? p.gate + row * p.gate_stride : nullptr;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = tid + j * stride;
             if (i >= nv) continue;
-            float a[8], x[8], w[8];
-            unpack8(yv[j], a);
-            unpack8(xv[j], x);
-            if (p.w_post) {
-                unpack8(__ldg(reinterpret_cast<const uint4*>(p.w_post + 8 * i)), w);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) a[k] = a[k] * ry * w[k];
-            }
-            if (gate) {
-                unpack8(__ldg(reinterpret_cast<const uint4*>(gate + 8 * i)), w);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) a[k] *= w[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = fmaf(p.scale, a[k], x[k]);
-            xv[j] = pack8(x);
+            xv[j] = join8(xv[j], yv[j], w_post ? w_post + i : nullptr, gate ? gate + i : nullptr,
+                          ry, p.scale);
             *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
         }
     }
-    float s = 0.0f;
+    f32x2 s = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        float a[8];
-        unpack8(xv[j], a);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s = fmaf(a[k], a[k], s);
-    }
-    const float rx = rsqrtf(row_sum<WARP_ROW>(s, red[1]) * inv_d + p.eps);
+    for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
+    const float rx = rsqrtf(row_sum<WARP_ROW>(hsum2(s), red[1]) * inv_d + p.eps);
     if (p.rstd && tid == 0) p.rstd[row] = rx;
-    const uint32_t emax = mx::emax_of(p.q_type);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const uint32_t i = tid + j * stride;
         const bool on = i < nv;
-        float a[8], w[8];
-        unpack8(xv[j], a);
-        unpack8(on ? __ldg(reinterpret_cast<const uint4*>(p.w + 8 * i)) : make_uint4(0, 0, 0, 0),
-                w);
+        const uint4 w = on ? __ldg(reinterpret_cast<const uint4*>(p.w) + i) : make_uint4(0, 0, 0, 0);
+        finish8(p, xv[j], w, rx, row, base, i, on, lane, k_tiles);
+    }
+}
+
+// ---- many rows: a ring of rows in shared memory ------------------------------------------------
+// One CTA per SM walks the rows blockIdx, blockIdx + grid, ...; a producer lane streams each row's
+// inputs into a ring of stages with bulk copies, and groups of consumer threads take the rows in
+// turn, so that the loads of later rows, one row's sums and another's stores overlap and up to
+// 200 KB per SM are in flight whatever the groups wait for. The column weights sit in shared
+// memory for the CTA's life.
+constexpr uint32_t kRingBytes = 222 * 1024;
+constexpr uint32_t kMaxRing = 8;
+enum : uint32_t { kDetailFwdProducer = 0x4100, kDetailFwdConsumer = 0x4200,
+                  kDetailBwdProducer = 0x4300, kDetailBwdConsumer = 0x4400 };
+
+struct Ring {
+    uint64_t full[kMaxRing];
+    uint64_t empty[kMaxRing];
+    uint32_t abort;
+};
+
+__device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+
+// A consumer warp's wait for a stage. After a timeout (recorded) the kernel runs on without
+// waiting, on whatever the stages hold, so that every barrier still sees all of its threads.
+__device__ __forceinline__ void ring_wait(Ring& r, uint32_t stage, uint32_t phase, uint32_t* err,
+                                          uint32_t detail) {
+    volatile uint32_t* abort_flag = &r.abort;
+    if (!*abort_flag && !ptxstd::mbar_wait(&r.full[stage], phase)) {
+        ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail | stage);
+        *abort_flag = 1u;
+    }
+}
+
+// The producer lane: row k of this CTA into stage k % stages, from the `n` non-null arrays.
+struct Sources {
+    const uint16_t* p[5];
+    uint32_t n;
+};
+__device__ __forceinline__ void produce_rows(Ring& r, uint8_t* base, uint32_t stages,
+                                             const Sources& src, uint32_t rows, uint32_t cols,
+                                             uint32_t* err, uint32_t detail) {
+    volatile uint32_t* abort_flag = &r.abort;
+    const uint32_t bytes = cols * 2;
+    uint32_t stage = 0, phase = 0, issued = 0, parity = 0;
+    for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        if (!ptxstd::mbar_wait(&r.empty[stage], phase ^ 1u)) {
+            ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail | stage);
+            *abort_flag = 1u;
+        }
+        if (*abort_flag) break;
+        ptxstd::mbar_arrive_expect_tx(&r.full[stage], bytes * src.n);
+        uint8_t* dst = base + static_cast<size_t>(stage) * bytes * src.n;
+        uint32_t n = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] = a[k] * rx * w[k];
-        if (p.n && on) *reinterpret_cast<uint4*>(p.n + base + 8 * i) = pack8(a);
-        if (p.q) {
-            // a block of 32 is the vectors of four neighbouring lanes (cols % 32 == 0, so a block
-            // is inside the row or outside it as a whole); lanes outside hold zeros
-            const float m = mx::amax_quad(mx::amax_of(a));  // every lane takes part
-            const uint32_t code = on ? mx::scale_code(m, emax) : 0u;
-            const float inv = dt::ue8m0_inverse(code);
-            if (on)
-                *reinterpret_cast<uint2*>(p.q + base + 8 * i) =
-                    make_uint2(mx::pack4(p.q_type, a[0], a[1], a[2], a[3], inv),
-                               mx::pack4(p.q_type, a[4], a[5], a[6], a[7], inv));
-            if (p.blocked) {
-                // four blocks' codes (16 lanes) as one word of the scale tile
-                uint32_t c = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;
-                c |= __shfl_down_sync(0xffffffffu, c, 8) << 16;
-                if ((lane & 15u) == 0 && on)
-                    *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, i >> 4, k_tiles)) = c;
-            } else if ((lane & 3u) == 0 && on) {
-                p.sf[static_cast<size_t>(row) * (p.cols / 32) + (i >> 2)] =
-                    static_cast<uint8_t>(code);
+        for (int k = 0; k < 5; ++k)
+            if (src.p[k])
+                ptxstd::bulk_load(dst + n++ * bytes, src.p[k] + static_cast<size_t>(row) * cols,
+                                  bytes, &r.full[stage]);
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    if (*abort_flag)
+        for (uint32_t i = 0; i < stages; ++i)
+            if (issued & (1u << i)) ptxstd::mbar_wait(&r.full[i], (parity >> i) & 1u);
+}
+
+__device__ __forceinline__ void init_ring(Ring& r, uint32_t stages, uint32_t consumer_warps) {
+    for (uint32_t i = 0; i < stages; ++i) {
+        ptxstd::mbar_init(&r.full[i], 1);
+        ptxstd::mbar_init(&r.empty[i], consumer_warps);
+    }
+    r.abort = 0;
+    ptxstd::fence_mbarrier_init();
+}
+
+constexpr uint32_t kGroupThreads = 256, kGroups = 3;
+
+template <int V>
+__global__ void __launch_bounds__(kGroupThreads* kGroups + 32, 1)
+    norm_ring_kernel(const __grid_constant__ Fwd p, uint32_t stages, uint32_t* err) {
+    extern __shared__ uint4 ring_smem[];
+    __shared__ Ring ring;
+    __shared__ float4 red[kGroups][3][2];  // eight warps' partial sums; a buffer per exchange
+    const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
+    const uint32_t nv = p.cols / 8;
+    const size_t k_tiles = mx::tiles_k(p.cols / 32);
+    const bool gate_rows = p.gate && p.gate_stride;
+    // shared memory: w | w_post | gate (if one for all rows) | stages of x | y | gate row
+    uint4* const w = ring_smem;
+    uint4* const w_post = w + nv;
+    uint4* const gate = w_post + (p.w_post ? nv : 0);
+    uint4* const stage0 = gate + (p.gate && !gate_rows ? nv : 0);
+    const uint32_t arrays = 1 + (p.y ? 1 : 0) + (gate_rows ? 1 : 0);
+
+    ptxstd::pdl_launch_dependents();
+    if (tid == 0) init_ring(ring, stages, kGroupThreads / 32);
+    ptxstd::pdl_wait();
+    for (uint32_t i = tid; i < nv; i += blockDim.x) {
+        w[i] = __ldg(reinterpret_cast<const uint4*>(p.w) + i);
+        if (p.w_post) w_post[i] = __ldg(reinterpret_cast<const uint4*>(p.w_post) + i);
+        if (p.gate && !gate_rows) gate[i] = __ldg(reinterpret_cast<const uint4*>(p.gate) + i);
+    }
+    for (uint32_t row = p.rows + blockIdx.x; row < mx::padded_rows(p.rows); row += gridDim.x)
+        pad_row(p, row, tid, blockDim.x, k_tiles);
+    __syncthreads();
+
+    const uint32_t g = warp / (kGroupThreads / 32);
+    if (g == kGroups) {
+        if (lane == 0) {
+            const Sources s = {{p.x, p.y, gate_rows ? p.gate : nullptr, nullptr, nullptr}, arrays};
+            produce_rows(ring, reinterpret_cast<uint8_t*>(stage0), stages, s, p.rows, p.cols, err,
+                         kDetailFwdProducer);
+        }
+        return;
+    }
+    const uint32_t t = tid - g * kGroupThreads, gw = t >> 5;
+    const float inv_d = 1.0f / static_cast<float>(p.cols);
+    auto group_sum = [&](float v, float4* buf) {
+        v = warp_sum(v);
+        if (lane == 0) reinterpret_cast<float*>(buf)[gw] = v;
+        group_sync(g, kGroupThreads);
+        const float4 a = buf[0], b = buf[1];
+        return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+    };
+    uint32_t stage = g % stages, phase = (g / stages) & 1u, flip = 0;
+    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows; row += kGroups * gridDim.x) {
+        ring_wait(ring, stage, phase, err, kDetailFwdConsumer);
+        __syncwarp();
+        const uint4* const xs = stage0 + static_cast<size_t>(stage) * arrays * nv;
+        const uint4 *const ys = xs + nv, *const gs = gate_rows ? xs + 2 * nv : gate;
+        const size_t base = static_cast<size_t>(row) * p.cols;
+        uint4 xv[V];
+        if (p.y) {
+            float ry = 1.0f;
+            if (p.w_post) {
+                f32x2 s = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const uint32_t i = t + j * kGroupThreads;
+                    if (i < nv) s = square_sum(ys[i], s);
+                }
+                ry = rsqrtf(group_sum(hsum2(s), red[g][0]) * inv_d + p.eps);
+                if (p.rstd_post && t == 0) p.rstd_post[row] = ry;
             }
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint32_t i = t + j * kGroupThreads;
+                xv[j] = make_uint4(0, 0, 0, 0);
+                if (i < nv) {
+                    xv[j] = join8(xs[i], ys[i], p.w_post ? w_post + i : nullptr,
+                                  p.gate ? gs + i : nullptr, ry, p.scale);
+                    *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint32_t i = t + j * kGroupThreads;
+                xv[j] = i < nv ? xs[i] : make_uint4(0, 0, 0, 0);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) ptxstd::mbar_arrive(&ring.empty[stage]);
+        f32x2 s = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
+        const float rx = rsqrtf(group_sum(hsum2(s), red[g][1 + flip]) * inv_d + p.eps);
+        if (p.rstd && t == 0) p.rstd[row] = rx;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = t + j * kGroupThreads;
+            const bool on = i < nv;
+            finish8(p, xv[j], on ? w[i] : make_uint4(0, 0, 0, 0), rx, row, base, i, on, lane,
+                    k_tiles);
+        }
+        flip ^= 1u;
+        stage += kGroups;
+        while (stage >= stages) {
+            stage -= stages;
+            phase ^= 1u;
         }
     }
 }
@@ -196,62 +413,229 @@ int launch_fwd(const Fwd& p, uint32_t threads, cudaStream_t stream) {
     return ptxstd::launch_status();
 }
 
+// Stages of a ring of rows beside `fixed` bytes of weights.
+uint32_t ring_stages(size_t fixed, size_t row_bytes) {
+    if (fixed > kRingBytes) return 0;
+    const size_t n = (kRingBytes - fixed) / row_bytes;
+    return static_cast<uint32_t>(n < kMaxRing ? n : kMaxRing);
+}
+
+template <int V>
+int launch_fwd_ring(const Fwd& p, uint32_t stages, size_t smem, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    const int st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(norm_ring_kernel<V>),
+                                                kRingBytes);
+    if (st) return st;
+    uint32_t* err = ptxstd::device_error_word();
+    if (!err) return PTXSTD_ECUDA;
+    const uint32_t sms = static_cast<uint32_t>(ptxstd::sm_count());
+    ptxstd::set_pdl(cfg, attr, p.rows < sms ? p.rows : sms, kGroupThreads * kGroups + 32, stream);
+    cfg.dynamicSmemBytes = smem;
+    if (cudaLaunchKernelEx(&cfg, norm_ring_kernel<V>, p, stages, err) != cudaSuccess)
+        return PTXSTD_ECUDA;
+    return ptxstd::launch_status();
+}
+
 // ---- backward ---------------------------------------------------------------------------------
 struct Bwd {
     const uint16_t *dn, *du, *x, *w, *y, *w_post, *gate;
     const float *rstd, *rstd_post;
     uint16_t *dx, *dy, *dgate_rows;
-    float* partial;  // [grid][sums][cols]
+    float* partial;  // [groups of the grid][sums][cols]
     float scale;
     uint32_t rows, cols;
-    uint32_t sums;      // 1 dw, + dw_post, + dgate (vector gate), in that order
-    uint32_t post_at, gate_at;  // index of their sums, or 0
+    uint32_t sums;  // 1: dw; 2: dw and S
     size_t gate_stride;
 };
 
-// Column sums of a thread's V vectors, in registers, or in shared memory when V is large.
+// Column factors of eight columns: w, and c = scale w_post gate (the gate of all rows; 1 where
+// there is none).
+struct Factors {
+    Oct w, c;
+};
+__device__ __forceinline__ Factors column_factors(const Bwd& p, uint32_t i) {
+    Factors f;
+    f.w = widen(__ldg(reinterpret_cast<const uint4*>(p.w) + i));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.c.v[k] = pack2f(p.scale, p.scale);
+    if (p.w_post) {
+        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(p.w_post) + i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.c.v[k] = mul2(f.c.v[k], o.v[k]);
+    }
+    if (p.gate && !p.gate_stride) {
+        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(p.gate) + i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.c.v[k] = mul2(f.c.v[k], o.v[k]);
+    }
+    return f;
+}
+
+// What a row's sums need of eight columns: sum(a x'), sum(t du), sum(t a), sum(t x') with
+// a = dn w, t = c gate y. `gate` is this row's own gate, or null.
+struct Sums {
+    f32x2 ax = 0, td = 0, ta = 0, tx = 0;
+};
+__device__ __forceinline__ void sums8(Sums& s, const uint4& dnv, const uint4& duv, const uint4& xv,
+                                      const uint4& yv, const Factors& f, bool post,
+                                      const uint4* gate) {
+    Oct a = widen(dnv);
+    const Oct x = widen(xv);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        a.v[k] = mul2(a.v[k], f.w.v[k]);
+        s.ax = fma2(a.v[k], x.v[k], s.ax);
+    }
+    if (!post) return;  // without w_post nothing is divided by y's norm
+    Oct t = widen(yv);
+    const Oct u = widen(duv);
+    if (gate) {
+        const Oct g = widen(*gate);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t.v[k] = mul2(t.v[k], g.v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        t.v[k] = mul2(t.v[k], f.c.v[k]);
+        s.td = fma2(t.v[k], u.v[k], s.td);
+        s.ta = fma2(t.v[k], a.v[k], s.ta);
+        s.tx = fma2(t.v[k], x.v[k], s.tx);
+    }
+}
+
+// The factors of a row in the gradients, from its sums and statistics.
+struct RowFactors {
+    float rx, ry, k1, k2;
+};
+__device__ __forceinline__ RowFactors row_factors(const float4& s, float rx, float ry,
+                                                  float inv_d) {
+    RowFactors f;
+    f.rx = rx;
+    f.ry = ry;
+    f.k1 = rx * rx * rx * (s.x * inv_d);
+    f.k2 = ry * ry * ry * ((s.y + rx * s.z - f.k1 * s.w) * inv_d);
+    return f;
+}
+
+// The gradients of eight columns of a row; adds dn x' rx to `dw` and dx y ry (times the row's own
+// gate) to `S`.
+__device__ __forceinline__ void grads8(const Bwd& p, const RowFactors& r, const uint4& dnv,
+                                       const uint4& duv, const uint4& xv, const uint4& yv,
+                                       const Factors& f, const uint4* gate, size_t at, Oct& dw,
+                                       Oct& S) {
+    const Oct dn = widen(dnv), x = widen(xv);
+    Oct dx = widen(duv);
+    const f32x2 rx = pack2f(r.rx, r.rx), k1 = pack2f(-r.k1, -r.k1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        dw.v[k] = fma2(mul2(x.v[k], rx), dn.v[k], dw.v[k]);
+        dx.v[k] = fma2(rx, mul2(dn.v[k], f.w.v[k]), dx.v[k]);
+        dx.v[k] = fma2(x.v[k], k1, dx.v[k]);
+    }
+    *reinterpret_cast<uint4*>(p.dx + at) = narrow(dx);
+    if (!p.y) return;
+    const Oct y = widen(yv);
+    const f32x2 ry = pack2f(r.ry, r.ry), k2 = pack2f(-r.k2, -r.k2);
+    Oct b;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b.v[k] = mul2(dx.v[k], f.c.v[k]);
+    if (gate) {
+        const Oct g = widen(*gate);
+        Oct dg;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f32x2 yh = mul2(y.v[k], ry);
+            dg.v[k] = mul2(b.v[k], yh);
+            S.v[k] = fma2(mul2(dx.v[k], g.v[k]), yh, S.v[k]);
+            b.v[k] = mul2(b.v[k], g.v[k]);
+        }
+        *reinterpret_cast<uint4*>(p.dgate_rows + at) = narrow(dg);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) S.v[k] = fma2(dx.v[k], mul2(y.v[k], ry), S.v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b.v[k] = fma2(ry, b.v[k], mul2(y.v[k], k2));
+    *reinterpret_cast<uint4*>(p.dy + at) = narrow(b);
+}
+
+__device__ __forceinline__ void store_oct(float* dst, const Oct& o) {
+    const float2 a = unpack2(o.v[0]), b = unpack2(o.v[1]), c = unpack2(o.v[2]),
+                 d = unpack2(o.v[3]);
+    reinterpret_cast<float4*>(dst)[0] = make_float4(a.x, a.y, b.x, b.y);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(c.x, c.y, d.x, d.y);
+}
+__device__ __forceinline__ Oct load_oct(const float* src) {
+    const float4 a = reinterpret_cast<const float4*>(src)[0];
+    const float4 b = reinterpret_cast<const float4*>(src)[1];
+    return {{pack2f(a.x, a.y), pack2f(a.z, a.w), pack2f(b.x, b.y), pack2f(b.z, b.w)}};
+}
+constexpr Oct kZeroOct = {{0, 0, 0, 0}};
+
+// A warp's four sums, lane 8 q holding sum q (six shuffles: halves of the lanes take halves of the
+// sums, then a tree).
+__device__ __forceinline__ float warp_sum4(const Sums& q, uint32_t lane) {
+    const float4 s = make_float4(hsum2(q.ax), hsum2(q.td), hsum2(q.ta), hsum2(q.tx));
+    const bool hi = lane & 16u, odd = lane & 8u;
+    float a = hi ? s.z : s.x, b = hi ? s.w : s.y;
+    a += __shfl_xor_sync(0xffffffffu, hi ? s.x : s.z, 16);
+    b += __shfl_xor_sync(0xffffffffu, hi ? s.y : s.w, 16);
+    float c = odd ? b : a;
+    c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+    for (int d = 4; d; d >>= 1) c += __shfl_xor_sync(0xffffffffu, c, d);
+    return c;
+}
+
+// Sum over the group's warps: every warp leaves its four sums in buf[warp], every thread adds them
+// in warp order. `buf` alternates between rows, so one barrier per row is enough.
+template <uint32_t WARPS>
+__device__ __forceinline__ float4 group_sum4(const Sums& s, float4* buf, uint32_t warp,
+                                             uint32_t lane, uint32_t warps, uint32_t group) {
+    const float c = warp_sum4(s, lane);
+    if ((lane & 7u) == 0) reinterpret_cast<float*>(buf + warp)[lane >> 3] = c;
+    group_sync(group, warps * 32);
+    float4 r = buf[0];
+#pragma unroll
+    for (uint32_t k = 1; k < WARPS; ++k)
+        if (k < warps) {
+            const float4 o = buf[k];
+            r.x += o.x;
+            r.y += o.y;
+            r.z += o.z;
+            r.w += o.w;
+        }
+    return r;
+}
+
+// Rows of up to 1024 columns (few threads per row, many blocks per SM) and of more than 8192 (whose
+// column sums need shared memory). V vectors per thread.
 template <int V>
-__global__ void __launch_bounds__(V == 4 ? 512 : 512)
+__global__ void __launch_bounds__(V == 1 ? 128 : 512)
     norm_backward_kernel(const __grid_constant__ Bwd p) {
-    constexpr bool kShared = V == 4;
-    extern __shared__ float acc_smem[];  // [3][cols] when kShared
-    __shared__ float red[2][4][16];
+    constexpr bool kShared = V > 1;
+    constexpr uint32_t kMaxWarps = V == 1 ? 4 : 16;
+    extern __shared__ float acc_smem[];  // [sums][cols] when kShared
+    __shared__ float4 red[2][kMaxWarps];
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t warps = blockDim.x >> 5, stride = blockDim.x, nv = p.cols / 8;
-    float acc[kShared ? 1 : 3][kShared ? 1 : V][8];
+    Oct dw = kZeroOct, S = kZeroOct;
     ptxstd::pdl_launch_dependents();
     if constexpr (kShared) {
         for (uint32_t i = tid; i < p.sums * p.cols; i += stride) acc_smem[i] = 0.0f;
         __syncthreads();
-    } else {
-#pragma unroll
-        for (int s = 0; s < 3; ++s)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) acc[s][j][k] = 0.0f;
     }
-    auto add = [&](uint32_t s, int si, int j, uint32_t i, const float (&v)[8]) {
-        if constexpr (kShared) {
-            float4* a = reinterpret_cast<float4*>(acc_smem + s * p.cols + 8 * i);
-            float4 lo = a[0], hi = a[1];
-            lo.x += v[0]; lo.y += v[1]; lo.z += v[2]; lo.w += v[3];
-            hi.x += v[4]; hi.y += v[5]; hi.z += v[6]; hi.w += v[7];
-            a[0] = lo;
-            a[1] = hi;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[si][j][k] += v[k];
-        }
-    };
     ptxstd::pdl_wait();
 
     const float inv_d = 1.0f / static_cast<float>(p.cols);
     uint32_t flip = 0;
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 1u) {
         const size_t base = static_cast<size_t>(row) * p.cols;
-        const uint16_t* gate = p.gate ? p.gate + row * p.gate_stride : nullptr;
+        const uint4* const gate =
+            p.gate_stride ? reinterpret_cast<const uint4*>(p.gate + base) : nullptr;
         uint4 dnv[V], duv[V], xv[V], yv[V];
+        Sums s;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = tid + j * stride;
@@ -263,108 +647,31 @@ __global__ void __launch_bounds__(V == 4 ? 512 : 512)
                 if (p.y) yv[j] = *reinterpret_cast<const uint4*>(p.y + base + 8 * i);
             }
         }
-        const float rx = p.rstd[row];
-        const float ry = p.w_post ? p.rstd_post[row] : 1.0f;
-        float s_ax = 0.0f, s_td = 0.0f, s_ta = 0.0f, s_tx = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = tid + j * stride;
+            if (i < nv)
+                sums8(s, dnv[j], duv[j], xv[j], yv[j], column_factors(p, i), p.w_post,
+                      gate ? gate + i : nullptr);
+        }
+        const float4 sum = group_sum4<kMaxWarps>(s, red[flip], warp, lane, warps, 0);
+        const RowFactors r =
+            row_factors(sum, p.rstd[row], p.w_post ? p.rstd_post[row] : 1.0f, inv_d);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = tid + j * stride;
             if (i >= nv) continue;
-            float dn[8], x[8], w[8];
-            unpack8(dnv[j], dn);
-            unpack8(xv[j], x);
-            unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + 8 * i)), w);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                dn[k] *= w[k];
-                s_ax = fmaf(dn[k], x[k], s_ax);
-            }
-            if (p.w_post) {
-                float t[8], u[8];
-                unpack8(yv[j], t);
-                unpack8(__ldg(reinterpret_cast<const uint4*>(p.w_post + 8 * i)), u);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) t[k] *= p.scale * u[k];
-                if (gate) {
-                    unpack8(__ldg(reinterpret_cast<const uint4*>(gate + 8 * i)), u);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) t[k] *= u[k];
-                }
-                unpack8(duv[j], u);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    s_td = fmaf(t[k], u[k], s_td);
-                    s_ta = fmaf(t[k], dn[k], s_ta);
-                    s_tx = fmaf(t[k], x[k], s_tx);
-                }
-            }
-        }
-        s_ax = warp_sum(s_ax);
-        if (p.w_post) {
-            s_td = warp_sum(s_td);
-            s_ta = warp_sum(s_ta);
-            s_tx = warp_sum(s_tx);
-        }
-        if (lane == 0) {
-            red[flip][0][warp] = s_ax;
-            red[flip][1][warp] = s_td;
-            red[flip][2][warp] = s_ta;
-            red[flip][3][warp] = s_tx;
-        }
-        __syncthreads();  // one per row: the two halves of `red` alternate
-        s_ax = warp_sum(lane < warps ? red[flip][0][lane & 15] : 0.0f);
-        const float k1 = rx * rx * rx * (s_ax * inv_d);
-        float k2 = 0.0f;
-        if (p.w_post) {
-            s_td = warp_sum(lane < warps ? red[flip][1][lane & 15] : 0.0f);
-            s_ta = warp_sum(lane < warps ? red[flip][2][lane & 15] : 0.0f);
-            s_tx = warp_sum(lane < warps ? red[flip][3][lane & 15] : 0.0f);
-            k2 = ry * ry * ry * ((s_td + rx * s_ta - k1 * s_tx) * inv_d);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t i = tid + j * stride;
-            if (i >= nv) continue;
-            float dx[8], x[8], dn[8], w[8], v[8];
-            unpack8(dnv[j], dn);
-            unpack8(xv[j], x);
-            unpack8(duv[j], dx);
-            unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + 8 * i)), w);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[k] = dn[k] * x[k] * rx;
-                dx[k] += rx * (dn[k] * w[k]) - x[k] * k1;
-            }
-            add(0, 0, j, i, v);
-            *reinterpret_cast<uint4*>(p.dx + base + 8 * i) = pack8(dx);
-            if (p.y) {
-                float y[8], g[8], wp[8];
-                unpack8(yv[j], y);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    dx[k] *= p.scale;
-                    g[k] = wp[k] = 1.0f;
-                }
-                if (p.w_post) unpack8(__ldg(reinterpret_cast<const uint4*>(p.w_post + 8 * i)), wp);
-                if (gate) {
-                    unpack8(__ldg(reinterpret_cast<const uint4*>(gate + 8 * i)), g);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = dx[k] * (y[k] * ry * wp[k]);
-                    if (p.dgate_rows)
-                        *reinterpret_cast<uint4*>(p.dgate_rows + base + 8 * i) = pack8(v);
-                    else
-                        add(p.gate_at, 2, j, i, v);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) dx[k] *= g[k];  // dp
-                if (p.w_post) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = dx[k] * y[k] * ry;
-                    add(p.post_at, 1, j, i, v);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) dx[k] = ry * (dx[k] * wp[k]) - y[k] * k2;
-                }
-                *reinterpret_cast<uint4*>(p.dy + base + 8 * i) = pack8(dx);
+            if constexpr (kShared) {
+                float *a = acc_smem + 8 * i, *b = a + p.cols;
+                dw = load_oct(a);
+                if (p.sums > 1) S = load_oct(b);
+                grads8(p, r, dnv[j], duv[j], xv[j], yv[j], column_factors(p, i),
+                       gate ? gate + i : nullptr, base + 8 * i, dw, S);
+                store_oct(a, dw);
+                if (p.sums > 1) store_oct(b, S);
+            } else {
+                grads8(p, r, dnv[j], duv[j], xv[j], yv[j], column_factors(p, i),
+                       gate ? gate + i : nullptr, base + 8 * i, dw, S);
             }
         }
     }
@@ -372,47 +679,150 @@ __global__ void __launch_bounds__(V == 4 ? 512 : 512)
     if constexpr (kShared) {
         __syncthreads();
         for (uint32_t i = tid; i < p.sums * p.cols; i += stride) out[i] = acc_smem[i];
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t i = tid + j * stride;
-            if (i >= nv) continue;
-#pragma unroll
-            for (int s = 0; s < 3; ++s) {
-                const uint32_t at = s == 0 ? 0 : s == 1 ? p.post_at : p.gate_at;
-                if (s > 0 && at == 0) continue;
-                float4* o = reinterpret_cast<float4*>(out + at * p.cols + 8 * i);
-                o[0] = make_float4(acc[s][j][0], acc[s][j][1], acc[s][j][2], acc[s][j][3]);
-                o[1] = make_float4(acc[s][j][4], acc[s][j][5], acc[s][j][6], acc[s][j][7]);
-            }
-        }
+    } else if (tid < nv) {
+        store_oct(out + 8 * tid, dw);
+        if (p.sums > 1) store_oct(out + p.cols + 8 * tid, S);
     }
 }
 
-// CTAs of the backward kernel: its threads hold V vectors each.
-int bwd_vectors(int64_t cols) { return cols <= 4096 ? 1 : cols <= 8192 ? 2 : 4; }
-uint32_t bwd_threads(int64_t cols) {
-    const int64_t v = bwd_vectors(cols), nv = cols / 8;
-    return static_cast<uint32_t>(((nv + v - 1) / v + 31) / 32 * 32);
+// 1024 < columns <= 8192: the ring. GROUPS groups of THREADS threads take the CTA's rows in turn;
+// a thread keeps its V vectors' column sums in registers for all of its group's rows.
+template <int V, uint32_t THREADS, uint32_t GROUPS>
+__global__ void __launch_bounds__(THREADS* GROUPS + 32, 1)
+    norm_backward_ring_kernel(const __grid_constant__ Bwd p, uint32_t stages, uint32_t* err) {
+    constexpr uint32_t kWarps = THREADS / 32;
+    extern __shared__ uint4 ring_smem[];
+    __shared__ Ring ring;
+    __shared__ float4 red[GROUPS][2][kWarps];
+    const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
+    const uint32_t nv = p.cols / 8;
+    // shared memory: column factors w | c in f32, stages of dn | x | du | y | gate row
+    float* const w = reinterpret_cast<float*>(ring_smem);
+    float* const c = w + p.cols;
+    uint4* const stage0 = ring_smem + 4 * nv;
+    const uint32_t arrays = 2 + (p.du ? 1 : 0) + (p.y ? 1 : 0) + (p.gate_stride ? 1 : 0);
+
+    ptxstd::pdl_launch_dependents();
+    if (tid == 0) init_ring(ring, stages, kWarps);
+    ptxstd::pdl_wait();
+    for (uint32_t i = tid; i < nv; i += blockDim.x) {
+        const Factors f = column_factors(p, i);
+        store_oct(w + 8 * i, f.w);
+        store_oct(c + 8 * i, f.c);
+    }
+    __syncthreads();
+
+    const uint32_t g = warp / kWarps;
+    if (g == GROUPS) {
+        if (lane == 0) {
+            const Sources s = {{p.dn, p.x, p.du, p.y, p.gate_stride ? p.gate : nullptr}, arrays};
+            produce_rows(ring, reinterpret_cast<uint8_t*>(stage0), stages, s, p.rows, p.cols, err,
+                         kDetailBwdProducer);
+        }
+        return;
+    }
+    const uint32_t t = tid - g * THREADS, gw = t >> 5;
+    const float inv_d = 1.0f / static_cast<float>(p.cols);
+    Oct dw[V], S[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[j] = S[j] = kZeroOct;
+    uint32_t stage = g % stages, phase = (g / stages) & 1u, flip = 0;
+    const uint32_t step = GROUPS * gridDim.x;
+    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows; row += step, flip ^= 1u) {
+        const float rx = p.rstd[row], ry = p.w_post ? p.rstd_post[row] : 1.0f;
+        ring_wait(ring, stage, phase, err, kDetailBwdConsumer);
+        __syncwarp();
+        const uint4* const dns = stage0 + static_cast<size_t>(stage) * arrays * nv;
+        const uint4* const xs = dns + nv;
+        const uint4* const dus = xs + nv;
+        const uint4* const ys = dus + (p.du ? nv : 0);
+        const uint4* const gs = p.gate_stride ? ys + nv : nullptr;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        Sums s;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = t + j * THREADS;
+            if (i < nv)
+                sums8(s, dns[i], p.du ? dus[i] : zero, xs[i], p.y ? ys[i] : zero,
+                      {load_oct(w + 8 * i), load_oct(c + 8 * i)}, p.w_post, gs ? gs + i : nullptr);
+        }
+        const float4 sum = group_sum4<kWarps>(s, red[g][flip], gw, lane, kWarps, g);
+        const RowFactors r = row_factors(sum, rx, ry, inv_d);
+        const size_t base = static_cast<size_t>(row) * p.cols;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = t + j * THREADS;
+            if (i < nv)
+                grads8(p, r, dns[i], p.du ? dus[i] : zero, xs[i], p.y ? ys[i] : zero,
+                       {load_oct(w + 8 * i), load_oct(c + 8 * i)}, gs ? gs + i : nullptr,
+                       base + 8 * i, dw[j], S[j]);
+        }
+        __syncwarp();
+        if (lane == 0) ptxstd::mbar_arrive(&ring.empty[stage]);
+        stage += GROUPS;
+        while (stage >= stages) {
+            stage -= stages;
+            phase ^= 1u;
+        }
+    }
+    float* out = p.partial + static_cast<size_t>(blockIdx.x * GROUPS + g) * p.sums * p.cols;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const uint32_t i = t + j * THREADS;
+        if (i >= nv) continue;
+        store_oct(out + 8 * i, dw[j]);
+        if (p.sums > 1) store_oct(out + p.cols + 8 * i, S[j]);
+    }
 }
-int64_t bwd_grid(int64_t rows, int64_t cols) {
-    const int64_t per_sm = cols > 8192 ? 1 : 1024 / bwd_threads(cols) > 8 ? 8 : 1024 / bwd_threads(cols);
-    const int64_t g = static_cast<int64_t>(ptxstd::sm_count()) * per_sm;
-    return rows < g ? rows : g;
+
+// How a backward call runs, by its sizes: the grid and the groups that write partial sums.
+struct BwdPlan {
+    bool ring;
+    uint32_t grid, groups;
+};
+BwdPlan bwd_plan(int64_t rows, int64_t cols) {
+    const int64_t sms = ptxstd::sm_count();
+    BwdPlan b = {};
+    b.ring = cols > 1024 && cols <= 8192;
+    b.groups = b.ring && cols <= 4096 ? 2 : 1;
+    const int64_t grid = cols <= 1024 ? 8 * sms : sms;  // 128-thread blocks: eight per SM
+    b.grid = static_cast<uint32_t>(rows < grid ? rows : grid);
+    return b;
 }
 
 template <int V>
-int launch_bwd(const Bwd& p, uint32_t grid, uint32_t threads, cudaStream_t stream) {
+int launch_bwd(const Bwd& p, uint32_t grid, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    ptxstd::set_pdl(cfg, attr, grid, threads, stream);
-    if (V == 4) {
+    const uint32_t nv = p.cols / 8;
+    ptxstd::set_pdl(cfg, attr, grid, ((nv + V - 1) / V + 31) / 32 * 32, stream);
+    if (V > 1) {
         cfg.dynamicSmemBytes = static_cast<size_t>(p.sums) * p.cols * 4;
         const int st = ptxstd::set_max_dynamic_smem(
-            reinterpret_cast<const void*>(norm_backward_kernel<V>), 3 * 16384 * 4);
+            reinterpret_cast<const void*>(norm_backward_kernel<V>), 2 * 16384 * 4);
         if (st) return st;
     }
     if (cudaLaunchKernelEx(&cfg, norm_backward_kernel<V>, p) != cudaSuccess) return PTXSTD_ECUDA;
+    return ptxstd::launch_status();
+}
+
+template <int V, uint32_t THREADS, uint32_t GROUPS>
+int launch_bwd_ring(const Bwd& p, uint32_t grid, cudaStream_t stream) {
+    auto* kernel = norm_backward_ring_kernel<V, THREADS, GROUPS>;
+    const int st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes);
+    if (st) return st;
+    uint32_t* err = ptxstd::device_error_word();
+    if (!err) return PTXSTD_ECUDA;
+    const size_t vec = static_cast<size_t>(p.cols) * 2, fixed = 4 * vec;
+    const size_t row = vec * (2 + (p.du ? 1 : 0) + (p.y ? 1 : 0) + (p.gate_stride ? 1 : 0));
+    // at most 8192 columns: beside 64 KB of factors, two rows of 64 KB or one of 80 KB
+    const uint32_t stages = ring_stages(fixed, row);
+    if (stages < GROUPS) return PTXSTD_EINVAL;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    ptxstd::set_pdl(cfg, attr, grid, THREADS * GROUPS + 32, stream);
+    cfg.dynamicSmemBytes = fixed + stages * row;
+    if (cudaLaunchKernelEx(&cfg, kernel, p, stages, err) != cudaSuccess) return PTXSTD_ECUDA;
     return ptxstd::launch_status();
 }
 
@@ -467,9 +877,25 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
     if (nv <= 32) return launch_fwd<1, true>(p, 32, s);
     if (nv <= 64) return launch_fwd<2, true>(p, 32, s);
     if (nv <= 128) return launch_fwd<4, true>(p, 32, s);
-    // few rows: one vector per thread (the row's latency counts); many rows: four (fewer threads
-    // per row, more loads in flight per thread)
-    const int v = nv > 2048 || rows > 296 ? 4 : nv > 1024 ? 2 : 1;
+    // Many rows: the ring. 8192 x 8192 with everything on, E4M3 out: 00 us against 99 us for the
+    // row-per-block kernel below; with fewer rows than the GPU holds groups the latter starts
+    // sooner.
+    if (rows >= 4 * ptxstd::sm_count() && nv <= 4 * kGroupThreads) {
+        const bool per_row = d_gate && p.gate_stride;
+        const size_t vec = static_cast<size_t>(cols) * 2;
+        const size_t fixed = vec * (1 + (d_w_post ? 1 : 0) + (d_gate && !per_row ? 1 : 0));
+        const size_t row_bytes = vec * (1 + (d_y ? 1 : 0) + (per_row ? 1 : 0));
+        const uint32_t stages = ring_stages(fixed, row_bytes);
+        if (stages >= kGroups) {
+            const size_t smem = fixed + stages * row_bytes;
+            if (nv <= kGroupThreads) return launch_fwd_ring<1>(p, stages, smem, s);
+            if (nv <= 2 * kGroupThreads) return launch_fwd_ring<2>(p, stages, smem, s);
+            return launch_fwd_ring<4>(p, stages, smem, s);
+        }
+    }
+    // One row per block: one vector per thread while the block can be that large (a row's latency
+    // counts when there are few), else as many as the row needs.
+    const int v = nv > 2048 ? 4 : nv > 1024 ? 2 : 1;
     const uint32_t threads = ((nv + v - 1) / v + 31) / 32 * 32;
     if (v == 1) return launch_fwd<1, false>(p, threads, s);
     if (v == 2) return launch_fwd<2, false>(p, threads, s);
@@ -478,7 +904,8 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
 
 extern "C" size_t ptxstd_rmsnorm_residual_backward_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0 || cols % 8 || cols > 16384) return 0;
-    return static_cast<size_t>(bwd_grid(rows, cols)) * 3 * static_cast<size_t>(cols) * 4;
+    const BwdPlan b = bwd_plan(rows, cols);
+    return static_cast<size_t>(b.grid) * b.groups * 2 * static_cast<size_t>(cols) * 4;
 }
 
 extern "C" int ptxstd_rmsnorm_residual_backward(
@@ -503,9 +930,9 @@ extern "C" int ptxstd_rmsnorm_residual_backward(
         misaligned(d_gate) || misaligned(d_dx) || misaligned(d_dw) || misaligned(d_dy) ||
         misaligned(d_dw_post) || misaligned(d_dgate) || misaligned(d_workspace))
         return PTXSTD_EINVAL;
-    const int64_t grid = bwd_grid(rows, cols);
-    if (workspace_bytes < static_cast<size_t>(grid) * 3 * static_cast<size_t>(cols) * 4)
+    if (workspace_bytes < ptxstd_rmsnorm_residual_backward_workspace_bytes(rows, cols))
         return PTXSTD_EINVAL;
+    const BwdPlan plan = bwd_plan(rows, cols);
     Bwd p = {};
     p.dn = d_dn;
     p.du = d_dx_out;
@@ -521,28 +948,35 @@ extern "C" int ptxstd_rmsnorm_residual_backward(
     p.scale = scale;
     p.rows = static_cast<uint32_t>(rows);
     p.cols = static_cast<uint32_t>(cols);
-    p.sums = 1;
-    // a single row's gate is a vector gate either way: its gradient is f32 [cols]
+    // a single row's gate is a gate of all rows either way: its gradient is f32 [cols]
     const bool vector_gate = d_gate && gate_rows == 1;
-    if (d_w_post) p.post_at = p.sums++;
-    if (vector_gate) p.gate_at = p.sums++;
-    if (d_gate && !vector_gate) p.dgate_rows = static_cast<uint16_t*>(d_dgate);
-    p.gate_stride = vector_gate ? 0 : static_cast<size_t>(cols);
+    if (d_gate && !vector_gate) {
+        p.dgate_rows = static_cast<uint16_t*>(d_dgate);
+        p.gate_stride = static_cast<size_t>(cols);
+    }
+    p.sums = d_w_post || vector_gate ? 2 : 1;
     p.partial = static_cast<float*>(d_workspace);
     auto s = static_cast<cudaStream_t>(stream);
-    const uint32_t threads = bwd_threads(cols), g = static_cast<uint32_t>(grid);
-    const int v = bwd_vectors(cols);
-    int st = v == 1 ? launch_bwd<1>(p, g, threads, s)
-             : v == 2 ? launch_bwd<2>(p, g, threads, s) : launch_bwd<4>(p, g, threads, s);
+    int st;
+    if (!plan.ring)
+        st = cols <= 1024 ? launch_bwd<1>(p, plan.grid, s) : launch_bwd<4>(p, plan.grid, s);
+    else if (cols <= 2048)
+        st = launch_bwd_ring<1, 256, 2>(p, plan.grid, s);
+    else if (cols <= 4096)
+        st = launch_bwd_ring<2, 256, 2>(p, plan.grid, s);
+    else
+        st = launch_bwd_ring<2, 512, 1>(p, plan.grid, s);
     if (st) return st;
     ptxstd::Reduce r = {};
     r.partial = p.partial;
-    r.P = g;
-    r.cols = p.sums * p.cols;
-    r.split0 = p.cols;
-    r.split1 = p.cols * (d_w_post ? 2 : 1);
+    r.P = plan.grid * plan.groups;
+    r.sums = p.sums;
+    r.cols = p.cols;
+    r.scale = scale;
     r.o0 = d_dw;
     r.o1 = d_dw_post;
-    r.o2 = static_cast<float*>(d_dgate);
+    r.f1 = vector_gate ? d_gate : nullptr;
+    r.o2 = vector_gate ? static_cast<float*>(d_dgate) : nullptr;
+    r.f2 = d_w_post;
     return ptxstd::launch_reduce(r, s);
 }

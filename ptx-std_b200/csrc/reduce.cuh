@@ -8,8 +8,8 @@
 namespace ptxstd {
 
 // One-dimensional launch with programmatic stream serialisation; `attr` has room for one.
-inline void set_pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, uint32_t grid, uint32_t block,
-            cudaStream_t stream) {
+inline void set_pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, uint32_t grid,
+                    uint32_t block, cudaStream_t stream) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(grid);
@@ -19,40 +19,50 @@ inline void set_pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, uint32_t
     cfg.numAttrs = 1;
 }
 
-// out[c] = sum over the P partial rows of column c. `cols` counts all sums' columns; the first
-// `split0` belong to o0, up to `split1` to o1, the rest to o2. A block covers 32 columns with 8
-// groups of threads, each adding every 8th row; the groups' sums are added in order.
+// Sums over the P rows of partial [P][sums * cols]: o0 takes the first `cols` columns' sums; the
+// second `cols` columns' sums, times scale and a bf16 factor per column (null: 1), go to o1 and o2
+// (either may be null). A block covers 32 columns with 8 groups of threads, each adding every 8th
+// row; the groups' sums are added in order.
 struct Reduce {
     const float* partial;
     float *o0, *o1, *o2;
-    uint32_t P, cols, split0, split1;
+    const uint16_t *f1, *f2;
+    float scale;
+    uint32_t P, sums, cols;
 };
 constexpr uint32_t kRedGroups = 8;
-static __global__ void __launch_bounds__(32 * kRedGroups) reduce_kernel(const __grid_constant__ Reduce p) {
+static __global__ void __launch_bounds__(32 * kRedGroups)
+    reduce_kernel(const __grid_constant__ Reduce p) {
     __shared__ float part[kRedGroups][32];
     const uint32_t lane = lane_id(), g = threadIdx.x >> 5;
-    const uint32_t c = blockIdx.x * 32 + lane;
+    const uint32_t c = blockIdx.x * 32 + lane, width = p.sums * p.cols;
     pdl_launch_dependents();
     pdl_wait();
     float s = 0.0f;
-    if (c < p.cols)
+    if (c < width) {
+#pragma unroll 8
         for (uint32_t r = g; r < p.P; r += kRedGroups)
-            s += p.partial[static_cast<size_t>(r) * p.cols + c];
+            s += p.partial[static_cast<size_t>(r) * width + c];
+    }
     part[g][lane] = s;
     __syncthreads();
-    if (g == 0 && c < p.cols) {
+    if (g || c >= width) return;
 #pragma unroll
-        for (uint32_t k = 1; k < kRedGroups; ++k) s += part[k][lane];
-        if (c < p.split0) p.o0[c] = s;
-        else if (c < p.split1) p.o1[c - p.split0] = s;
-        else p.o2[c - p.split1] = s;
+    for (uint32_t k = 1; k < kRedGroups; ++k) s += part[k][lane];
+    if (c < p.cols) {
+        p.o0[c] = s;
+        return;
     }
+    const uint32_t i = c - p.cols;
+    s *= p.scale;
+    if (p.o1) p.o1[i] = p.f1 ? s * data_types::bf16_lo(p.f1[i]) : s;
+    if (p.o2) p.o2[i] = p.f2 ? s * data_types::bf16_lo(p.f2[i]) : s;
 }
 
 inline int launch_reduce(const Reduce& r, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    set_pdl(cfg, attr, (r.cols + 31) / 32, 32 * kRedGroups, stream);
+    set_pdl(cfg, attr, (r.sums * r.cols + 31) / 32, 32 * kRedGroups, stream);
     if (cudaLaunchKernelEx(&cfg, reduce_kernel, r) != cudaSuccess) return PTXSTD_ECUDA;
     return launch_status();
 }

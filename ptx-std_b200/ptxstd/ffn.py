@@ -60,33 +60,51 @@ def _want_mx(q, sf, name: str, cols: int | None = None) -> tuple[int, int]:
     return rows, k
 
 
-def _ptrs(stream, *tensors):
-    """Device pointers (0 for None) and the stream handle; every tensor has to be contiguous and
-    on the current device."""
-    torch = _torch()
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+def _ins(*tensors) -> list[int]:
+    """Device pointers of the inputs (0 for None), each contiguous and on the current device."""
     out = []
+    dev = None
     for t in tensors:
         if t is None:
             out.append(0)
             continue
-        if not t.is_cuda:
-            raise TypeError("expected a CUDA tensor")
-        if t.get_device() != dev:
-            raise ValueError(f"tensor on cuda:{t.get_device()}, but the current device is "
-                             f"cuda:{dev}")
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise TypeError("expected a CUDA tensor")
+            dev = _torch().cuda.current_device()
+            if d != dev:
+                raise ValueError(f"tensor on cuda:{d}, but the current device is cuda:{dev}")
         if not t.is_contiguous():
             raise ValueError("expected a contiguous tensor")
         out.append(t.data_ptr())
-    s = stream if stream is not None else torch.cuda.current_stream()
-    out.append(s.cuda_stream)
     return out
 
 
+def _outs(*tensors) -> list[int]:
+    """Device pointers of tensors allocated here."""
+    return [0 if t is None else t.data_ptr() for t in tensors]
+
+
+def _handle(stream, like) -> int:
+    """The cudaStream_t of `stream`, or of the current stream of the tensor's device."""
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(like.get_device())
+
+
+def _new(rows: int, cols: int, dtype, device):
+    """An uninitialised [rows, cols] tensor (empty_strided is the cheapest of torch's calls)."""
+    return _torch().empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
+def _new1(n: int, dtype, device):
+    return _torch().empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
 def _mx_empty(rows: int, cols: int, device):
-    torch = _torch()
-    return (torch.empty((rows, cols), dtype=torch.uint8, device=device),
-            torch.empty(sf_numel(rows, cols), dtype=torch.uint8, device=device))
+    u8 = _torch().uint8
+    return _new(rows, cols, u8, device), _new1(sf_numel(rows, cols), u8, device)
 
 
 def rmsnorm_residual(x, w, y=None, w_post=None, gate=None, scale: float = 1.0, eps: float = 1e-6,
@@ -115,7 +133,8 @@ def rmsnorm_residual(x, w, y=None, w_post=None, gate=None, scale: float = 1.0, e
     else:
         _want(gate, "gate", bf, (cols,))
     t = None if elem_type is None else _out_type(elem_type)
-    dev = x.device
+    px, py, pwp, pg, pw = _ins(x, y, w_post, gate, w)
+    dev, s = x.device, _handle(stream, x)
     x_out = torch.empty_like(x) if y is not None else None
     n = q = sf = None
     if t is None:
@@ -123,12 +142,11 @@ def rmsnorm_residual(x, w, y=None, w_post=None, gate=None, scale: float = 1.0, e
     elif sf_layout == 1:
         q, sf = _mx_empty(rows, cols, dev)
     else:
-        q = torch.empty((rows, cols), dtype=torch.uint8, device=dev)
-        sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
-    rstd_post = torch.empty(rows, dtype=torch.float32, device=dev) if w_post is not None else None
-    px, py, pwp, pg, pw, pxo, pn, pq, psf, pr, prp, s = _ptrs(
-        stream, x, y, w_post, gate, w, x_out, n, q, sf, rstd, rstd_post)
+        q = _new(rows, cols, torch.uint8, dev)
+        sf = _new(rows, cols // 32, torch.uint8, dev)
+    rstd = _new1(rows, torch.float32, dev)
+    rstd_post = _new1(rows, torch.float32, dev) if w_post is not None else None
+    pxo, pn, pq, psf, pr, prp = _outs(x_out, n, q, sf, rstd, rstd_post)
     check(lib().ptxstd_rmsnorm_residual(px, py, pwp, pg, gate_rows, scale, pw, eps, rows, cols,
                                         pxo, pn, t or 0, pq, psf, sf_layout, pr, prp, s),
           "rmsnorm_residual")
@@ -165,17 +183,19 @@ def rmsnorm_residual_backward(dn, x_out, w, stats, dx_out=None, y=None, w_post=N
         got = rmsnorm_residual_backward(dn, x_out, w, stats, dx_out, y, w_post, gate.view(cols),
                                         scale, stream)
         return (*got[:4], got[4].to(bf).view(1, cols))
+    pdn, pdu, px, pw, pr, py, pwp, prp, pg = _ins(dn, dx_out, x_out, w, rstd, y, w_post, rstd_post,
+                                                  gate)
+    s = _handle(stream, dn)
     dx = torch.empty_like(dn)
-    dw = torch.empty(cols, dtype=f32, device=dev)
+    dw = _new1(cols, f32, dev)
     dy = torch.empty_like(dn) if y is not None else None
-    dwp = torch.empty(cols, dtype=f32, device=dev) if w_post is not None else None
+    dwp = _new1(cols, f32, dev) if w_post is not None else None
     dg = None
     if gate is not None:
-        dg = torch.empty_like(gate) if per_row else torch.empty(cols, dtype=f32, device=dev)
+        dg = torch.empty_like(gate) if per_row else _new1(cols, f32, dev)
     nbytes = lib().ptxstd_rmsnorm_residual_backward_workspace_bytes(rows, cols)
-    ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device=dev)
-    (pdn, pdu, px, pw, pr, py, pwp, prp, pg, pdx, pdw, pdy, pdwp, pdg, pws, s) = _ptrs(
-        stream, dn, dx_out, x_out, w, rstd, y, w_post, rstd_post, gate, dx, dw, dy, dwp, dg, ws)
+    ws = _new1(max(16, nbytes), torch.uint8, dev)
+    pdx, pdw, pdy, pdwp, pdg, pws = _outs(dx, dw, dy, dwp, dg, ws)
     check(lib().ptxstd_rmsnorm_residual_backward(
         pdn, pdu, px, pw, pr, py, pwp, prp, pg, rows if per_row else 1, scale, rows, cols, pdx,
         pdw, pdy, pdwp, pdg, pws, nbytes, s), "rmsnorm_residual_backward")
@@ -194,17 +214,16 @@ def gemm_mx_epilogue(a, a_type, sfa, b, b_type, sfb, bias=None, act="none", resi
     N, _ = _want_mx(b, sfb, "b", K)
     _want(bias, "bias", torch.bfloat16, (N,))
     _want(residual, "residual", torch.bfloat16, (M, N))
-    dev = a.device
+    t = 0 if elem_type is None else _out_type(elem_type)
+    pa, psa, pb, psb, pbias, pres = _ins(a, sfa, b, sfb, bias, residual)
+    dev, s = a.device, _handle(stream, a)
     c = q = sf = None
-    t = 0
     if elem_type is None:
-        c = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        c = _new(M, N, torch.bfloat16, dev)
     else:
-        t = _out_type(elem_type)
         q, sf = _mx_empty(M, N, dev)
-    pre = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if save_pre else None
-    pa, psa, pb, psb, pbias, pres, pc, ppre, pq, psf, s = _ptrs(
-        stream, a, sfa, b, sfb, bias, residual, c, pre, q, sf)
+    pre = _new(M, N, torch.bfloat16, dev) if save_pre else None
+    pc, ppre, pq, psf = _outs(c, pre, q, sf)
     check(lib().ptxstd_gemm_mx_epilogue(pa, ta, psa, pb, tb, psb, pbias, f, pres, pc, ppre, t, pq,
                                         psf, M, N, K, s), "gemm_mx_epilogue")
     r = c if elem_type is None else (q, sf)
@@ -223,19 +242,17 @@ def gemm_mx_gated(a, a_type, sfa, w_gate, sf_gate, w_up, sf_up, w_type, act="sil
     F, _ = _want_mx(w_gate, sf_gate, "w_gate", K)
     if _want_mx(w_up, sf_up, "w_up", K)[0] != F:
         raise ValueError("w_gate and w_up have different numbers of rows")
-    dev = a.device
+    t = 0 if elem_type is None else _out_type(elem_type)
+    pa, psa, pg, psg, pu, psu = _ins(a, sfa, w_gate, sf_gate, w_up, sf_up)
+    dev, s = a.device, _handle(stream, a)
     h = q = sf = gate = up = None
-    t = 0
     if elem_type is None:
-        h = torch.empty((M, F), dtype=torch.bfloat16, device=dev)
+        h = _new(M, F, torch.bfloat16, dev)
     else:
-        t = _out_type(elem_type)
         q, sf = _mx_empty(M, F, dev)
     if save:
-        gate = torch.empty((M, F), dtype=torch.bfloat16, device=dev)
-        up = torch.empty((M, F), dtype=torch.bfloat16, device=dev)
-    pa, psa, pg, psg, pu, psu, ph, pgate, pup, pq, psf, s = _ptrs(
-        stream, a, sfa, w_gate, sf_gate, w_up, sf_up, h, gate, up, q, sf)
+        gate, up = _new(M, F, torch.bfloat16, dev), _new(M, F, torch.bfloat16, dev)
+    ph, pgate, pup, pq, psf = _outs(h, gate, up, q, sf)
     check(lib().ptxstd_gemm_mx_gated(pa, ta, psa, pg, psg, pu, psu, tw, f, ph, pgate, pup, t, pq,
                                      psf, M, F, K, s), "gemm_mx_gated")
     r = h if elem_type is None else (q, sf)
@@ -255,18 +272,18 @@ def act_backward_mx(dh, gate, up=None, act="silu", elem_type="e5m2", bias_grad: 
     rows, cols = dh.shape
     _want(gate, "gate", torch.bfloat16, (rows, cols))
     _want(up, "up", torch.bfloat16, (rows, cols))
-    dev = dh.device
+    pdh, pg, pu = _ins(dh, gate, up)
+    dev, s = dh.device, _handle(stream, dh)
     W, R = cols * (1 if up is None else 2), -(-rows // 32) * 32
     q, sf = _mx_empty(rows, W, dev)
     qt, sft = _mx_empty(W, R, dev)
     db = ws = None
     nbytes = 0
     if bias_grad:
-        db = torch.empty(W, dtype=torch.float32, device=dev)
+        db = _new1(W, torch.float32, dev)
         nbytes = lib().ptxstd_act_backward_mx_workspace_bytes(rows, cols, up is not None, 1)
-        ws = torch.empty(max(16, nbytes), dtype=torch.uint8, device=dev)
-    pdh, pg, pu, pq, psf, pqt, psft, pdb, pws, s = _ptrs(stream, dh, gate, up, q, sf, qt, sft, db,
-                                                         ws)
+        ws = _new1(max(16, nbytes), torch.uint8, dev)
+    pq, psf, pqt, psft, pdb, pws = _outs(q, sf, qt, sft, db, ws)
     check(lib().ptxstd_act_backward_mx(f, pdh, pg, pu, rows, cols, t, pq, psf, pqt, psft, pdb, pws,
                                        nbytes, s), "act_backward_mx")
     return ((q, sf), (qt, sft), db) if bias_grad else ((q, sf), (qt, sft))
@@ -280,9 +297,10 @@ def quantize_mx_t(x, elem_type, stream=None):
         raise TypeError("expected a 2-D bfloat16 tensor")
     t = _out_type(elem_type)
     rows, cols = x.shape
+    (px,) = _ins(x)
     qt, sft = _mx_empty(cols, -(-rows // 32) * 32, x.device)
-    px, pq, psf, s = _ptrs(stream, x, qt, sft)
-    check(lib().ptxstd_quantize_mx_t(px, rows, cols, t, pq, psf, s), "quantize_mx_t")
+    check(lib().ptxstd_quantize_mx_t(px, rows, cols, t, *_outs(qt, sft), _handle(stream, x)),
+          "quantize_mx_t")
     return qt, sft
 
 

@@ -78,7 +78,7 @@ def test_c_refusals(ptxstd_lib):
                                                   dx, dw, dy, dwp, dg, ws, nb, None)
 
     for kw in (dict(rows=0), dict(cols=20), dict(cols=16392), dict(dn=0), dict(r=0), dict(ws=0),
-               dict(nb=8 * 3 * 64 * 4 - 1), dict(dy=0), dict(y=0), dict(y=0, dy=0, wp=p),
+               dict(nb=8 * 2 * 64 * 4 - 1), dict(dy=0), dict(y=0), dict(y=0, dy=0, wp=p),
                dict(wp=p), dict(wp=p, rp=p), dict(g=p), dict(g=p, dg=p, gr=2), dict(dx=p + 8)):
         assert nback(**kw) == E, kw
 
@@ -89,7 +89,7 @@ def test_workspace_sizes(ptxstd_lib):
     assert f(1, 64, 0, 1) == 256 and f(129, 64, 1, 1) == 1024
     assert f(129, 64, 1, 0) == 0 and f(0, 64, 0, 1) == 0
     g = L.ptxstd_rmsnorm_residual_backward_workspace_bytes
-    assert g(1, 64) == 3 * 64 * 4 and g(8, 64) == 8 * 3 * 64 * 4
+    assert g(1, 64) == 2 * 64 * 4 and g(8, 64) == 8 * 2 * 64 * 4
     assert g(0, 64) == 0 and g(8, 16392) == 0
     assert g(1 << 20, 8192) < 64 << 20
 
