@@ -55,16 +55,14 @@ __device__ __forceinline__ void put8(float* row, uint32_t l, const float (&v)[8]
 // One row block (four lanes) of D at (row, first column col of this lane's eight values).
 __device__ __forceinline__ void row_block(const Params& p, const float (&v)[8], uint32_t row,
                                           uint32_t col, bool on, bool in_tiles, uint32_t lane) {
-    const uint32_t code = mx::scale_code(mx::amax_quad(mx::amax_of(v)), mx::emax_of(p.type));
-    const float inv = dt::ue8m0_inverse(code);
+    const mx::Scale sc = mx::scale_of(mx::amax_quad(mx::amax_of(v)), mx::emax_of(p.type));
     if (on)
         *reinterpret_cast<uint2*>(p.q + static_cast<size_t>(row) * p.W + col) =
-            make_uint2(mx::pack4(p.type, v[0], v[1], v[2], v[3], inv),
-                       mx::pack4(p.type, v[4], v[5], v[6], v[7], inv));
+            mx::pack8(p.type, v, sc.inv);
     if ((lane & 3u) == 0 && in_tiles) {
         const uint32_t s = col / 32;
         p.sf[mx::word_offset(row, s >> 2, mx::tiles_k(p.W / 32)) + (s & 3u)] =
-            on ? static_cast<uint8_t>(code) : 0;
+            on ? static_cast<uint8_t>(sc.code) : 0;
     }
 }
 
@@ -162,25 +160,20 @@ __global__ void __launch_bounds__(kThreads)
             v[i] = src[i * kCols];
             sum += v[i];
         }
-        const uint32_t code = mx::scale_code(mx::amax_of(v), emax);
-        const float inv = dt::ue8m0_inverse(code);
+        const mx::Scale sc = mx::scale_of(mx::amax_of(v), emax);
         const uint32_t feature = h * p.cols + col0 + f;
         if (col0 + f < p.cols) {
             if (t0 < p.R) {
                 uint4* dst = reinterpret_cast<uint4*>(p.qt + static_cast<size_t>(feature) * p.R + t0);
 #pragma unroll
                 for (uint32_t c = 0; c < 2; ++c) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const uint32_t i = 16 * c + 4 * k;
-                        w[k] = mx::pack4(p.type, v[i], v[i + 1], v[i + 2], v[i + 3], inv);
-                    }
-                    dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                    const uint2 lo = mx::pack8(p.type, v + 16 * c, sc.inv);
+                    const uint2 hi = mx::pack8(p.type, v + 16 * c + 8, sc.inv);
+                    dst[c] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                 }
             }
             p.sft[mx::word_offset(feature, rt, kt) + b] =
-                t0 < p.R ? static_cast<uint8_t>(code) : 0;
+                t0 < p.R ? static_cast<uint8_t>(sc.code) : 0;
         }
         if (MODE != kTranspose && p.partial) {
             sums[b][f] = sum;

@@ -169,20 +169,17 @@ struct Out {
 #pragma unroll
             for (uint32_t i = 0; i < 32; i += 2)
                 m = mx::amax(m, f(r[FIRST + 32 * h + i]), f(r[FIRST + 32 * h + i + 1]));
-            const uint32_t code = mx::scale_code(m, emax);
-            const float inv = dt::ue8m0_inverse(code);
-            if (row < M && col0 + 32 * h < N) codes |= code << (8 * h);
+            const mx::Scale sc = mx::scale_of(m, emax);
+            if (row < M && col0 + 32 * h < N) codes |= sc.code << (8 * h);
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c) {
-                uint32_t p[4];
+                float v[16];
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    const uint32_t i = FIRST + 32 * h + 16 * c + 4 * k;
-                    p[k] = mx::pack4(type, f(r[i]), f(r[i + 1]), f(r[i + 2]), f(r[i + 3]), inv);
-                }
+                for (uint32_t k = 0; k < 16; ++k) v[k] = f(r[FIRST + 32 * h + 16 * c + k]);
+                const uint2 lo = mx::pack8(type, v, sc.inv), hi = mx::pack8(type, v + 8, sc.inv);
                 if (any)
-                    ptxstd::st_shared_v4(stg + StageBox::offset(lane, 2 * h + c), p[0], p[1], p[2],
-                                         p[3]);
+                    ptxstd::st_shared_v4(stg + StageBox::offset(lane, 2 * h + c), lo.x, lo.y, hi.x,
+                                         hi.y);
             }
         }
         if (any) {
@@ -807,15 +804,12 @@ __global__ void __launch_bounds__(kThreads)
             }
             if (on && e.c) store_bf16(e.c, y);
             if (e.q) {
-                const uint32_t code = mx::scale_code(mx::amax_quad(mx::amax_of(y)), mx::emax_of(e.q_type));
-                const float inv = dt::ue8m0_inverse(code);
-                if (on)
-                    *reinterpret_cast<uint2*>(e.q + at) =
-                        make_uint2(mx::pack4(e.q_type, y[0], y[1], y[2], y[3], inv),
-                                   mx::pack4(e.q_type, y[4], y[5], y[6], y[7], inv));
+                const mx::Scale sc =
+                    mx::scale_of(mx::amax_quad(mx::amax_of(y)), mx::emax_of(e.q_type));
+                if (on) *reinterpret_cast<uint2*>(e.q + at) = mx::pack8(e.q_type, y, sc.inv);
                 if ((lane & 3u) == 0 && t < upto)
                     e.sfq[mx::word_offset(tok0 + t, block, q_tiles_k) + ((tid & 15u) >> 2)] =
-                        on ? static_cast<uint8_t>(code) : 0;
+                        on ? static_cast<uint8_t>(sc.code) : 0;
             }
         }
     }

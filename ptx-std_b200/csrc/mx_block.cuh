@@ -116,11 +116,25 @@ __device__ __forceinline__ float amax_quad(float m) {
     m = amax(m, __shfl_xor_sync(0xffffffffu, m, 1));
     return amax(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
-// Scale code of a block from its largest magnitude: floor-pow2 (TowardZero, SaturateFinite) minus
-// the format's emax (E4M3 8, E5M2 15), clamped at 0; NaN stays NaN.
-__device__ __forceinline__ uint32_t scale_code(float amax, uint32_t emax) {
-    const uint32_t u = data_types::ue8m0_from_f32<false, true>(amax);
-    return u == 0xFFu ? 0xFFu : (u > emax ? u - emax : 0u);
+// Scale of a block from its largest magnitude: code = floor(log2 amax) + 127 - emax (E4M3 8,
+// E5M2 15), clamped at 0, and inv = 2^-(code-127). The exponent field is the floor-pow2
+// (TowardZero) code already; an infinite amax takes the largest finite exponent
+// (SaturateFinite), a NaN gives the NaN code and a NaN factor. The code is at most 246, so inv is
+// a normal number.
+struct Scale {
+    uint32_t code;
+    float inv;
+};
+__device__ __forceinline__ Scale scale_of(float amax, uint32_t emax) {
+    const uint32_t bits = __float_as_uint(amax);
+    const uint32_t e = max(bits >> 23, emax);
+    Scale s = {e - emax, __uint_as_float((254u + emax - e) << 23)};
+    if (bits >= 0x7F800000u) {
+        const bool nan = bits > 0x7F800000u;
+        s.code = nan ? 0xFFu : 254u - emax;
+        s.inv = __uint_as_float(nan ? 0x7FFFFFFFu : emax << 23);
+    }
+    return s;
 }
 // Two values times 2^-(code-127) (exact but for subnormal results) as a code pair.
 template <uint32_t T>
@@ -129,10 +143,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, float inv) {
     return T == kE4m3 ? data_types::e4m3x2_from_f32<false>(v.x, v.y)
                       : data_types::e5m2x2_from_f32<false>(v.x, v.y);
 }
-__device__ __forceinline__ uint32_t pack4(uint32_t type, float a, float b, float c, float d,
-                                          float inv) {
-    return type == kE4m3 ? pack2<kE4m3>(a, b, inv) | (pack2<kE4m3>(c, d, inv) << 16)
-                         : pack2<kE5m2>(a, b, inv) | (pack2<kE5m2>(c, d, inv) << 16);
+// Eight values as eight codes.
+template <uint32_t T>
+__device__ __forceinline__ uint2 pack8(const float* v, float inv) {
+    return make_uint2(pack2<T>(v[0], v[1], inv) | (pack2<T>(v[2], v[3], inv) << 16),
+                      pack2<T>(v[4], v[5], inv) | (pack2<T>(v[6], v[7], inv) << 16));
+}
+__device__ __forceinline__ uint2 pack8(uint32_t type, const float* v, float inv) {
+    return type == kE4m3 ? pack8<kE4m3>(v, inv) : pack8<kE5m2>(v, inv);
 }
 __host__ __device__ __forceinline__ uint32_t emax_of(uint32_t type) {
     return type == kE4m3 ? 8u : 15u;

@@ -100,13 +100,35 @@ __device__ __forceinline__ uint4 join8(const uint4& xv, const uint4& yv, const u
     return narrow(x);
 }
 
+// Where a row's scales go: the scale of vector i (eight columns) at sf[at(i)], written by the first
+// of the four lanes that hold a block.
+struct ScaleRow {
+    uint8_t* sf;
+    uint32_t blocked;
+    __device__ __forceinline__ ScaleRow(const Fwd& p, uint32_t row, size_t k_tiles)
+        : sf(nullptr), blocked(p.blocked) {
+        if (p.q)
+            sf = p.sf + (blocked ? mx::word_offset(row, 0, k_tiles)
+                                 : static_cast<size_t>(row) * (p.cols / 32));
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const {
+        return blocked ? (i >> 4) * 512 + ((i >> 2) & 3u) : i >> 2;
+    }
+    // The padding columns of a row's last scale tile.
+    __device__ __forceinline__ void pad(const Fwd& p, uint32_t tid) const {
+        const uint32_t blocks = p.cols / 32;
+        if (sf && blocked && tid < 3 && (blocks & 3u) + tid < 4 && (blocks & 3u))
+            sf[at(4 * (blocks + tid))] = 0;
+    }
+};
+
 // n = x' rx w of eight columns (vector i of the row), stored as bf16 and / or quantised. Every
 // lane of the warp calls it; lanes outside the row pass on = false and zeros. A block of 32 is the
 // vectors of four neighbouring lanes (cols % 32 == 0, so a block is inside the row or outside it
 // as a whole).
 __device__ __forceinline__ void finish8(const Fwd& p, const uint4& xv, const uint4& wv, float rx,
-                                        uint32_t row, size_t base, uint32_t i, bool on,
-                                        uint32_t lane, size_t k_tiles) {
+                                        size_t base, uint32_t i, bool on, uint32_t lane,
+                                        const ScaleRow& sr) {
     Oct n = widen(xv);
     const Oct w = widen(wv);
     const f32x2 r = pack2f(rx, rx);
@@ -121,21 +143,10 @@ __device__ __forceinline__ void finish8(const Fwd& p, const uint4& xv, const uin
         a[2 * k] = f.x;
         a[2 * k + 1] = f.y;
     }
-    const float m = mx::amax_quad(mx::amax_of(a));
-    const uint32_t code = on ? mx::scale_code(m, mx::emax_of(p.q_type)) : 0u;
-    const float inv = dt::ue8m0_inverse(code);
-    if (on)
-        *reinterpret_cast<uint2*>(p.q + base + 8 * i) =
-            make_uint2(mx::pack4(p.q_type, a[0], a[1], a[2], a[3], inv),
-                       mx::pack4(p.q_type, a[4], a[5], a[6], a[7], inv));
-    if (p.blocked) {
-        // four blocks' codes (16 lanes) as one word of the scale tile
-        uint32_t c = code | __shfl_down_sync(0xffffffffu, code, 4) << 8;
-        c |= __shfl_down_sync(0xffffffffu, c, 8) << 16;
-        if ((lane & 15u) == 0 && on)
-            *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, i >> 4, k_tiles)) = c;
-    } else if ((lane & 3u) == 0 && on) {
-        p.sf[static_cast<size_t>(row) * (p.cols / 32) + (i >> 2)] = static_cast<uint8_t>(code);
+    const mx::Scale sc = mx::scale_of(mx::amax_quad(mx::amax_of(a)), mx::emax_of(p.q_type));
+    if (on) {
+        *reinterpret_cast<uint2*>(p.q + base + 8 * i) = mx::pack8(p.q_type, a, sc.inv);
+        if ((lane & 3u) == 0) sr.sf[sr.at(i)] = static_cast<uint8_t>(sc.code);
     }
 }
 
@@ -145,6 +156,25 @@ __device__ __forceinline__ void pad_row(const Fwd& p, uint32_t row, uint32_t tid
     if (p.q && p.blocked && row < mx::padded_rows(p.rows))
         for (size_t t = tid; t < k_tiles; t += stride)
             *reinterpret_cast<uint32_t*>(p.sf + mx::word_offset(row, t, k_tiles)) = 0;
+}
+
+// scale w_post gate of eight columns (either may be null).
+__device__ __forceinline__ Oct branch_factor(const uint16_t* w_post, const uint16_t* gate,
+                                             float scale, uint32_t i) {
+    Oct f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.v[k] = pack2f(scale, scale);
+    if (w_post) {
+        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(w_post) + i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.v[k] = mul2(f.v[k], o.v[k]);
+    }
+    if (gate) {
+        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(gate) + i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.v[k] = mul2(f.v[k], o.v[k]);
+    }
+    return f;
 }
 
 // One row per warp or per block, straight from global memory: for few rows (a single row's
@@ -206,133 +236,158 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
     for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
     const float rx = rsqrtf(row_sum<WARP_ROW>(hsum2(s), red[1]) * inv_d + p.eps);
     if (p.rstd && tid == 0) p.rstd[row] = rx;
+    const ScaleRow sr(p, row, k_tiles);
+    sr.pad(p, tid);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const uint32_t i = tid + j * stride;
         const bool on = i < nv;
         const uint4 w = on ? __ldg(reinterpret_cast<const uint4*>(p.w) + i) : make_uint4(0, 0, 0, 0);
-        finish8(p, xv[j], w, rx, row, base, i, on, lane, k_tiles);
+        finish8(p, xv[j], w, rx, base, i, on, lane, sr);
     }
 }
 
 // ---- many rows: a ring of rows in shared memory ------------------------------------------------
-// One CTA per SM walks the rows blockIdx, blockIdx + grid, ...; a producer lane streams each row's
-// inputs into a ring of stages with bulk copies, and groups of consumer threads take the rows in
-// turn, so that the loads of later rows, one row's sums and another's stores overlap and up to
-// 200 KB per SM are in flight whatever the groups wait for. The column weights sit in shared
-// memory for the CTA's life.
+// One CTA per SM walks the rows blockIdx, blockIdx + grid, ...: its k-th row goes through stage
+// k % stages of a ring by bulk copies, and groups of threads take the rows in turn, so that one
+// row's sums, another's stores and the loads of later rows overlap. A group copies its row to
+// registers first; once it has met in the row's first sum, the stage is free and its first thread
+// sends the row `stages` further on into it. The ring is thus in flight nearly all of the time,
+// whatever the groups wait for. Column weights sit in shared memory for the CTA's life.
 constexpr uint32_t kRingBytes = 222 * 1024;
-constexpr uint32_t kMaxRing = 8;
-enum : uint32_t { kDetailFwdProducer = 0x4100, kDetailFwdConsumer = 0x4200,
-                  kDetailBwdProducer = 0x4300, kDetailBwdConsumer = 0x4400 };
-
-struct Ring {
-    uint64_t full[kMaxRing];
-    uint64_t empty[kMaxRing];
-    uint32_t abort;
-};
+constexpr uint32_t kMaxRing = 12;
+enum : uint32_t { kDetailFwd = 0x4200, kDetailBwd = 0x4400 };
 
 __device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
 }
 
-// A consumer warp's wait for a stage. After a timeout (recorded) the kernel runs on without
-// waiting, on whatever the stages hold, so that every barrier still sees all of its threads.
-__device__ __forceinline__ void ring_wait(Ring& r, uint32_t stage, uint32_t phase, uint32_t* err,
-                                          uint32_t detail) {
-    volatile uint32_t* abort_flag = &r.abort;
-    if (!*abort_flag && !ptxstd::mbar_wait(&r.full[stage], phase)) {
-        ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail | stage);
-        *abort_flag = 1u;
-    }
-}
-
-// The producer lane: row k of this CTA into stage k % stages, from the `n` non-null arrays.
-struct Sources {
-    const uint16_t* p[5];
-    uint32_t n;
+struct RingState {
+    uint64_t full[kMaxRing];
+    uint32_t row[kMaxRing];  // the row whose load is under way in, or has landed in, each stage
+    uint32_t abort;
 };
-__device__ __forceinline__ void produce_rows(Ring& r, uint8_t* base, uint32_t stages,
-                                             const Sources& src, uint32_t rows, uint32_t cols,
-                                             uint32_t* err, uint32_t detail) {
-    volatile uint32_t* abort_flag = &r.abort;
-    const uint32_t bytes = cols * 2;
-    uint32_t stage = 0, phase = 0, issued = 0, parity = 0;
-    for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        if (!ptxstd::mbar_wait(&r.empty[stage], phase ^ 1u)) {
-            ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail | stage);
-            *abort_flag = 1u;
-        }
-        if (*abort_flag) break;
-        ptxstd::mbar_arrive_expect_tx(&r.full[stage], bytes * src.n);
-        uint8_t* dst = base + static_cast<size_t>(stage) * bytes * src.n;
-        uint32_t n = 0;
-#pragma unroll
-        for (int k = 0; k < 5; ++k)
-            if (src.p[k])
-                ptxstd::bulk_load(dst + n++ * bytes, src.p[k] + static_cast<size_t>(row) * cols,
-                                  bytes, &r.full[stage]);
-        issued |= 1u << stage;
-        parity = (parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-        }
-    }
-    if (*abort_flag)
-        for (uint32_t i = 0; i < stages; ++i)
-            if (issued & (1u << i)) ptxstd::mbar_wait(&r.full[i], (parity >> i) & 1u);
-}
 
-__device__ __forceinline__ void init_ring(Ring& r, uint32_t stages, uint32_t consumer_warps) {
-    for (uint32_t i = 0; i < stages; ++i) {
-        ptxstd::mbar_init(&r.full[i], 1);
-        ptxstd::mbar_init(&r.empty[i], consumer_warps);
+// Where row k comes from (the non-null arrays, in this order) and where it goes.
+struct Ring {
+    RingState& st;
+    uint8_t* base;
+    const uint16_t* src[5];
+    uint32_t arrays, stages, rows, cols;
+
+    __device__ __forceinline__ uint32_t stage_bytes() const { return arrays * cols * 2; }
+
+    __device__ __forceinline__ void init() {
+        for (uint32_t i = 0; i < stages; ++i) {
+            ptxstd::mbar_init(&st.full[i], 1);
+            st.row[i] = ~0u;
+        }
+        st.abort = 0;
+        ptxstd::fence_mbarrier_init();
     }
-    r.abort = 0;
-    ptxstd::fence_mbarrier_init();
+    // One thread: the CTA's k-th row into `stage`, whose readers are done.
+    __device__ __forceinline__ void load(uint32_t k, uint32_t stage) {
+        const uint64_t row = blockIdx.x + static_cast<uint64_t>(k) * gridDim.x;
+        if (row >= rows) return;
+        const uint32_t bytes = cols * 2;
+        uint8_t* dst = base + static_cast<size_t>(stage) * stage_bytes();
+        ptxstd::mbar_arrive_expect_tx(&st.full[stage], stage_bytes());
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            if (src[i]) {
+                ptxstd::bulk_load(dst, src[i] + row * cols, bytes, &st.full[stage]);
+                dst += bytes;
+            }
+        *reinterpret_cast<volatile uint32_t*>(&st.row[stage]) = k;
+    }
+    // Every thread of a group: waits for row k in `stage`. The row number is waited for first: two
+    // consecutive rows of a stage may belong to different groups, so a group can be two rows
+    // ahead of the stage, where the parity alone would let it pass. Once the number is there, the
+    // row before it has been consumed and the barrier is in row k's phase or past it.
+    // After a timeout (recorded) the kernel runs on without waiting, on whatever the stages hold,
+    // so that every barrier still sees all of its threads; drain() then keeps the block until its
+    // copies have landed.
+    __device__ __forceinline__ void wait(uint32_t k, uint32_t stage, uint32_t parity, uint32_t* err,
+                                         uint32_t detail) {
+        volatile uint32_t* abort_flag = &st.abort;
+        volatile uint32_t* row = &st.row[stage];
+        if (!*abort_flag) {
+            bool ok = *row == k;
+            if (!ok) {
+                const uint64_t t0 = ptxstd::global_timer();
+                while (!(ok = *row == k) && !*abort_flag)
+                    if (ptxstd::global_timer() - t0 > ptxstd::kWaitLimitNs) break;
+            }
+            if (!ok || !ptxstd::mbar_wait(&st.full[stage], parity)) {
+                ptxstd::record_error(err, PTXSTD_ETIMEOUT, detail | stage);
+                *abort_flag = 1u;
+            }
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void drain() {
+        volatile uint32_t* abort_flag = &st.abort;
+        if (!*abort_flag) return;
+        const uint32_t mine = rows > blockIdx.x ? (rows - blockIdx.x - 1) / gridDim.x + 1 : 0;
+        for (uint32_t i = 0; i < stages && i < mine; ++i) {
+            const uint32_t k = *reinterpret_cast<volatile uint32_t*>(&st.row[i]);
+            if (k != ~0u) ptxstd::mbar_wait(&st.full[i], (k / stages) & 1u);
+        }
+    }
+};
+
+// Eight f32 column factors per vector in shared memory, the first four columns in one plane and
+// the last four in another, so that neighbouring lanes read neighbouring 16 bytes.
+__device__ __forceinline__ void store_planes(float4* dst, uint32_t nv, uint32_t i, const Oct& o) {
+    const float2 a = unpack2(o.v[0]), b = unpack2(o.v[1]), c = unpack2(o.v[2]),
+                 d = unpack2(o.v[3]);
+    dst[i] = make_float4(a.x, a.y, b.x, b.y);
+    dst[nv + i] = make_float4(c.x, c.y, d.x, d.y);
+}
+__device__ __forceinline__ Oct load_planes(const float4* src, uint32_t nv, uint32_t i) {
+    const float4 a = src[i], b = src[nv + i];
+    return {{pack2f(a.x, a.y), pack2f(a.z, a.w), pack2f(b.x, b.y), pack2f(b.z, b.w)}};
 }
 
 constexpr uint32_t kGroupThreads = 256, kGroups = 3;
 
 template <int V>
-__global__ void __launch_bounds__(kGroupThreads* kGroups + 32, 1)
+__global__ void __launch_bounds__(kGroupThreads* kGroups, 1)
     norm_ring_kernel(const __grid_constant__ Fwd p, uint32_t stages, uint32_t* err) {
     extern __shared__ uint4 ring_smem[];
-    __shared__ Ring ring;
+    __shared__ RingState state;
     __shared__ float4 red[kGroups][3][2];  // eight warps' partial sums; a buffer per exchange
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t nv = p.cols / 8;
     const size_t k_tiles = mx::tiles_k(p.cols / 32);
     const bool gate_rows = p.gate && p.gate_stride;
-    // shared memory: w | w_post | gate (if one for all rows) | stages of x | y | gate row
+    // shared memory: w (bf16) | with y, c = scale w_post gate in f32 (the gate of all rows; 1 where
+    // there is none) | stages of x | y | gate row
     uint4* const w = ring_smem;
-    uint4* const w_post = w + nv;
-    uint4* const gate = w_post + (p.w_post ? nv : 0);
-    uint4* const stage0 = gate + (p.gate && !gate_rows ? nv : 0);
+    float4* const c = reinterpret_cast<float4*>(w + nv);
+    uint4* const stage0 = w + (p.y ? 3 : 1) * nv;
     const uint32_t arrays = 1 + (p.y ? 1 : 0) + (gate_rows ? 1 : 0);
+    Ring ring = {state,
+                 reinterpret_cast<uint8_t*>(stage0),
+                 {p.x, p.y, gate_rows ? p.gate : nullptr, nullptr, nullptr},
+                 arrays, stages, p.rows, p.cols};
 
     ptxstd::pdl_launch_dependents();
-    if (tid == 0) init_ring(ring, stages, kGroupThreads / 32);
+    if (tid == 0) ring.init();
     ptxstd::pdl_wait();
+    if (tid == 0)
+        for (uint32_t k = 0; k < stages; ++k) ring.load(k, k);
     for (uint32_t i = tid; i < nv; i += blockDim.x) {
         w[i] = __ldg(reinterpret_cast<const uint4*>(p.w) + i);
-        if (p.w_post) w_post[i] = __ldg(reinterpret_cast<const uint4*>(p.w_post) + i);
-        if (p.gate && !gate_rows) gate[i] = __ldg(reinterpret_cast<const uint4*>(p.gate) + i);
+        if (p.y)
+            store_planes(c, nv, i,
+                         branch_factor(p.w_post, gate_rows ? nullptr : p.gate, p.scale, i));
     }
     for (uint32_t row = p.rows + blockIdx.x; row < mx::padded_rows(p.rows); row += gridDim.x)
         pad_row(p, row, tid, blockDim.x, k_tiles);
     __syncthreads();
 
     const uint32_t g = warp / (kGroupThreads / 32);
-    if (g == kGroups) {
-        if (lane == 0) {
-            const Sources s = {{p.x, p.y, gate_rows ? p.gate : nullptr, nullptr, nullptr}, arrays};
-            produce_rows(ring, reinterpret_cast<uint8_t*>(stage0), stages, s, p.rows, p.cols, err,
-                         kDetailFwdProducer);
-        }
-        return;
-    }
     const uint32_t t = tid - g * kGroupThreads, gw = t >> 5;
     const float inv_d = 1.0f / static_cast<float>(p.cols);
     auto group_sum = [&](float v, float4* buf) {
@@ -342,64 +397,76 @@ __global__ void __launch_bounds__(kGroupThreads* kGroups + 32, 1)
         const float4 a = buf[0], b = buf[1];
         return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
     };
-    uint32_t stage = g % stages, phase = (g / stages) & 1u, flip = 0;
-    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows; row += kGroups * gridDim.x) {
-        ring_wait(ring, stage, phase, err, kDetailFwdConsumer);
-        __syncwarp();
+    uint32_t stage = g % stages, parity = (g / stages) & 1u, flip = 0, k = g;
+    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows;
+         row += kGroups * gridDim.x, k += kGroups) {
+        ring.wait(k, stage, parity, err, kDetailFwd);
         const uint4* const xs = stage0 + static_cast<size_t>(stage) * arrays * nv;
-        const uint4 *const ys = xs + nv, *const gs = gate_rows ? xs + 2 * nv : gate;
         const size_t base = static_cast<size_t>(row) * p.cols;
-        uint4 xv[V];
+        uint4 xv[V], yv[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = t + j * kGroupThreads;
+            xv[j] = yv[j] = make_uint4(0, 0, 0, 0);
+            if (i < nv) {
+                xv[j] = xs[i];
+                if (p.y) yv[j] = xs[nv + i];
+            }
+        }
         if (p.y) {
             float ry = 1.0f;
             if (p.w_post) {
                 f32x2 s = 0;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const uint32_t i = t + j * kGroupThreads;
-                    if (i < nv) s = square_sum(ys[i], s);
-                }
+                for (int j = 0; j < V; ++j) s = square_sum(yv[j], s);
                 ry = rsqrtf(group_sum(hsum2(s), red[g][0]) * inv_d + p.eps);
-                if (p.rstd_post && t == 0) p.rstd_post[row] = ry;
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t i = t + j * kGroupThreads;
-                xv[j] = make_uint4(0, 0, 0, 0);
-                if (i < nv) {
-                    xv[j] = join8(xs[i], ys[i], p.w_post ? w_post + i : nullptr,
-                                  p.gate ? gs + i : nullptr, ry, p.scale);
-                    *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
+                if (t == 0) {
+                    if (p.rstd_post) p.rstd_post[row] = ry;
+                    if (!gate_rows) ring.load(k + stages, stage);
                 }
             }
-        } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const uint32_t i = t + j * kGroupThreads;
-                xv[j] = i < nv ? xs[i] : make_uint4(0, 0, 0, 0);
+                if (i >= nv) continue;
+                Oct x = widen(xv[j]), y = widen(yv[j]);
+                const Oct f = load_planes(c, nv, i);
+                const f32x2 r = pack2f(ry, ry);
+                if (gate_rows) {
+                    const Oct g = widen(xs[2 * nv + i]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) y.v[q] = mul2(y.v[q], g.v[q]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x.v[q] = fma2(mul2(y.v[q], r), f.v[q], x.v[q]);
+                xv[j] = narrow(x);
+                *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
             }
         }
-        __syncwarp();
-        if (lane == 0) ptxstd::mbar_arrive(&ring.empty[stage]);
         f32x2 s = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
         const float rx = rsqrtf(group_sum(hsum2(s), red[g][1 + flip]) * inv_d + p.eps);
-        if (p.rstd && t == 0) p.rstd[row] = rx;
+        if (t == 0) {
+            if (p.rstd) p.rstd[row] = rx;
+            if (!p.w_post || gate_rows) ring.load(k + stages, stage);
+        }
+        const ScaleRow sr(p, row, k_tiles);
+        sr.pad(p, t);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = t + j * kGroupThreads;
             const bool on = i < nv;
-            finish8(p, xv[j], on ? w[i] : make_uint4(0, 0, 0, 0), rx, row, base, i, on, lane,
-                    k_tiles);
+            finish8(p, xv[j], on ? w[i] : make_uint4(0, 0, 0, 0), rx, base, i, on, lane, sr);
         }
         flip ^= 1u;
         stage += kGroups;
         while (stage >= stages) {
             stage -= stages;
-            phase ^= 1u;
+            parity ^= 1u;
         }
     }
+    ring.drain();
 }
 
 template <int V, bool WARP_ROW>
@@ -430,7 +497,7 @@ int launch_fwd_ring(const Fwd& p, uint32_t stages, size_t smem, cudaStream_t str
     uint32_t* err = ptxstd::device_error_word();
     if (!err) return PTXSTD_ECUDA;
     const uint32_t sms = static_cast<uint32_t>(ptxstd::sm_count());
-    ptxstd::set_pdl(cfg, attr, p.rows < sms ? p.rows : sms, kGroupThreads * kGroups + 32, stream);
+    ptxstd::set_pdl(cfg, attr, p.rows < sms ? p.rows : sms, kGroupThreads * kGroups, stream);
     cfg.dynamicSmemBytes = smem;
     if (cudaLaunchKernelEx(&cfg, norm_ring_kernel<V>, p, stages, err) != cudaSuccess)
         return PTXSTD_ECUDA;
@@ -455,21 +522,8 @@ struct Factors {
     Oct w, c;
 };
 __device__ __forceinline__ Factors column_factors(const Bwd& p, uint32_t i) {
-    Factors f;
-    f.w = widen(__ldg(reinterpret_cast<const uint4*>(p.w) + i));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f.c.v[k] = pack2f(p.scale, p.scale);
-    if (p.w_post) {
-        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(p.w_post) + i));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f.c.v[k] = mul2(f.c.v[k], o.v[k]);
-    }
-    if (p.gate && !p.gate_stride) {
-        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(p.gate) + i));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f.c.v[k] = mul2(f.c.v[k], o.v[k]);
-    }
-    return f;
+    return {widen(__ldg(reinterpret_cast<const uint4*>(p.w) + i)),
+            branch_factor(p.w_post, p.gate_stride ? nullptr : p.gate, p.scale, i)};
 }
 
 // What a row's sums need of eight columns: sum(a x'), sum(t du), sum(t a), sum(t x') with
@@ -688,81 +742,87 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512)
 // 1024 < columns <= 8192: the ring. GROUPS groups of THREADS threads take the CTA's rows in turn;
 // a thread keeps its V vectors' column sums in registers for all of its group's rows.
 template <int V, uint32_t THREADS, uint32_t GROUPS>
-__global__ void __launch_bounds__(THREADS* GROUPS + 32, 1)
+__global__ void __launch_bounds__(THREADS* GROUPS, 1)
     norm_backward_ring_kernel(const __grid_constant__ Bwd p, uint32_t stages, uint32_t* err) {
     constexpr uint32_t kWarps = THREADS / 32;
     extern __shared__ uint4 ring_smem[];
-    __shared__ Ring ring;
+    __shared__ RingState state;
     __shared__ float4 red[GROUPS][2][kWarps];
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t nv = p.cols / 8;
     // shared memory: column factors w | c in f32, stages of dn | x | du | y | gate row
-    float* const w = reinterpret_cast<float*>(ring_smem);
-    float* const c = w + p.cols;
+    float4* const w = reinterpret_cast<float4*>(ring_smem);
+    float4* const c = w + 2 * nv;
     uint4* const stage0 = ring_smem + 4 * nv;
     const uint32_t arrays = 2 + (p.du ? 1 : 0) + (p.y ? 1 : 0) + (p.gate_stride ? 1 : 0);
+    Ring ring = {state,
+                 reinterpret_cast<uint8_t*>(stage0),
+                 {p.dn, p.x, p.du, p.y, p.gate_stride ? p.gate : nullptr},
+                 arrays, stages, p.rows, p.cols};
 
     ptxstd::pdl_launch_dependents();
-    if (tid == 0) init_ring(ring, stages, kWarps);
+    if (tid == 0) ring.init();
     ptxstd::pdl_wait();
+    if (tid == 0)
+        for (uint32_t k = 0; k < stages; ++k) ring.load(k, k);
     for (uint32_t i = tid; i < nv; i += blockDim.x) {
         const Factors f = column_factors(p, i);
-        store_oct(w + 8 * i, f.w);
-        store_oct(c + 8 * i, f.c);
+        store_planes(w, nv, i, f.w);
+        store_planes(c, nv, i, f.c);
     }
     __syncthreads();
 
     const uint32_t g = warp / kWarps;
-    if (g == GROUPS) {
-        if (lane == 0) {
-            const Sources s = {{p.dn, p.x, p.du, p.y, p.gate_stride ? p.gate : nullptr}, arrays};
-            produce_rows(ring, reinterpret_cast<uint8_t*>(stage0), stages, s, p.rows, p.cols, err,
-                         kDetailBwdProducer);
-        }
-        return;
-    }
     const uint32_t t = tid - g * THREADS, gw = t >> 5;
     const float inv_d = 1.0f / static_cast<float>(p.cols);
     Oct dw[V], S[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[j] = S[j] = kZeroOct;
-    uint32_t stage = g % stages, phase = (g / stages) & 1u, flip = 0;
-    const uint32_t step = GROUPS * gridDim.x;
-    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows; row += step, flip ^= 1u) {
+    uint32_t stage = g % stages, parity = (g / stages) & 1u, flip = 0, k = g;
+    for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows;
+         row += GROUPS * gridDim.x, k += GROUPS, flip ^= 1u) {
         const float rx = p.rstd[row], ry = p.w_post ? p.rstd_post[row] : 1.0f;
-        ring_wait(ring, stage, phase, err, kDetailBwdConsumer);
-        __syncwarp();
+        ring.wait(k, stage, parity, err, kDetailBwd);
         const uint4* const dns = stage0 + static_cast<size_t>(stage) * arrays * nv;
         const uint4* const xs = dns + nv;
         const uint4* const dus = xs + nv;
         const uint4* const ys = dus + (p.du ? nv : 0);
         const uint4* const gs = p.gate_stride ? ys + nv : nullptr;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
+        uint4 dnv[V], duv[V], xv[V], yv[V];
         Sums s;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = t + j * THREADS;
-            if (i < nv)
-                sums8(s, dns[i], p.du ? dus[i] : zero, xs[i], p.y ? ys[i] : zero,
-                      {load_oct(w + 8 * i), load_oct(c + 8 * i)}, p.w_post, gs ? gs + i : nullptr);
+            dnv[j] = duv[j] = xv[j] = yv[j] = make_uint4(0, 0, 0, 0);
+            if (i < nv) {
+                dnv[j] = dns[i];
+                xv[j] = xs[i];
+                if (p.du) duv[j] = dus[i];
+                if (p.y) yv[j] = ys[i];
+                sums8(s, dnv[j], duv[j], xv[j], yv[j], {load_planes(w, nv, i), load_planes(c, nv, i)},
+                      p.w_post, gs ? gs + i : nullptr);
+            }
         }
         const float4 sum = group_sum4<kWarps>(s, red[g][flip], gw, lane, kWarps, g);
+        if (t == 0 && !gs) ring.load(k + stages, stage);
         const RowFactors r = row_factors(sum, rx, ry, inv_d);
         const size_t base = static_cast<size_t>(row) * p.cols;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = t + j * THREADS;
             if (i < nv)
-                grads8(p, r, dns[i], p.du ? dus[i] : zero, xs[i], p.y ? ys[i] : zero,
-                       {load_oct(w + 8 * i), load_oct(c + 8 * i)}, gs ? gs + i : nullptr,
+                grads8(p, r, dnv[j], duv[j], xv[j], yv[j],
+                       {load_planes(w, nv, i), load_planes(c, nv, i)}, gs ? gs + i : nullptr,
                        base + 8 * i, dw[j], S[j]);
         }
-        __syncwarp();
-        if (lane == 0) ptxstd::mbar_arrive(&ring.empty[stage]);
+        if (gs) {  // the gate row was read until here
+            group_sync(g, THREADS);
+            if (t == 0) ring.load(k + stages, stage);
+        }
         stage += GROUPS;
         while (stage >= stages) {
             stage -= stages;
-            phase ^= 1u;
+            parity ^= 1u;
         }
     }
     float* out = p.partial + static_cast<size_t>(blockIdx.x * GROUPS + g) * p.sums * p.cols;
@@ -773,6 +833,7 @@ __global__ void __launch_bounds__(THREADS* GROUPS + 32, 1)
         store_oct(out + 8 * i, dw[j]);
         if (p.sums > 1) store_oct(out + p.cols + 8 * i, S[j]);
     }
+    ring.drain();
 }
 
 // How a backward call runs, by its sizes: the grid and the groups that write partial sums.
@@ -820,7 +881,7 @@ int launch_bwd_ring(const Bwd& p, uint32_t grid, cudaStream_t stream) {
     if (stages < GROUPS) return PTXSTD_EINVAL;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    ptxstd::set_pdl(cfg, attr, grid, THREADS * GROUPS + 32, stream);
+    ptxstd::set_pdl(cfg, attr, grid, THREADS * GROUPS, stream);
     cfg.dynamicSmemBytes = fixed + stages * row;
     if (cudaLaunchKernelEx(&cfg, kernel, p, stages, err) != cudaSuccess) return PTXSTD_ECUDA;
     return ptxstd::launch_status();
@@ -877,13 +938,13 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
     if (nv <= 32) return launch_fwd<1, true>(p, 32, s);
     if (nv <= 64) return launch_fwd<2, true>(p, 32, s);
     if (nv <= 128) return launch_fwd<4, true>(p, 32, s);
-    // Many rows: the ring. 8192 x 8192 with everything on, E4M3 out: 00 us against 99 us for the
+    // Many rows: the ring. 8192 x 8192 with everything on, E4M3 out: 80 us against 99 us for the
     // row-per-block kernel below; with fewer rows than the GPU holds groups the latter starts
     // sooner.
     if (rows >= 4 * ptxstd::sm_count() && nv <= 4 * kGroupThreads) {
         const bool per_row = d_gate && p.gate_stride;
         const size_t vec = static_cast<size_t>(cols) * 2;
-        const size_t fixed = vec * (1 + (d_w_post ? 1 : 0) + (d_gate && !per_row ? 1 : 0));
+        const size_t fixed = vec * (d_y ? 3 : 1);
         const size_t row_bytes = vec * (1 + (d_y ? 1 : 0) + (per_row ? 1 : 0));
         const uint32_t stages = ring_stages(fixed, row_bytes);
         if (stages >= kGroups) {

@@ -357,6 +357,57 @@ def test_norm_forward(cuda, rows, cols, post, gate):
             R.check_mx(*n, ref, CHAIN * ref.abs(), fmt, padded=layout == 1, what="n")
 
 
+@pytest.mark.parametrize("rows,cols", [(592, 1056), (1037, 5152), (1500, 2048), (700, 8192)])
+@pytest.mark.parametrize("post,gate", [(True, "vector"), (True, "row"), (False, "row"),
+                                       (False, "none")])
+def test_norm_forward_many_rows(cuda, rows, cols, post, gate):
+    """Enough rows for several per block; repeated and back to back, so that blocks of consecutive
+    calls share SMs."""
+    import ptxstd
+    _, x, y, w, wp, gt = _norm_inputs(rows, cols, post, gate)
+    eps, s = 1e-6, 0.5
+    args = dict(y=y, w_post=wp, gate=gt, scale=s, eps=eps, elem_type="e4m3")
+    runs = [ptxstd.rmsnorm_residual(x, w, **args) for _ in range(20)]
+    _ok()
+    for r in runs[1:]:
+        for p, q in zip(_flat(runs[0]), _flat(r)):
+            assert torch.equal(p, q)
+    xo, n, (r, rp) = runs[0]
+    ref, mag, _ = R.norm_forward(_d(x), _d(y), _d(wp), _d(gt), s, eps)
+    R.check_bf16(xo, ref, CHAIN * mag, "x'")
+    ref, rx = R.norm_result(xo.double(), _d(w), eps)
+    assert ((r.double() - rx).abs() <= CHAIN * rx).all()
+    R.check_mx(*n, ref, CHAIN * ref.abs(), "e4m3", what="n")
+    plain = ptxstd.rmsnorm_residual(x, w)[1]
+    _ok()
+    ref = R.norm_result(_d(x), _d(w), 1e-6)[0]
+    R.check_bf16(plain, ref, CHAIN * ref.abs(), "plain")
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 1056), (1100, 8192), (2000, 4096)])
+@pytest.mark.parametrize("gate", ["vector", "row"])
+def test_norm_backward_many_rows(cuda, rows, cols, gate):
+    import ptxstd
+    g, xo, y, w, wp, gt = _norm_inputs(rows, cols, True, gate)
+    dn, du = _bf(g, rows, cols, std=0.3), _bf(g, rows, cols, std=0.3)
+    rx = torch.rsqrt(xo.double().square().mean(1) + 1e-6).float()
+    ry = torch.rsqrt(y.double().square().mean(1) + 1e-6).float()
+    runs = [ptxstd.rmsnorm_residual_backward(dn, xo, w, (rx, ry), dx_out=du, y=y, w_post=wp,
+                                             gate=gt, scale=0.5) for _ in range(20)]
+    _ok()
+    for r in runs[1:]:
+        for p, q in zip(runs[0], r):
+            assert torch.equal(p, q)
+    dx, dw, dy, dwp, dg = runs[0]
+    ref = R.norm_backward(_d(dn), _d(du), _d(xo), _d(w), _d(rx), _d(y), _d(wp), _d(ry), _d(gt),
+                          0.5)
+    R.check_bf16(dx, ref["dx"][0], CHAIN * ref["dx"][1], "dx")
+    R.check_bf16(dy, ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
+    terms = CHAIN + (rows / 148 + 200) * 2.0 ** -24
+    for name, got in (("dw", dw), ("dw_post", dwp)):
+        assert ((got.double() - ref[name][0]).abs() <= 4 * terms * ref[name][1]).all(), name
+
+
 def test_norm_without_branch(cuda):
     """No y: x' is x; columns that are not a multiple of 32 in bf16; a zero row stays zero."""
     import ptxstd
