@@ -32,38 +32,29 @@ struct Params {
     uint32_t col_tiles, act, type;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& v, float (&o)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        o[2 * k] = dt::bf16_lo(w[k]);
-        o[2 * k + 1] = dt::bf16_hi(w[k]);
-    }
+using ptxstd::f32x2;
+using ptxstd::mul2;
+using ptxstd::Oct;
+using ptxstd::widen;
+
+// The tile in shared memory, [row][64] f32 as 16 slots of four columns. Slot s of a row sits at
+// s ^ (s / 8): then the eight lanes of a quarter-warp, which hold slots 0, 2, .. 14 (then 1, 3, ..
+// 15) of one row, store into different banks. A column keeps its place in every row, so reading
+// 32 neighbouring columns of a row is free of conflicts too.
+__device__ __forceinline__ uint32_t slot_of(uint32_t s) { return s ^ (s >> 3); }
+
+// Eight values (lane l of a row's eight) to the tile.
+__device__ __forceinline__ void put8(float4* row, uint32_t l, const float (&v)[8]) {
+    row[slot_of(2 * l)] = make_float4(v[0], v[1], v[2], v[3]);
+    row[slot_of(2 * l + 1)] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// Eight values of a row to the tile in shared memory. The halves are swapped for lanes 4..7 of a
-// row so that eight lanes' 16-byte stores fall into different banks.
-__device__ __forceinline__ void put8(float* row, uint32_t l, const float (&v)[8]) {
-    float4* p = reinterpret_cast<float4*>(row + 8 * l);
-    const float4 lo = make_float4(v[0], v[1], v[2], v[3]);
-    const float4 hi = make_float4(v[4], v[5], v[6], v[7]);
-    const uint32_t h = (l >> 2) & 1u;
-    p[h] = h ? hi : lo;
-    p[h ^ 1u] = h ? lo : hi;
-}
-
-// One row block (four lanes) of D at (row, first column col of this lane's eight values).
-__device__ __forceinline__ void row_block(const Params& p, const float (&v)[8], uint32_t row,
-                                          uint32_t col, bool on, bool in_tiles, uint32_t lane) {
-    const mx::Scale sc = mx::scale_of(mx::amax_quad(mx::amax_of(v)), mx::emax_of(p.type));
-    if (on)
-        *reinterpret_cast<uint2*>(p.q + static_cast<size_t>(row) * p.W + col) =
-            mx::pack8(p.type, v, sc.inv);
-    if ((lane & 3u) == 0 && in_tiles) {
-        const uint32_t s = col / 32;
-        p.sf[mx::word_offset(row, s >> 2, mx::tiles_k(p.W / 32)) + (s & 3u)] =
-            on ? static_cast<uint8_t>(sc.code) : 0;
-    }
+// One row block (four lanes) of D: eight codes to q, the block's scale to sf (first lane).
+__device__ __forceinline__ void row_block(uint32_t type, const float (&v)[8], bool on, uint8_t* q,
+                                          bool first, uint8_t* sf) {
+    const mx::Scale sc = mx::scale_of(mx::amax_quad(mx::amax_of(v)), mx::emax_of(type));
+    if (on) *reinterpret_cast<uint2*>(q) = mx::pack8(type, v, sc.inv);
+    if (first) *sf = on ? static_cast<uint8_t>(sc.code) : 0;
 }
 
 template <int MODE>
@@ -71,7 +62,7 @@ __global__ void __launch_bounds__(kThreads)
     act_backward_kernel(const __grid_constant__ Params p) {
     constexpr int kTiles = MODE == kGated ? 2 : 1;
     extern __shared__ float4 smem_raw[];
-    float* const tile = reinterpret_cast<float*>(smem_raw);  // [kTiles][kRows][kCols]
+    float4* const tile = smem_raw;  // [kTiles][kRows][kCols / 4]
     __shared__ float sums[4][kCols];
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t ct = blockIdx.x % p.col_tiles, rt = blockIdx.x / p.col_tiles;
@@ -82,65 +73,68 @@ __global__ void __launch_bounds__(kThreads)
     ptxstd::pdl_wait();
 
     {
+        // pass i: rows r, r + 32, ... of the tile
+        const uint32_t r = warp * 4 + (lane >> 3), row = row0 + r;
+        const bool col_on = col < p.cols;
+        const size_t at = static_cast<size_t>(row) * p.cols + col, step = 32ull * p.cols;
         uint4 gv[kPasses], dv[kPasses], uv[kPasses];
 #pragma unroll
         for (uint32_t i = 0; i < kPasses; ++i) {
-            const uint32_t row = row0 + i * 32 + warp * 4 + (lane >> 3);
             gv[i] = dv[i] = uv[i] = make_uint4(0, 0, 0, 0);
-            if (row < p.rows && col < p.cols) {
-                const size_t at = static_cast<size_t>(row) * p.cols + col;
-                gv[i] = *reinterpret_cast<const uint4*>(p.gate + at);
-                if (MODE != kTranspose) dv[i] = *reinterpret_cast<const uint4*>(p.dh + at);
-                if (MODE == kGated) uv[i] = *reinterpret_cast<const uint4*>(p.up + at);
+            if (row + 32 * i < p.rows && col_on) {
+                gv[i] = *reinterpret_cast<const uint4*>(p.gate + at + i * step);
+                if (MODE != kTranspose)
+                    dv[i] = *reinterpret_cast<const uint4*>(p.dh + at + i * step);
+                if (MODE == kGated) uv[i] = *reinterpret_cast<const uint4*>(p.up + at + i * step);
             }
         }
+        float4* const dst = tile + r * (kCols / 4);
+        if constexpr (MODE == kTranspose) {
 #pragma unroll
-        for (uint32_t i = 0; i < kPasses; ++i) {
-            const uint32_t r = i * 32 + warp * 4 + (lane >> 3), row = row0 + r;
-            float g[8], d[8];
-            unpack8(gv[i], g);
-            if constexpr (MODE == kTranspose) {
-                put8(tile + r * kCols, l, g);
-            } else {
-                const bool on = row < p.rows && col < p.cols, in_tiles = col < p.cols;
-                float a[8], b[8];
-                unpack8(dv[i], d);
-                switch (p.act) {
-#define PTXSTD_CASE(K)                                                              \
-    case K:                                                                         \
-        _Pragma("unroll") for (int k = 0; k < 8; ++k) mx::act_grad(K, g[k], a[k], b[k]); \
-        break;
-                    PTXSTD_CASE(PTXSTD_ACT_RELU)
-                    PTXSTD_CASE(PTXSTD_ACT_SILU)
-                    PTXSTD_CASE(PTXSTD_ACT_GELU)
-                    PTXSTD_CASE(PTXSTD_ACT_GELU_TANH)
-#undef PTXSTD_CASE
-                default:
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        a[k] = g[k];
-                        b[k] = 1.0f;
-                    }
-                }
-                if constexpr (MODE == kGated) {
-                    float u[8];
-                    unpack8(uv[i], u);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        b[k] *= d[k] * u[k];  // dgate
-                        a[k] *= d[k];         // dup
-                    }
-                    put8(tile + r * kCols, l, b);
-                    put8(tile + (kRows + r) * kCols, l, a);
-                    row_block(p, b, row, col, on, in_tiles, lane);
-                    row_block(p, a, row, p.cols + col, on, in_tiles, lane);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) b[k] *= d[k];
-                    put8(tile + r * kCols, l, b);
-                    row_block(p, b, row, col, on, in_tiles, lane);
-                }
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                float v[8];
+                ptxstd::flatten(widen(gv[i]), v);
+                put8(dst + i * 32 * (kCols / 4), l, v);
             }
+        } else {
+            const size_t k_tiles = mx::tiles_k(p.W / 32);
+            uint8_t* const q = p.q + static_cast<size_t>(row) * p.W + col;
+            // scales of rows r + 32 i of one 128-row tile are four bytes apart
+            const uint32_t s0 = col / 32, s1 = (p.cols + col) / 32;
+            const bool first = (lane & 3u) == 0 && col_on;
+            uint8_t* const sf = p.sf + mx::word_offset(row, 0, k_tiles);
+            uint8_t* const sf0 = sf + (s0 >> 2) * 512 + (s0 & 3u);
+            uint8_t* const sf1 = sf + (s1 >> 2) * 512 + (s1 & 3u);
+            mx::with_act(p.act, [&](auto kind) {
+#pragma unroll
+                for (uint32_t i = 0; i < kPasses; ++i) {
+                    const bool on = row + 32 * i < p.rows && col_on;
+                    const Oct g = widen(gv[i]), d = widen(dv[i]);
+                    Oct a, b;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        mx::act_grad2<decltype(kind)::value>(g.v[k], a.v[k], b.v[k]);
+                        b.v[k] = mul2(b.v[k], d.v[k]);
+                    }
+                    if constexpr (MODE == kGated) {
+                        const Oct u = widen(uv[i]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            b.v[k] = mul2(b.v[k], u.v[k]);  // dgate
+                            a.v[k] = mul2(a.v[k], d.v[k]);  // dup
+                        }
+                    }
+                    float v[8];
+                    ptxstd::flatten(b, v);
+                    put8(dst + i * 32 * (kCols / 4), l, v);
+                    row_block(p.type, v, on, q + i * 32ull * p.W, first, sf0 + 4 * i);
+                    if constexpr (MODE == kGated) {
+                        ptxstd::flatten(a, v);
+                        put8(dst + (kRows + i * 32) * (kCols / 4), l, v);
+                        row_block(p.type, v, on, q + i * 32ull * p.W + p.cols, first, sf1 + 4 * i);
+                    }
+                }
+            });
         }
     }
     __syncthreads();
@@ -150,16 +144,13 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t t0 = row0 + 32 * b;
     const size_t kt = mx::tiles_k(p.R / 32);
     const uint32_t emax = mx::emax_of(p.type);
+    const float* const column = reinterpret_cast<const float*>(tile) + 4 * slot_of(f >> 2) + (f & 3u);
 #pragma unroll
     for (int h = 0; h < kTiles; ++h) {
-        const float* src = tile + (h * kRows + 32 * b) * kCols + f;
+        const float* src = column + (h * kRows + 32 * b) * kCols;
         float v[32];
-        float sum = 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-            v[i] = src[i * kCols];
-            sum += v[i];
-        }
+        for (uint32_t i = 0; i < 32; ++i) v[i] = src[i * kCols];
         const mx::Scale sc = mx::scale_of(mx::amax_of(v), emax);
         const uint32_t feature = h * p.cols + col0 + f;
         if (col0 + f < p.cols) {
@@ -176,7 +167,11 @@ __global__ void __launch_bounds__(kThreads)
                 t0 < p.R ? static_cast<uint8_t>(sc.code) : 0;
         }
         if (MODE != kTranspose && p.partial) {
-            sums[b][f] = sum;
+            f32x2 sum = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 32; i += 2)
+                sum = ptxstd::add2(sum, ptxstd::pack2f(v[i], v[i + 1]));
+            sums[b][f] = ptxstd::hsum2(sum);
             __syncthreads();
             if (b == 0 && col0 + f < p.cols)
                 p.partial[static_cast<size_t>(rt) * p.W + feature] =

@@ -213,19 +213,16 @@ __device__ __forceinline__ void add_bias32(uint32_t (&r)[L], const uint16_t* bia
 
 template <uint32_t FIRST, uint32_t L>
 __device__ __forceinline__ void act32(uint32_t (&r)[L], uint32_t kind) {
-    switch (kind) {  // one loop per kind: the choice is made once per 32 elements
-#define PTXSTD_CASE(K)                                                            \
-    case K:                                                                       \
-        _Pragma("unroll") for (uint32_t i = 0; i < 32; ++i)                       \
-            r[FIRST + i] = __float_as_uint(mx::act(K, f(r[FIRST + i])));          \
-        break;
-        PTXSTD_CASE(PTXSTD_ACT_RELU)
-        PTXSTD_CASE(PTXSTD_ACT_SILU)
-        PTXSTD_CASE(PTXSTD_ACT_GELU)
-        PTXSTD_CASE(PTXSTD_ACT_GELU_TANH)
-#undef PTXSTD_CASE
-    default: break;
-    }
+    if (kind == PTXSTD_ACT_NONE) return;
+    mx::with_act(kind, [&](auto k) {
+#pragma unroll
+        for (uint32_t i = FIRST; i < FIRST + 32; i += 2) {
+            const float2 v =
+                ptxstd::unpack2(mx::act2<decltype(k)::value>(ptxstd::pack2f(f(r[i]), f(r[i + 1]))));
+            r[i] = __float_as_uint(v.x);
+            r[i + 1] = __float_as_uint(v.y);
+        }
+    });
 }
 
 // The linear epilogue of 32 accumulator columns r[FIRST..] at column `col` of the result.
@@ -557,6 +554,19 @@ struct Bars {
     uint32_t abort;
 };
 
+__device__ __forceinline__ void act8(float (&v)[8], uint32_t kind) {
+    if (kind == PTXSTD_ACT_NONE) return;
+    mx::with_act(kind, [&](auto k) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i += 2) {
+            const float2 y =
+                ptxstd::unpack2(mx::act2<decltype(k)::value>(ptxstd::pack2f(v[i], v[i + 1])));
+            v[i] = y.x;
+            v[i + 1] = y.y;
+        }
+    });
+}
+
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads)
     narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape p,
@@ -788,19 +798,18 @@ __global__ void __launch_bounds__(kThreads)
                     store_bf16(e.pre, v[0]);
                     store_bf16(e.up, v[1]);
                 }
+                act8(v[0], e.act);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) y[i] = mx::act(e.act, v[0][i]) * v[G - 1][i];
+                for (uint32_t i = 0; i < 8; ++i) y[i] = v[0][i] * v[G - 1][i];
             } else {
                 const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) v[0][i] += bias[i];
                 if (on && e.pre) store_bf16(e.pre, v[0]);
+                act8(v[0], e.act);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    y[i] = mx::act(e.act, v[0][i]);
-                    if (e.residual)
-                        y[i] += (i & 1) ? dt::bf16_hi(rw[i >> 1]) : dt::bf16_lo(rw[i >> 1]);
-                }
+                for (uint32_t i = 0; i < 8; ++i)
+                    y[i] = v[0][i] + ((i & 1) ? dt::bf16_hi(rw[i >> 1]) : dt::bf16_lo(rw[i >> 1]));
             }
             if (on && e.c) store_bf16(e.c, y);
             if (e.q) {

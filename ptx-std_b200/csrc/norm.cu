@@ -137,12 +137,7 @@ __device__ __forceinline__ void finish8(const Fwd& p, const uint4& xv, const uin
     if (p.n && on) *reinterpret_cast<uint4*>(p.n + base + 8 * i) = narrow(n);
     if (!p.q) return;
     float a[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack2(n.v[k]);
-        a[2 * k] = f.x;
-        a[2 * k + 1] = f.y;
-    }
+    ptxstd::flatten(n, a);
     const mx::Scale sc = mx::scale_of(mx::amax_quad(mx::amax_of(a)), mx::emax_of(p.q_type));
     if (on) {
         *reinterpret_cast<uint2*>(p.q + base + 8 * i) = mx::pack8(p.q_type, a, sc.inv);
