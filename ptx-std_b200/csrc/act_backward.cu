@@ -4,7 +4,7 @@
 // D = dh up f'(gate) | dh f(gate)   (gated), or dh f'(gate)
 // is needed twice as an MX operand: with blocks of 32 along its rows (dX = D Wt^T sums over the
 // features) and along its columns (dW = D^T X sums over the rows of D). Both come from one pass
-// over dh, gate and up, which HBM bounds: a CTA takes 128 rows x 64 columns, computes D in f32
+// over dh, gate and up, which HBM bounds: a CTA takes 64 rows x 64 columns, computes D in f32
 // once, quantises and stores the row blocks from registers, leaves D in shared memory and reads it
 // back by columns for the transposed operand. Loads are 128-byte row segments, all of a tile
 // issued before the first use; 8 lanes hold a row segment, so a row block of 32 is four lanes. In
@@ -20,8 +20,9 @@ namespace {
 namespace dt = ptxstd::data_types;
 namespace mx = ptxstd::mx;
 
-constexpr uint32_t kRows = 128, kCols = 64, kThreads = 256;
-constexpr uint32_t kPasses = kRows / 32;  // 8 warps x 4 rows a pass
+constexpr uint32_t kRows = 64, kCols = 64, kThreads = 128;
+constexpr uint32_t kPassRows = kThreads / 8;  // eight lanes to a row's 64 columns
+constexpr uint32_t kPasses = kRows / kPassRows;
 enum Mode { kTranspose = 0, kPlain = 1, kGated = 2 };
 
 struct Params {
@@ -57,13 +58,16 @@ __device__ __forceinline__ void row_block(uint32_t type, const float (&v)[8], bo
     if (first) *sf = on ? static_cast<uint8_t>(sc.code) : 0;
 }
 
+// Blocks per SM asked of the compiler: enough registers that all of a tile's loads are in flight at
+// once. Gated, SiLU, 4096 x 10240: 92 us with 5 (92 registers), 119 us without a bound (80
+// registers, loads in turn with their use), 101 us with tiles of 128 rows and 256 threads.
 template <int MODE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
     act_backward_kernel(const __grid_constant__ Params p) {
     constexpr int kTiles = MODE == kGated ? 2 : 1;
     extern __shared__ float4 smem_raw[];
     float4* const tile = smem_raw;  // [kTiles][kRows][kCols / 4]
-    __shared__ float sums[4][kCols];
+    __shared__ float sums[kRows / 32][kCols];
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t ct = blockIdx.x % p.col_tiles, rt = blockIdx.x / p.col_tiles;
     const uint32_t row0 = rt * kRows, col0 = ct * kCols;
@@ -73,15 +77,15 @@ __global__ void __launch_bounds__(kThreads)
     ptxstd::pdl_wait();
 
     {
-        // pass i: rows r, r + 32, ... of the tile
+        // pass i: rows r, r + kPassRows, ... of the tile
         const uint32_t r = warp * 4 + (lane >> 3), row = row0 + r;
         const bool col_on = col < p.cols;
-        const size_t at = static_cast<size_t>(row) * p.cols + col, step = 32ull * p.cols;
+        const size_t at = static_cast<size_t>(row) * p.cols + col, step = static_cast<size_t>(kPassRows) * p.cols;
         uint4 gv[kPasses], dv[kPasses], uv[kPasses];
 #pragma unroll
         for (uint32_t i = 0; i < kPasses; ++i) {
             gv[i] = dv[i] = uv[i] = make_uint4(0, 0, 0, 0);
-            if (row + 32 * i < p.rows && col_on) {
+            if (row + kPassRows * i < p.rows && col_on) {
                 gv[i] = *reinterpret_cast<const uint4*>(p.gate + at + i * step);
                 if (MODE != kTranspose)
                     dv[i] = *reinterpret_cast<const uint4*>(p.dh + at + i * step);
@@ -94,21 +98,23 @@ __global__ void __launch_bounds__(kThreads)
             for (uint32_t i = 0; i < kPasses; ++i) {
                 float v[8];
                 ptxstd::flatten(widen(gv[i]), v);
-                put8(dst + i * 32 * (kCols / 4), l, v);
+                put8(dst + i * kPassRows * (kCols / 4), l, v);
             }
         } else {
             const size_t k_tiles = mx::tiles_k(p.W / 32);
             uint8_t* const q = p.q + static_cast<size_t>(row) * p.W + col;
-            // scales of rows r + 32 i of one 128-row tile are four bytes apart
             const uint32_t s0 = col / 32, s1 = (p.cols + col) / 32;
             const bool first = (lane & 3u) == 0 && col_on;
-            uint8_t* const sf = p.sf + mx::word_offset(row, 0, k_tiles);
+            // the tile's rows lie in one 128-row scale tile
+            uint8_t* const sf = p.sf + (row0 >> 7) * k_tiles * 512;
             uint8_t* const sf0 = sf + (s0 >> 2) * 512 + (s0 & 3u);
             uint8_t* const sf1 = sf + (s1 >> 2) * 512 + (s1 & 3u);
+            const uint32_t rr = row & 127u;
             mx::with_act(p.act, [&](auto kind) {
 #pragma unroll
                 for (uint32_t i = 0; i < kPasses; ++i) {
-                    const bool on = row + 32 * i < p.rows && col_on;
+                    const uint32_t ri = rr + kPassRows * i, at_sf = (ri & 31u) * 16 + (ri >> 5) * 4;
+                    const bool on = row + kPassRows * i < p.rows && col_on;
                     const Oct g = widen(gv[i]), d = widen(dv[i]);
                     Oct a, b;
 #pragma unroll
@@ -126,12 +132,14 @@ __global__ void __launch_bounds__(kThreads)
                     }
                     float v[8];
                     ptxstd::flatten(b, v);
-                    put8(dst + i * 32 * (kCols / 4), l, v);
-                    row_block(p.type, v, on, q + i * 32ull * p.W, first, sf0 + 4 * i);
+                    put8(dst + i * kPassRows * (kCols / 4), l, v);
+                    row_block(p.type, v, on, q + i * static_cast<size_t>(kPassRows) * p.W, first,
+                              sf0 + at_sf);
                     if constexpr (MODE == kGated) {
                         ptxstd::flatten(a, v);
-                        put8(dst + (kRows + i * 32) * (kCols / 4), l, v);
-                        row_block(p.type, v, on, q + i * 32ull * p.W + p.cols, first, sf1 + 4 * i);
+                        put8(dst + (kRows + i * kPassRows) * (kCols / 4), l, v);
+                        row_block(p.type, v, on, q + i * static_cast<size_t>(kPassRows) * p.W + p.cols,
+                                  first, sf1 + at_sf);
                     }
                 }
             });
@@ -163,7 +171,7 @@ __global__ void __launch_bounds__(kThreads)
                     dst[c] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                 }
             }
-            p.sft[mx::word_offset(feature, rt, kt) + b] =
+            p.sft[mx::word_offset(feature, t0 >> 7, kt) + ((t0 >> 5) & 3u)] =
                 t0 < p.R ? static_cast<uint8_t>(sc.code) : 0;
         }
         if (MODE != kTranspose && p.partial) {
@@ -174,8 +182,7 @@ __global__ void __launch_bounds__(kThreads)
             sums[b][f] = ptxstd::hsum2(sum);
             __syncthreads();
             if (b == 0 && col0 + f < p.cols)
-                p.partial[static_cast<size_t>(rt) * p.W + feature] =
-                    (sums[0][f] + sums[1][f]) + (sums[2][f] + sums[3][f]);
+                p.partial[static_cast<size_t>(rt) * p.W + feature] = sums[0][f] + sums[1][f];
             if (h + 1 < kTiles) __syncthreads();
         }
     }
@@ -183,8 +190,9 @@ __global__ void __launch_bounds__(kThreads)
     // padding of the scale tiles: the CTAs of the first column tile write it
     if (ct == 0) {
         const uint32_t w_rows = static_cast<uint32_t>(mx::padded_rows(p.W));
-        for (uint32_t r = p.W + tid; r < w_rows; r += kThreads)
-            *reinterpret_cast<uint32_t*>(p.sft + mx::word_offset(r, rt, kt)) = 0;
+        if (row0 % 128 == 0)
+            for (uint32_t r = p.W + tid; r < w_rows; r += kThreads)
+                *reinterpret_cast<uint32_t*>(p.sft + mx::word_offset(r, row0 >> 7, kt)) = 0;
         if (MODE != kTranspose) {
             const uint32_t blocks = p.W / 32;
             const size_t k_tiles = mx::tiles_k(blocks);
@@ -199,8 +207,7 @@ template <int MODE>
 int launch(Params& p, cudaStream_t stream) {
     p.R = (p.rows + 31) / 32 * 32;
     p.col_tiles = (p.cols + kCols - 1) / kCols;
-    const uint64_t tiles =
-        static_cast<uint64_t>(p.col_tiles) * ((static_cast<uint64_t>(p.rows) + kRows - 1) / kRows);
+    const uint64_t tiles = p.col_tiles * static_cast<uint64_t>(mx::padded_rows(p.rows) / kRows);
     if (tiles >= (1ull << 31)) return PTXSTD_EINVAL;
     constexpr int kSmem = (MODE == kGated ? 2 : 1) * kRows * kCols * 4;
     const int st = ptxstd::set_max_dynamic_smem(
@@ -225,7 +232,7 @@ bool sizes_ok(int64_t rows, int64_t cols) {
 extern "C" size_t ptxstd_act_backward_mx_workspace_bytes(int64_t rows, int64_t cols, int gated,
                                                          int with_dbias) {
     if (!with_dbias || !sizes_ok(rows, cols)) return 0;
-    return static_cast<size_t>((rows + kRows - 1) / kRows) * static_cast<size_t>(cols) *
+    return mx::padded_rows(static_cast<size_t>(rows)) / kRows * static_cast<size_t>(cols) *
            (gated ? 2 : 1) * 4;
 }
 
@@ -264,7 +271,7 @@ extern "C" int ptxstd_act_backward_mx(int act, const uint16_t* d_dh, const uint1
     if (st || !d_dbias) return st;
     ptxstd::Reduce r = {};
     r.partial = p.partial;
-    r.P = (p.rows + kRows - 1) / kRows;
+    r.P = static_cast<uint32_t>(mx::padded_rows(p.rows) / kRows);
     r.sums = 1;
     r.cols = p.W;
     r.o0 = d_dbias;

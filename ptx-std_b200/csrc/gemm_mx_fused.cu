@@ -567,8 +567,103 @@ __device__ __forceinline__ void act8(float (&v)[8], uint32_t kind) {
     });
 }
 
+// The sum of a row chunk's partials over the cluster's CTAs, in rank order: eight columns at byte
+// `at` of every CTA's partial buffer. All loads are issued before the first add.
+template <uint32_t S>
+__device__ __forceinline__ void sum_peers(const uint32_t (&peer)[S], uint32_t at, float (&v)[8]) {
+    float4 lo[S], hi[S];
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) {
+        lo[s] = ld_cluster_v4(peer[s] + at);
+        hi[s] = ld_cluster_v4(peer[s] + at + 16);
+    }
+    v[0] = lo[0].x, v[1] = lo[0].y, v[2] = lo[0].z, v[3] = lo[0].w;
+    v[4] = hi[0].x, v[5] = hi[0].y, v[6] = hi[0].z, v[7] = hi[0].w;
+#pragma unroll
+    for (uint32_t s = 1; s < S; ++s) {
+        v[0] += lo[s].x, v[1] += lo[s].y, v[2] += lo[s].z, v[3] += lo[s].w;
+        v[4] += hi[s].x, v[5] += hi[s].y, v[6] += hi[s].z, v[7] += hi[s].w;
+    }
+}
+
+// The epilogue proper: 16 threads per token, eight result columns (weight rows) each; CTA `rank`
+// takes the tokens rank, rank + S, ... of the tile. With an MX result the padding rows of the last
+// scale tile get zero codes.
+template <bool GATED, uint32_t S>
+__device__ __forceinline__ void narrow_epilogue(const Shape& p, const Epi& e, uint32_t part_addr,
+                                                uint32_t rank, uint32_t block, uint32_t tok0,
+                                                const float (&bias)[8]) {
+    constexpr uint32_t G = GATED ? 2 : 1;
+    const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id();
+    const uint32_t c8 = (tid & 15u) * 8, col = block * 128 + c8, T = p.tokens;
+    const uint32_t live = min(T, p.M - tok0);
+    const bool last_y = blockIdx.y + 1 == gridDim.y;
+    const uint32_t upto =
+        e.q ? (last_y ? static_cast<uint32_t>(mx::padded_rows(p.M)) - tok0 : T) : live;
+    const bool col_ok = col < p.N;
+    const size_t q_tiles_k = mx::tiles_k(p.N / 32);
+    uint32_t peer[S];
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) peer[s] = S > 1 ? ptxstd::mapa_shared(part_addr, s) : part_addr;
+    // uniform trip count per warp (the shuffles below take all lanes)
+    for (uint32_t t0 = rank; t0 < upto; t0 += 16 * S) {
+        const uint32_t t = t0 + (tid >> 4) * S;
+        const bool on = t < live && col_ok;
+        const size_t at = static_cast<size_t>(tok0 + t) * p.N + col;
+        float v[G][8];
+        uint4 res = make_uint4(0, 0, 0, 0);
+        if (on) {
+            if (!GATED && e.residual) res = *reinterpret_cast<const uint4*>(e.residual + at);
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g)
+                sum_peers<S>(peer, ((g * T + t) * 128 + c8) * 4, v[g]);
+        } else {
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g)
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) v[g][i] = 0.0f;
+        }
+        auto store_bf16 = [&](uint16_t* dst, const float* x) {
+            uint4 o;
+            o.x = dt::bf16x2_from_f32(x[0], x[1]);
+            o.y = dt::bf16x2_from_f32(x[2], x[3]);
+            o.z = dt::bf16x2_from_f32(x[4], x[5]);
+            o.w = dt::bf16x2_from_f32(x[6], x[7]);
+            *reinterpret_cast<uint4*>(dst + at) = o;
+        };
+        float y[8];
+        if constexpr (GATED) {
+            if (on && e.pre) {
+                store_bf16(e.pre, v[0]);
+                store_bf16(e.up, v[1]);
+            }
+            act8(v[0], e.act);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) y[i] = v[0][i] * v[G - 1][i];
+        } else {
+            const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) v[0][i] += bias[i];
+            if (on && e.pre) store_bf16(e.pre, v[0]);
+            act8(v[0], e.act);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                y[i] = v[0][i] + ((i & 1) ? dt::bf16_hi(rw[i >> 1]) : dt::bf16_lo(rw[i >> 1]));
+        }
+        if (on && e.c) store_bf16(e.c, y);
+        if (e.q) {
+            const mx::Scale sc =
+                mx::scale_of(mx::amax_quad(mx::amax_of(y)), mx::emax_of(e.q_type));
+            if (on) *reinterpret_cast<uint2*>(e.q + at) = mx::pack8(e.q_type, y, sc.inv);
+            if ((lane & 3u) == 0 && t < upto)
+                e.sfq[mx::word_offset(tok0 + t, block, q_tiles_k) + ((tid & 15u) >> 2)] =
+                    on ? static_cast<uint8_t>(sc.code) : 0;
+        }
+    }
+}
+
 template <bool GATED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     narrow_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape p,
                   uint32_t wtype, uint32_t xtype, const __grid_constant__ Epi e, uint32_t* err) {
     constexpr uint32_t G = GATED ? 2 : 1;
@@ -614,6 +709,17 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t tmem = b.tmem_base;
     ptxstd::pdl_launch_dependents();  // after the TMEM allocation, as in the wide kernel
     ptxstd::pdl_wait();
+    float bias[8] = {};
+    if (!GATED && e.bias && block * 128 + (tid & 15u) * 8 < p.N) {
+        const uint4 w =
+            __ldg(reinterpret_cast<const uint4*>(e.bias + block * 128 + (tid & 15u) * 8));
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            bias[2 * k] = dt::bf16_lo(v[k]);
+            bias[2 * k + 1] = dt::bf16_hi(v[k]);
+        }
+    }
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
@@ -714,14 +820,22 @@ __global__ void __launch_bounds__(kThreads)
     ok = __syncthreads_and(ok && !*abort_flag);
     t5::fence_after_thread_sync();
     if (ok) {
-        const uint32_t q = warp & 3u;
-        for (uint32_t c = (warp >> 2) * 8; c < G * T; c += 16) {
-            uint32_t r[8];
-            t5::ld_32x32b_x8(tmem + ((32 * q) << 16) + c, r);
+        // warp w: lanes 32 (w % 4) .. + 31 of every other 16 columns, two loads in flight
+        const uint32_t q = warp & 3u, cols = G * T;
+        float* const dst = part + 32 * q + lane;
+        for (uint32_t c = (warp >> 2) * 16; c < cols; c += 64) {
+            const uint32_t ta = tmem + ((32 * q) << 16) + c;
+            const bool two = c + 32 < cols;
+            uint32_t r[16], r2[16];
+            t5::ld_32x32b_x16(ta, r);
+            if (two) t5::ld_32x32b_x16(ta + 32, r2);
             t5::wait_ld();
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                part[(c + i) * 128 + 32 * q + lane] = k_hi > k_lo ? f(r[i]) : 0.0f;
+            for (uint32_t i = 0; i < 16; ++i) dst[(c + i) * 128] = f(r[i]);
+            if (two) {
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) dst[(c + 32 + i) * 128] = f(r2[i]);
+            }
         }
     }
     t5::fence_before_thread_sync();
@@ -731,95 +845,12 @@ __global__ void __launch_bounds__(kThreads)
     if (warp == 1) t5::tmem_dealloc(tmem, p.tmem_cols);
 
     if (ok) {
-        // 16 threads per token, 8 result columns (weight rows) each; CTA `rank` takes the tokens
-        // rank, rank + split, ... of the tile. With an MX result the padding rows of the last
-        // scale tile get zero codes.
-        const uint32_t c8 = (tid & 15u) * 8, col = block * 128 + c8;
-        const uint32_t live = min(T, p.M - tok0);
-        const bool last_y = blockIdx.y + 1 == gridDim.y;
-        const uint32_t upto =
-            e.q ? (last_y ? static_cast<uint32_t>(mx::padded_rows(p.M)) - tok0 : T) : live;
-        const bool col_ok = col < p.N;
-        const size_t q_tiles_k = mx::tiles_k(p.N / 32);
-        const uint32_t part_addr = ptxstd::smem_u32(part);
-        float bias[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) bias[i] = 0.0f;
-        if (!GATED && e.bias && col_ok) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(e.bias + col));
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                bias[2 * k] = dt::bf16_lo(v[k]);
-                bias[2 * k + 1] = dt::bf16_hi(v[k]);
-            }
-        }
-        // uniform trip count per warp (the shuffles below take all lanes)
-        for (uint32_t t0 = rank; t0 < upto; t0 += 16 * p.split) {
-            const uint32_t t = t0 + (tid >> 4) * p.split;
-            const bool on = t < live && col_ok;
-            const size_t at = static_cast<size_t>(tok0 + t) * p.N + col;
-            float v[G][8];
-#pragma unroll
-            for (uint32_t g = 0; g < G; ++g)
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) v[g][i] = 0.0f;
-            uint4 res = make_uint4(0, 0, 0, 0);
-            if (on) {
-                if (!GATED && e.residual) res = *reinterpret_cast<const uint4*>(e.residual + at);
-                for (uint32_t s = 0; s < p.split; ++s) {
-#pragma unroll
-                    for (uint32_t g = 0; g < G; ++g) {
-                        uint32_t a = part_addr + ((g * T + t) * 128 + c8) * 4;
-                        if (p.split > 1) a = ptxstd::mapa_shared(a, s);
-                        const float4 x = ld_cluster_v4(a), y = ld_cluster_v4(a + 16);
-                        v[g][0] += x.x;
-                        v[g][1] += x.y;
-                        v[g][2] += x.z;
-                        v[g][3] += x.w;
-                        v[g][4] += y.x;
-                        v[g][5] += y.y;
-                        v[g][6] += y.z;
-                        v[g][7] += y.w;
-                    }
-                }
-            }
-            auto store_bf16 = [&](uint16_t* dst, const float* x) {
-                uint4 o;
-                o.x = dt::bf16x2_from_f32(x[0], x[1]);
-                o.y = dt::bf16x2_from_f32(x[2], x[3]);
-                o.z = dt::bf16x2_from_f32(x[4], x[5]);
-                o.w = dt::bf16x2_from_f32(x[6], x[7]);
-                *reinterpret_cast<uint4*>(dst + at) = o;
-            };
-            float y[8];
-            if constexpr (GATED) {
-                if (on && e.pre) {
-                    store_bf16(e.pre, v[0]);
-                    store_bf16(e.up, v[1]);
-                }
-                act8(v[0], e.act);
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) y[i] = v[0][i] * v[G - 1][i];
-            } else {
-                const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) v[0][i] += bias[i];
-                if (on && e.pre) store_bf16(e.pre, v[0]);
-                act8(v[0], e.act);
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    y[i] = v[0][i] + ((i & 1) ? dt::bf16_hi(rw[i >> 1]) : dt::bf16_lo(rw[i >> 1]));
-            }
-            if (on && e.c) store_bf16(e.c, y);
-            if (e.q) {
-                const mx::Scale sc =
-                    mx::scale_of(mx::amax_quad(mx::amax_of(y)), mx::emax_of(e.q_type));
-                if (on) *reinterpret_cast<uint2*>(e.q + at) = mx::pack8(e.q_type, y, sc.inv);
-                if ((lane & 3u) == 0 && t < upto)
-                    e.sfq[mx::word_offset(tok0 + t, block, q_tiles_k) + ((tid & 15u) >> 2)] =
-                        on ? static_cast<uint8_t>(sc.code) : 0;
-            }
+        const uint32_t pa = ptxstd::smem_u32(part);
+        switch (p.split) {
+        case 1: narrow_epilogue<GATED, 1>(p, e, pa, rank, block, tok0, bias); break;
+        case 2: narrow_epilogue<GATED, 2>(p, e, pa, rank, block, tok0, bias); break;
+        case 4: narrow_epilogue<GATED, 4>(p, e, pa, rank, block, tok0, bias); break;
+        default: narrow_epilogue<GATED, 8>(p, e, pa, rank, block, tok0, bias); break;
         }
     }
     // no CTA of the cluster leaves while another may still read its partial sums

@@ -51,8 +51,8 @@ def test_c_refusals(ptxstd_lib):
                                         None)
 
     for kw in (dict(rows=0), dict(cols=40), dict(t=3), dict(act=7), dict(dh=0), dict(gate=p + 2),
-               dict(q=0), dict(sft=0), dict(db=p), dict(db=p, ws=p, nb=255),
-               dict(db=p, ws=p, nb=511, up=p), dict(up=p + 8)):
+               dict(q=0), dict(sft=0), dict(db=p), dict(db=p, ws=p, nb=511),
+               dict(db=p, ws=p, nb=1023, up=p), dict(up=p + 8)):
         assert back(**kw) == E, kw
     assert L.ptxstd_quantize_mx_t(p, 8, 12, 0, p, p, None) == E
     assert L.ptxstd_quantize_mx_t(p, 0, 16, 0, p, p, None) == E
@@ -86,7 +86,7 @@ def test_c_refusals(ptxstd_lib):
 def test_workspace_sizes(ptxstd_lib):
     L = ptxstd_lib.lib()
     f = L.ptxstd_act_backward_mx_workspace_bytes
-    assert f(1, 64, 0, 1) == 256 and f(129, 64, 1, 1) == 1024
+    assert f(1, 64, 0, 1) == 512 and f(129, 64, 1, 1) == 2048
     assert f(129, 64, 1, 0) == 0 and f(0, 64, 0, 1) == 0
     g = L.ptxstd_rmsnorm_residual_backward_workspace_bytes
     assert g(1, 64) == 2 * 64 * 4 and g(8, 64) == 8 * 2 * 64 * 4
