@@ -519,7 +519,6 @@ namespace narrow {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWBytes = 128 * BK;  // one weight tile of a stage
 constexpr uint32_t kMaxStages = 12;
-constexpr uint32_t kMaxCluster = 8;
 
 enum : uint32_t { kDetailProducer = 0x3900, kDetailMma = 0x3A00, kDetailEpilogue = 0x3B00 };
 
@@ -775,6 +774,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 t5::idesc_with_field(t0, 4, 2, j, idesc[j]);
             }
             const uint32_t slot_cols = 4 * (G + tok_tiles);
+            // a column of the copied scales holds 32 rows: a 64-token tile may start at the third
+            const uint32_t x_col = 4 * G + (tok0 % 128) / 32;
             uint32_t stage = 0, phase = 0;
             for (uint32_t kb = k_lo; kb < k_hi; ++kb) {
                 if (!mbar_wait(&b.full[stage], phase)) {
@@ -798,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     for (uint32_t j = 0; j < kMmas; ++j)
                         if (j < live)
                             t5::mma_mxf8f6f4_block32(tmem + g * T, wd + 2 * j, xd + 2 * j,
-                                                     idesc[j], slot + 4 * g, slot + 4 * G,
+                                                     idesc[j], slot + 4 * g, slot + x_col,
                                                      kb > k_lo || j > 0);
                 }
                 t5::commit(&b.empty[stage]);
@@ -849,7 +850,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         switch (p.split) {
         case 1: narrow_epilogue<GATED, 1>(p, e, pa, rank, block, tok0, bias); break;
         case 2: narrow_epilogue<GATED, 2>(p, e, pa, rank, block, tok0, bias); break;
+        case 3: narrow_epilogue<GATED, 3>(p, e, pa, rank, block, tok0, bias); break;
         case 4: narrow_epilogue<GATED, 4>(p, e, pa, rank, block, tok0, bias); break;
+        case 5: narrow_epilogue<GATED, 5>(p, e, pa, rank, block, tok0, bias); break;
+        case 6: narrow_epilogue<GATED, 6>(p, e, pa, rank, block, tok0, bias); break;
         default: narrow_epilogue<GATED, 8>(p, e, pa, rank, block, tok0, bias); break;
         }
     }
@@ -940,66 +944,94 @@ int launch_wide(Operand a, int a_type, Operand b, Operand b2, int b_type, const 
     return ptxstd::launch_status();
 }
 
-// Token columns of a narrow CTA. The accumulators (one, or two when gated) and the scale slots
-// share 512 TMEM columns, so a gated CTA takes up to 128 tokens, a linear one up to 256.
-uint32_t narrow_tokens(int64_t M, bool gated) {
-    const int64_t cap = gated ? 128 : 256;
-    const int64_t t = (M + 15) / 16 * 16;
-    return static_cast<uint32_t>(t < cap ? t : cap);
+// How a narrow call runs: token columns of a CTA, K slices of a cluster, CTAs per SM.
+struct NarrowPlan {
+    uint32_t tokens, split, stages, tmem_cols, smem;
+    double us;  // estimated time
+};
+
+constexpr uint32_t kHalfSmem = 111 * 1024, kFullSmem = 225 * 1024;
+
+// The ring of one CTA, with `two` CTAs on an SM or one; false where it does not fit.
+bool narrow_ring(NarrowPlan& p, uint32_t G, uint32_t tokens, bool two) {
+    using namespace narrow;
+    const uint32_t tok_tiles = (tokens + 127) / 128, slot_cols = 4 * (G + tok_tiles);
+    const uint32_t per_stage = G * kWBytes + tokens * BK + (G + tok_tiles) * 512;
+    p.tokens = tokens;
+    p.stages = (two ? kHalfSmem : kFullSmem) / per_stage;
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    if (p.stages < 2) return false;
+    const uint32_t cols = G * tokens + p.stages * slot_cols;
+    if (cols > (two ? 256u : 512u)) return false;
+    // TMEM waits inside clusters must not be able to form a cycle, whatever else runs on the GPU
+    // (another stream's call, the next call's early start): a CTA that is to be alone takes all of
+    // its SM's shared memory and may then have all of its TMEM; the others take half of TMEM and
+    // more than a third of the shared memory, so that two is the most an SM holds.
+    p.tmem_cols = two ? 256 : 512;
+    p.smem = two ? p.stages * per_stage + 1024 : kFullSmem + 1024;
+    if (p.smem < 78 * 1024) p.smem = 78 * 1024;
+    const uint32_t part = G * tokens * 128 * 4 + 1024;
+    return p.smem >= part;
+}
+
+// The plan with the least estimated time. The model, fitted to sweeps of both choices over
+// 1 <= M <= 1000 on a B200 (within 15 % of the measured times at 8 to 40 us): an SM takes in about
+// 95 GB/s, a CTA's start and end cost 1.5 us that CTAs sharing an SM overlap, the exchange of
+// partial sums 1 us and 30 GB/s; a launch 2.5 us. At M = 200, N = 4128, K = 2080 it takes 64-token
+// tiles without a split: 8.2 us, against 10.5 us for one 208-token tile split in two and 9.8 us
+// for the wide kernel.
+NarrowPlan narrow_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+    const uint32_t G = gated ? 2 : 1, cap = gated ? 128 : 256;
+    const int64_t blocks = (N + 127) / 128, num_k = (K + BK - 1) / BK;
+    const int64_t sms = ptxstd::sm_count();
+    NarrowPlan best = {};
+    best.us = 1e30;
+    const int64_t whole = (M + 15) / 16 * 16;
+    // one tile of all tokens, or tiles of 64, 128 or 256 (a tile must not straddle a scale tile)
+    for (const int64_t t : {whole, int64_t{64}, int64_t{128}, int64_t{256}}) {
+        if (t > cap || (t != whole && t >= M)) continue;
+        const int64_t ytiles = (M + t - 1) / t;
+        for (const bool two : {false, true}) {
+            NarrowPlan p = {};
+            if (!narrow_ring(p, G, static_cast<uint32_t>(t), two)) continue;
+            const double stage = G * 16896.0 + t * 132.0;
+            for (const uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u}) {
+                if (s > 1 && num_k < 2 * s) break;
+                const int64_t ctas = blocks * ytiles * s;
+                // clusters of more than two leave SMs of a processing cluster unused
+                const int64_t slots = (s > 2 ? sms * 9 / 10 : sms) / s * s * (two ? 2 : 1);
+                const int64_t waves = (ctas + slots - 1) / slots;
+                // CTAs that share an SM share its intake
+                const double sharing = two ? (ctas > sms ? 2.0 : 1.5) : 1.0;
+                const double intake =
+                    sharing * static_cast<double>((num_k + s - 1) / s) * stage / 95e3;
+                const double exchange = s > 1 ? 1.0 + t * G * 512.0 * (s - 1) / s / 30e3 : 0.0;
+                const double us = 2.5 + waves * ((two && waves > 1 ? 0.75 : 1.5) + intake + exchange);
+                if (us < best.us) {
+                    best = p;
+                    best.split = s;
+                    best.us = us;
+                }
+            }
+        }
+    }
+    return best;
 }
 
 template <bool GATED>
-int launch_narrow(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e,
-                  int64_t M, int64_t N, int64_t K, cudaStream_t stream) {
+int launch_narrow(const NarrowPlan& plan, Operand a, int a_type, Operand b, Operand b2, int b_type,
+                  const Epi& e, int64_t M, int64_t N, int64_t K, cudaStream_t stream) {
     using namespace narrow;
-    constexpr uint32_t G = GATED ? 2 : 1;
     Shape p = {};
     p.M = static_cast<uint32_t>(M);
     p.N = static_cast<uint32_t>(N);
     p.K = static_cast<uint32_t>(K);
-    p.tokens = narrow_tokens(M, GATED);
-    const uint32_t tok_tiles = (p.tokens + 127) / 128;
-    const uint32_t per_stage = G * kWBytes + p.tokens * BK + (G + tok_tiles) * 512;
-    // Two CTAs per SM where the ring allows it (each at most half of the SM's shared memory and
-    // 256 TMEM columns), so that one CTA's prologue and epilogue run beside the other's stream.
-    const uint32_t half_smem = 112 * 1024 - 1024, full_smem = 225 * 1024;
-    const uint32_t slot_cols = 4 * (G + tok_tiles);
-    p.stages = half_smem / per_stage;
-    const bool two = p.stages >= 2 && G * p.tokens + p.stages * slot_cols <= 256;
-    if (!two) p.stages = full_smem / per_stage;
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    const uint32_t cols = G * p.tokens + p.stages * slot_cols;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < cols) p.tmem_cols *= 2;
-    if (p.tmem_cols > 512) return PTXSTD_EINVAL;
-    if (two) p.tmem_cols = 256;
-    uint32_t smem = p.stages * per_stage + 1024;
-    const uint32_t part = G * p.tokens * 128 * 4 + 1024;
-    if (smem < part) smem = part;
-    // TMEM waits inside clusters must not be able to form a cycle, whatever else runs on the GPU
-    // (another stream's call, the next call's early start): a CTA with more than 256 columns takes
-    // all of its SM's shared memory, the others at least a third plus, so that two is the most
-    // an SM holds and their TMEM always fits.
-    if (p.tmem_cols > 256) smem = full_smem + 1024;
-    else if (smem < 78 * 1024) smem = 78 * 1024;
-
-    // K slices: the split that fills the resident CTA slots best, counting a fixed cost of a few
-    // stages for each CTA's start and end.
+    p.tokens = plan.tokens;
+    p.stages = plan.stages;
+    p.split = plan.split;
+    p.tmem_cols = plan.tmem_cols;
+    const uint32_t smem = plan.smem;
     const int64_t blocks = (N + 127) / 128, ytiles = (M + p.tokens - 1) / p.tokens;
-    const int64_t num_k = (K + BK - 1) / BK;
-    const int64_t slots = static_cast<int64_t>(ptxstd::sm_count()) * (two ? 2 : 1);
-    double best = 0;
-    for (uint32_t s = 1; s <= kMaxCluster; s *= 2) {
-        if (s > 1 && num_k < 2 * s) break;
-        const int64_t ctas = blocks * ytiles * s;
-        const int64_t waves = (ctas + slots - 1) / slots;
-        const double cost = static_cast<double>(waves) *
-                            (static_cast<double>((num_k + s - 1) / s) + 6.0);
-        if (s == 1 || cost < best) {
-            best = cost;
-            p.split = s;
-        }
-    }
 
     Maps maps = {};
     int st = operand_maps(&maps.x, &maps.sfx, a, M, K, p.tokens);
@@ -1035,15 +1067,27 @@ int launch_narrow(Operand a, int a_type, Operand b, Operand b2, int b_type, cons
     return ptxstd::launch_status();
 }
 
-// Rows up to which the narrow kernel runs: its 256 token columns read every weight once, while a
-// 256-row tile of the wide kernel would be padding for the most part.
-constexpr int64_t kNarrowRows = 256;
+// Estimated time of the wide kernel: a pair's tile costs about 0.31 us per stage while few pairs
+// are active, 0.41 us when all are.
+double wide_us(int64_t M, int64_t N, int64_t K, bool gated) {
+    const int64_t tile_n = gated ? 128 : 256, pairs = ptxstd::sm_count() / 2;
+    const int64_t tiles = ((M + 255) / 256) * ((N + tile_n - 1) / tile_n);
+    const int64_t waves = (tiles + pairs - 1) / pairs, num_k = (K + BK - 1) / BK;
+    return 2.5 + waves * (2.0 + num_k * (tiles > pairs ? 0.41 : 0.31));
+}
+
+// The narrow kernel where its estimate is clearly the better one. Above 1024 rows the wide kernel's
+// 256-row tiles fill the GPU at every size that matters and the narrow plan is not considered.
+constexpr int64_t kNarrowRows = 1024;
 
 template <bool GATED>
 int dispatch(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e, int64_t M,
              int64_t N, int64_t K, cudaStream_t stream) {
-    if (M <= kNarrowRows)
-        return launch_narrow<GATED>(a, a_type, b, b2, b_type, e, M, N, K, stream);
+    if (M <= kNarrowRows) {
+        const NarrowPlan plan = narrow_plan(M, N, K, GATED);
+        if (plan.us < 0.95 * wide_us(M, N, K, GATED))
+            return launch_narrow<GATED>(plan, a, a_type, b, b2, b_type, e, M, N, K, stream);
+    }
     return launch_wide<GATED>(a, a_type, b, b2, b_type, e, M, N, K, stream);
 }
 
