@@ -4,6 +4,9 @@ Each .cu / .cpp is compiled to an object under ptx-std_b200/_build/ (rebuilt whe
 header is newer than its object), then linked with the CUDA runtime linked statically, so the
 library does not depend on which libcudart the host process (e.g. torch) has loaded.
 
+It also builds ptxstd/_ffn.so, the extension module behind the Python calls of the feed-forward
+operators (csrc/py/ffn_module.cpp: g++ against the installed torch and libptxstd.so).
+
     python ptx-std_b200/build.py [--force] [-j N]
 """
 
@@ -77,7 +80,36 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_module(force)
     return LIB
+
+
+MODULE_SRC = os.path.join(CSRC, "py", "ffn_module.cpp")
+MODULE = os.path.join(HERE, "ptxstd", "_ffn.so")
+
+
+def build_module(force: bool = False) -> str:
+    """ptxstd/_ffn.so, rebuilt when its source, the C header or this file is newer."""
+    inputs = [MODULE_SRC, os.path.join(ROOT, "include", "ptxstd.h"), __file__]
+    if not force and os.path.exists(MODULE) and \
+            os.path.getmtime(MODULE) > max(os.path.getmtime(f) for f in inputs):
+        return MODULE
+    import importlib.util
+    import sysconfig
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    inc = [os.path.join(torch, "include"), os.path.join(cuda, "include"),
+           sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+    lib = os.path.join(torch, "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden"] + [a for i in inc for a in ("-isystem", i)] + \
+          [MODULE_SRC, "-o", MODULE, "-L" + lib, "-L" + HERE, "-ltorch_python", "-ltorch_cuda",
+           "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-lptxstd",
+           "-Wl,-rpath," + lib, "-Wl,-rpath,$ORIGIN/.."]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {MODULE_SRC}:\n{r.stdout}\n{r.stderr}")
+    return MODULE
 
 
 def main() -> int:
