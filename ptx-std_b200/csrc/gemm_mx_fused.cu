@@ -9,7 +9,7 @@
 // Two kernels share that contract:
 //
 // 1. wide_kernel, for many rows: the CTA-pair pipeline of gemm_mxfp8.cu (256 x 256 tiles of
-//    cta_group::2 MMAs, 6 stages of 128 K elements, eight epilogue warps per CTA). For the gated
+//    cta_group::2 MMAs, a ring of 128-element K stages, eight epilogue warps per CTA). For the gated
 //    product the pair's 256 B rows are 128 rows of Wg (loaded by CTA 0) and the same 128 of Wu (by
 //    CTA 1), so the accumulator's columns 0..127 are gate and 128..255 up for the same 128
 //    features; an epilogue warp takes 64 columns of each, and the product needs no exchange. A
@@ -46,6 +46,9 @@ using ptxstd::mbar_wait;
 constexpr uint32_t BK = 128;            // K elements (= bytes) per stage
 constexpr uint32_t kMmaK = 32;          // K elements of one mxf8f6f4 MMA
 constexpr uint32_t kMmas = BK / kMmaK;  // 4 per stage, one scale byte each
+// One step of both scale-factor ids of the instruction descriptor (A's at bits 29-30, B's at bits
+// 4-5): MMA j of a stage reads scale byte j.
+constexpr uint32_t kScaleIdStep = (1u << 29) | (1u << 4);
 
 // What the epilogues read and write besides the tensor maps.
 struct Epi {
@@ -68,9 +71,19 @@ __device__ __forceinline__ float f(uint32_t r) { return __uint_as_float(r); }
 namespace wide {
 
 constexpr uint32_t P_BM = 256, P_BN = 256, P_HALF = 128;
-constexpr uint32_t STAGES = 6;
+// Five stages, not the six that would fit: the mainloop runs as fast (8192^3: 372.6 us with five,
+// 372.2 us with six, 389 us with four), and the epilogue warps get three staging buffers each:
+// with a residual, 4096 x 4096 x 1024 takes 26.6 us instead of 40.6 us with one buffer and the
+// residual read by each lane from its own row.
+constexpr uint32_t STAGES = 5;
 constexpr uint32_t kEpiWarps = 8;
-constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;
+// Warpgroup 0 holds the producer and MMA warps and needs few registers; the two epilogue
+// warpgroups hold 128 accumulator columns per thread and take what it gives up (setmaxnreg). The
+// kernel is launched at 168 registers for 384 threads: 128 x 80 + 256 x 208 stay within that.
+constexpr uint32_t kFirstEpiWarp = 4;
+constexpr uint32_t kThreads = 32 * (kFirstEpiWarp + kEpiWarps);
+constexpr uint32_t kRegsCtl = 80, kRegsEpi = 208;
+static_assert(128 * kRegsCtl + 256 * kRegsEpi <= 168 * kThreads, "register split");
 constexpr uint32_t kABytes = P_HALF * BK;
 constexpr uint32_t kBBytes = P_HALF * BK;
 constexpr uint32_t kSfaBytes = 512;
@@ -80,24 +93,28 @@ constexpr uint32_t kSlotCols = 4 + 4 * (P_BN / 128);
 constexpr uint32_t kSfBase = P_BN;
 constexpr uint32_t kTmemCols = 512;
 static_assert(kSfBase + STAGES * kSlotCols <= kTmemCols, "TMEM budget");
-constexpr uint32_t kGroupM = 8;
-constexpr uint32_t kCCols = 32;  // bf16 columns (or 64 MX bytes) per epilogue store
+constexpr uint32_t kGroupM = 16;  // 8192^3: 363 us, against 372 us with 8 and 381 us with 4
+constexpr uint32_t kCCols = 32;   // bf16 columns (or 64 MX bytes) per epilogue store
 using StageBox = ptxstd::epi::Box<kCCols>;
+constexpr uint32_t kBuffers = 3;  // staging buffers of an epilogue warp
 
 struct alignas(1024) Smem {
     uint8_t a[STAGES][kABytes];
     uint8_t b[STAGES][kBBytes];
     uint8_t sfa[STAGES][kSfaBytes];
     uint8_t sfb[STAGES][kSfbBytes];
-    uint8_t cstage[kEpiWarps][StageBox::kBytes];
+    uint8_t cstage[kEpiWarps][kBuffers][StageBox::kBytes];
     uint64_t full[STAGES];
     uint64_t empty[STAGES];
+    uint64_t res_full[kEpiWarps][kBuffers];
     uint64_t tfull;
     uint64_t tempty;
     uint64_t drain;
     uint32_t tmem_base;
     uint32_t abort;
 };
+static_assert(sizeof(Smem::cstage) % 1024 == 0 && (STAGES * (kSfaBytes + kSfbBytes)) % 512 == 0,
+              "staging buffers on swizzle boundaries");
 constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
@@ -107,7 +124,7 @@ struct Maps {
     CUtensorMap a, sfa;
     CUtensorMap b, sfb;    // linear: B; gated: Wg
     CUtensorMap b2, sfb2;  // gated: Wu
-    CUtensorMap c, pre, up, q;
+    CUtensorMap c, pre, up, q, residual;
 };
 
 __device__ __forceinline__ void tile_coords(uint32_t t, uint32_t num_m, uint32_t num_n,
@@ -140,28 +157,85 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint6
         : "memory");
 }
 
-// One epilogue warp's 32 rows, leaving through its staging buffer.
-struct Out {
-    uint32_t stg, lane;
+// One epilogue warp: its 32 rows of a tile, and its staging buffers. Results leave by TMA stores
+// from the buffers in turn, so that a buffer is rewritten when its store of three stores ago has
+// been read. A residual comes the other way: boxes of 32 columns are prefetched into the buffers
+// before the accumulator is complete, each lane adds its row's values, and the bf16 result is
+// written over them and stored from there.
+struct EpiWarp {
+    uint32_t stg, lane;        // .shared::cta address of buffer 0
+    uint64_t* res_full;        // one mbarrier per buffer
+    uint32_t next = 0;         // buffer of the next store, without a residual
+    uint32_t res_parity = 0;   // bit b: the parity that buffer b's next load completes
     int32_t row0;
-    uint32_t row, M, N;  // this lane's row; the result's sizes
+    uint32_t row, M, N;        // this lane's row; the result's sizes
 
-    // 32 bf16 columns r[FIRST..] at col0 of `map`.
+    __device__ __forceinline__ uint32_t buffer(uint32_t b) const {
+        return stg + b * StageBox::kBytes;
+    }
+    __device__ __forceinline__ bool live(uint32_t col) const {
+        return col < N && static_cast<uint32_t>(row0) < M;
+    }
+    // The next buffer of the rotation, free to be written.
+    __device__ __forceinline__ uint32_t rotate() {
+        ptxstd::epi::wait_staging<kBuffers - 1>(lane);
+        const uint32_t b = next;
+        next = next + 1 == kBuffers ? 0 : next + 1;
+        return buffer(b);
+    }
+    // 32 bf16 columns r[FIRST..] at col through the (free) buffer `at`.
+    template <uint32_t FIRST, uint32_t L>
+    __device__ __forceinline__ void store_bf16(const CUtensorMap* map, const uint32_t (&r)[L],
+                                               uint32_t col, uint32_t at) const {
+        ptxstd::epi::stage_store<kCCols, FIRST>(map, at, r, 1.0f, static_cast<int32_t>(col), row0,
+                                                lane);
+    }
     template <uint32_t FIRST, uint32_t L>
     __device__ __forceinline__ void bf16(const CUtensorMap* map, const uint32_t (&r)[L],
-                                         uint32_t col0) const {
-        if (col0 >= N || static_cast<uint32_t>(row0) >= M) return;
-        ptxstd::epi::wait_staging(lane);
-        ptxstd::epi::stage_store<kCCols, FIRST>(map, stg, r, 1.0f, static_cast<int32_t>(col0),
-                                                row0, lane);
+                                         uint32_t col) {
+        if (live(col)) store_bf16<FIRST>(map, r, col, rotate());
     }
-    // Two MX blocks r[FIRST .. FIRST + 63] at col0; returns their scale codes (0 outside N or M).
+    // Residual columns col .. + 31 into buffer b (free: nothing still reads it).
+    __device__ __forceinline__ void load_residual(const CUtensorMap* map, uint32_t col,
+                                                  uint32_t b) const {
+        if (lane == 0 && live(col)) {
+            ptxstd::mbar_arrive_expect_tx(&res_full[b], StageBox::kBytes);
+            asm volatile(
+                "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                " [%0], [%1, {%3, %4}], [%2];" ::"r"(buffer(b)),
+                "l"(reinterpret_cast<uint64_t>(map)), "r"(ptxstd::smem_u32(&res_full[b])),
+                "r"(col), "r"(row0)
+                : "memory");
+        }
+    }
+    // Adds buffer b's residual to r[FIRST..]; false after a timeout.
+    template <uint32_t FIRST, uint32_t L>
+    __device__ __forceinline__ bool add_residual(uint32_t (&r)[L], uint32_t b) {
+        const bool ok = mbar_wait(&res_full[b], (res_parity >> b) & 1u);
+        res_parity ^= 1u << b;
+#pragma unroll
+        for (uint32_t c = 0; c < StageBox::kChunks; ++c) {
+            uint32_t v[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                         : "r"(buffer(b) + StageBox::offset(lane, c))
+                         : "memory");
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t i = FIRST + 8 * c + 2 * k;
+                r[i] = __float_as_uint(f(r[i]) + dt::bf16_lo(v[k]));
+                r[i + 1] = __float_as_uint(f(r[i + 1]) + dt::bf16_hi(v[k]));
+            }
+        }
+        __syncwarp();  // every lane has read its row
+        return ok;
+    }
+    // Two MX blocks r[FIRST .. FIRST + 63] at col through the (free) buffer `at`; returns their
+    // scale codes (0 outside N or M).
     template <uint32_t FIRST, uint32_t L>
     __device__ __forceinline__ uint32_t mx2(const CUtensorMap* map, const uint32_t (&r)[L],
-                                            uint32_t col0, uint32_t type) const {
+                                            uint32_t col, uint32_t type, uint32_t at) const {
         uint32_t codes = 0;
-        const bool any = col0 < N && static_cast<uint32_t>(row0) < M;
-        if (any) ptxstd::epi::wait_staging(lane);
         const uint32_t emax = mx::emax_of(type);
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
@@ -170,45 +244,34 @@ struct Out {
             for (uint32_t i = 0; i < 32; i += 2)
                 m = mx::amax(m, f(r[FIRST + 32 * h + i]), f(r[FIRST + 32 * h + i + 1]));
             const mx::Scale sc = mx::scale_of(m, emax);
-            if (row < M && col0 + 32 * h < N) codes |= sc.code << (8 * h);
+            if (row < M && col + 32 * h < N) codes |= sc.code << (8 * h);
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c) {
                 float v[16];
 #pragma unroll
                 for (uint32_t k = 0; k < 16; ++k) v[k] = f(r[FIRST + 32 * h + 16 * c + k]);
                 const uint2 lo = mx::pack8(type, v, sc.inv), hi = mx::pack8(type, v + 8, sc.inv);
-                if (any)
-                    ptxstd::st_shared_v4(stg + StageBox::offset(lane, 2 * h + c), lo.x, lo.y, hi.x,
-                                         hi.y);
+                ptxstd::st_shared_v4(at + StageBox::offset(lane, 2 * h + c), lo.x, lo.y, hi.x,
+                                     hi.y);
             }
         }
-        if (any) {
-            ptxstd::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                ptxstd::tma_store_2d(map, stg, static_cast<int32_t>(col0), row0);
-                ptxstd::bulk_commit_group();
-            }
+        ptxstd::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            ptxstd::tma_store_2d(map, at, static_cast<int32_t>(col), row0);
+            ptxstd::bulk_commit_group();
         }
         return codes;
     }
 };
 
+// Adds the bias of columns FIRST .. FIRST + 31 of the warp's 128: lane l holds those of columns
+// 4 l .. 4 l + 3.
 template <uint32_t FIRST, uint32_t L>
-__device__ __forceinline__ void add_bias32(uint32_t (&r)[L], const uint16_t* bias, uint32_t col,
-                                           uint32_t N) {
+__device__ __forceinline__ void add_bias32(uint32_t (&r)[L], const float (&bias)[4]) {
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (col + 8 * c < N) w = __ldg(reinterpret_cast<const uint4*>(bias + col + 8 * c));
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t i = FIRST + 8 * c + 2 * k;
-            r[i] = __float_as_uint(f(r[i]) + dt::bf16_lo(v[k]));
-            r[i + 1] = __float_as_uint(f(r[i + 1]) + dt::bf16_hi(v[k]));
-        }
-    }
+    for (uint32_t i = FIRST; i < FIRST + 32; ++i)
+        r[i] = __float_as_uint(f(r[i]) + __shfl_sync(0xffffffffu, bias[i & 3u], (i >> 2) & 31u));
 }
 
 template <uint32_t FIRST, uint32_t L>
@@ -225,51 +288,66 @@ __device__ __forceinline__ void act32(uint32_t (&r)[L], uint32_t kind) {
     });
 }
 
-// The linear epilogue of 32 accumulator columns r[FIRST..] at column `col` of the result.
-template <uint32_t FIRST, uint32_t L>
-__device__ __forceinline__ void linear32(uint32_t (&r)[L], const Out& o, const Epi& e,
-                                         const Maps& maps, uint32_t col) {
-    uint4 res[4];
-    if (e.residual) {
-#pragma unroll
-        for (uint32_t c = 0; c < 4; ++c) {
-            res[c] = make_uint4(0, 0, 0, 0);
-            if (o.row < o.M && col + 8 * c < o.N)
-                res[c] = *reinterpret_cast<const uint4*>(
-                    e.residual + static_cast<size_t>(o.row) * o.N + col + 8 * c);
+// The buffers that hold residual boxes: all of them while nothing but the bf16 result is stored
+// (which replaces the residual in place), else two, the third being the other results'.
+__device__ __forceinline__ uint32_t residual_buffers(const Epi& e) {
+    return e.pre || e.q ? kBuffers - 1 : kBuffers;
+}
+
+// The linear epilogue of 32 accumulator columns r[32 J..], the J-th box of the warp's 128 columns
+// from `col0` on. False after a timeout.
+template <uint32_t J>
+__device__ __forceinline__ bool linear32(uint32_t (&r)[128], EpiWarp& w, const Epi& e,
+                                         const Maps& maps, uint32_t col0, const float (&bias)[4]) {
+    constexpr uint32_t FIRST = 32 * J;
+    const uint32_t col = col0 + FIRST;
+    const bool live = w.live(col);
+    if (e.bias) add_bias32<FIRST>(r, bias);
+    if (e.pre && live) {
+        if (e.residual) {
+            ptxstd::epi::wait_staging<0>(w.lane);
+            w.store_bf16<FIRST>(&maps.pre, r, col, w.buffer(kBuffers - 1));
+        } else {
+            w.store_bf16<FIRST>(&maps.pre, r, col, w.rotate());
         }
     }
-    if (e.bias) add_bias32<FIRST>(r, e.bias, col, o.N);
-    if (e.pre) o.bf16<FIRST>(&maps.pre, r, col);
     act32<FIRST>(r, e.act);
-    if (e.residual) {
-#pragma unroll
-        for (uint32_t c = 0; c < 4; ++c) {
-            const uint32_t v[4] = {res[c].x, res[c].y, res[c].z, res[c].w};
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                const uint32_t i = FIRST + 8 * c + 2 * k;
-                r[i] = __float_as_uint(f(r[i]) + dt::bf16_lo(v[k]));
-                r[i + 1] = __float_as_uint(f(r[i + 1]) + dt::bf16_hi(v[k]));
-            }
-        }
+    if (!e.residual) {
+        if (e.c && live) w.store_bf16<FIRST>(&maps.c, r, col, w.rotate());
+        return true;
     }
-    if (e.c) o.bf16<FIRST>(&maps.c, r, col);
+    bool ok = true;
+    const uint32_t n = residual_buffers(e), b = J % n;
+    if (live) {
+        ok = w.add_residual<FIRST>(r, b);
+        if (e.c) w.store_bf16<FIRST>(&maps.c, r, col, w.buffer(b));
+    }
+    // the next box that has no buffer yet, into the one that is free first
+    if (n == kBuffers) {
+        if (J == 1) {
+            ptxstd::epi::wait_staging<1>(w.lane);  // box 0's store has been read
+            w.load_residual(&maps.residual, col0 + 96, 0);
+        }
+    } else if (J < 2) {
+        ptxstd::epi::wait_staging<0>(w.lane);
+        w.load_residual(&maps.residual, col + 64, b);
+    }
+    return ok;
 }
 
 // h = act(gate) * up for 32 columns: gate r[FIRST..], up r[64 + FIRST..]; h replaces gate.
 template <uint32_t FIRST>
-__device__ __forceinline__ void gated32(uint32_t (&r)[128], const Out& o, const Epi& e,
+__device__ __forceinline__ void gated32(uint32_t (&r)[128], EpiWarp& w, const Epi& e,
                                         const Maps& maps, uint32_t col) {
     if (e.pre) {
-        o.bf16<FIRST>(&maps.pre, r, col);
-        o.bf16<64 + FIRST>(&maps.up, r, col);
+        w.bf16<FIRST>(&maps.pre, r, col);
+        w.bf16<64 + FIRST>(&maps.up, r, col);
     }
     act32<FIRST>(r, e.act);
 #pragma unroll
     for (uint32_t i = 0; i < 32; ++i)
         r[FIRST + i] = __float_as_uint(f(r[FIRST + i]) * f(r[64 + FIRST + i]));
-    if (e.c) o.bf16<FIRST>(&maps.c, r, col);
+    if (e.c) w.bf16<FIRST>(&maps.c, r, col);
 }
 
 template <bool GATED>
@@ -303,6 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptxstd::mbar_init(&s.tfull, 1);
         ptxstd::mbar_init(&s.tempty, 2 * kEpiWarps);
         ptxstd::mbar_init(&s.drain, 1);
+        for (uint32_t i = 0; i < kEpiWarps * kBuffers; ++i)
+            ptxstd::mbar_init(&s.res_full[0][0] + i, 1);
         s.abort = 0;
         ptxstd::fence_mbarrier_init();
     }
@@ -321,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
+        ptxstd::setmaxnreg_dec<kRegsCtl>();
         if (ptxstd::elect_one()) {
             const CUtensorMap* mb_ = GATED && rank == 1 ? &maps.b2 : &maps.b;
             uint32_t stage = 0, phase = 0, issued = 0, issued_parity = 0;
@@ -370,76 +451,121 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader) ----------------
-        if (rank == 0 && ptxstd::elect_one()) {
-            uint32_t idesc0 = 0;
-            t5::idesc_mxf8f6f4(atype, btype, P_BM, P_BN, idesc0);
-            uint32_t idesc[kMmas];
-#pragma unroll
-            for (uint32_t j = 0; j < kMmas; ++j) {
-                uint32_t t0 = 0;
-                t5::idesc_with_field(idesc0, 29, 2, j, t0);   // scale-factor A id
-                t5::idesc_with_field(t0, 4, 2, j, idesc[j]);  // scale-factor B id
-            }
+        ptxstd::setmaxnreg_dec<kRegsCtl>();
+        // The whole warp runs the loops and one lane issues: with uniform control flow the operands
+        // stay in uniform registers, which the tensor instructions take them from. (Inside a loop
+        // of one elected lane the compiler did that for some epilogues and not for others, and
+        // then a stage took 888 clocks to issue instead of 430: 8192^3 in 443 us, not 361 us.)
+        if (rank == 0) {
+            const bool lead = ptxstd::elect_one();
+            uint32_t idesc = 0;
+            t5::idesc_mxf8f6f4(atype, btype, P_BM, P_BN, idesc);
+            const uint64_t a0 = t5::smem_desc_k128(ptxstd::smem_u32(s.a[0]));
+            const uint64_t b0 = t5::smem_desc_k128(ptxstd::smem_u32(s.b[0]));
+            const uint64_t sfa0 = t5::smem_desc_nosw(ptxstd::smem_u32(s.sfa[0]), 0, 128);
+            const uint64_t sfb0 = t5::smem_desc_nosw(ptxstd::smem_u32(s.sfb[0]), 0, 128);
+            const uint32_t empty0 = ptxstd::smem_u32(&s.empty[0]);
+            const uint32_t peer_empty0 = ptxstd::mapa_shared(empty0, 1);
+            const uint32_t tfull = ptxstd::smem_u32(&s.tfull);
+            const uint32_t peer_tfull = ptxstd::mapa_shared(tfull, 1);
             uint32_t stage = 0, phase = 0, acc_phase = 0;
-            for (uint32_t t = pair; t < num_tiles && !aborted(s); t += n_pairs) {
-                if (!mbar_wait(&s.tempty, acc_phase ^ 1u)) {
-                    fail(s, err, kDetailMma | 0x90);
+            for (uint32_t t = pair; t < num_tiles; t += n_pairs) {
+                if (!__all_sync(0xffffffffu, !aborted(s) && mbar_wait(&s.tempty, acc_phase ^ 1u))) {
+                    if (lead && !aborted(s)) fail(s, err, kDetailMma | 0x90);
                     break;
                 }
                 t5::fence_after_thread_sync();
                 bool ok = true;
                 for (uint32_t kb = 0; kb < num_k; ++kb) {
-                    if (!mbar_wait(&s.full[stage], phase)) {
-                        fail(s, err, kDetailMma | 0x80 | stage);
+                    if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase))) {
+                        if (lead) fail(s, err, kDetailMma | 0x80 | stage);
                         ok = false;
                         break;
                     }
                     t5::fence_after_thread_sync();
-                    const uint64_t ad = t5::smem_desc_k128(ptxstd::smem_u32(s.a[stage]));
-                    const uint64_t bd = t5::smem_desc_k128(ptxstd::smem_u32(s.b[stage]));
+                    const uint64_t ad = a0 + stage * (kABytes >> 4);
+                    const uint64_t bd = b0 + stage * (kBBytes >> 4);
+                    const uint64_t sfa = sfa0 + stage * (kSfaBytes >> 4);
+                    const uint64_t sfb = sfb0 + stage * (kSfbBytes >> 4);
                     const uint32_t slot = tmem + kSfBase + stage * kSlotCols;
-                    t5::cp_32x128b_warpx4_pair(
-                        slot, t5::smem_desc_nosw(ptxstd::smem_u32(s.sfa[stage]), 0, 128));
-#pragma unroll
-                    for (uint32_t h = 0; h < P_BN / 128; ++h)
-                        t5::cp_32x128b_warpx4_pair(
-                            slot + 4 + 4 * h,
-                            t5::smem_desc_nosw(ptxstd::smem_u32(s.sfb[stage] + 512 * h), 0, 128));
                     const uint32_t live = (K - kb * BK) / kMmaK;  // MMAs inside K
+                    if (lead) {
+                        t5::cp_32x128b_warpx4_pair(slot, sfa);
 #pragma unroll
-                    for (uint32_t j = 0; j < kMmas; ++j)
-                        if (j < live)
-                            mma_pair(tmem, ad + 2 * j, bd + 2 * j, idesc[j], slot, slot + 4,
-                                     (kb | j) != 0u);
-                    const uint32_t em = ptxstd::smem_u32(&s.empty[stage]);
-                    t5::commit_pair(em);
-                    t5::commit_pair(ptxstd::mapa_shared(em, 1));
+                        for (uint32_t h = 0; h < P_BN / 128; ++h)
+                            t5::cp_32x128b_warpx4_pair(slot + 4 + 4 * h, sfb + 32 * h);
+#pragma unroll
+                        for (uint32_t j = 0; j < kMmas; ++j)
+                            if (j < live)
+                                mma_pair(tmem, ad + 2 * j, bd + 2 * j, idesc + j * kScaleIdStep,
+                                         slot, slot + 4, (kb | j) != 0u);
+                        t5::commit_pair(empty0 + 8 * stage);
+                        t5::commit_pair(peer_empty0 + 8 * stage);
+                    }
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                const uint32_t fu = ptxstd::smem_u32(&s.tfull);
-                t5::commit_pair(fu);
-                t5::commit_pair(ptxstd::mapa_shared(fu, 1));
+                if (lead) {
+                    t5::commit_pair(tfull);
+                    t5::commit_pair(peer_tfull);
+                }
                 acc_phase ^= 1u;
             }
-            t5::commit_pair(ptxstd::smem_u32(&s.drain));
-            mbar_wait(&s.drain, 0);
+            if (lead) {
+                t5::commit_pair(ptxstd::smem_u32(&s.drain));
+                mbar_wait(&s.drain, 0);
+            }
+            __syncwarp();
         }
+    } else if (warp < kFirstEpiWarp) {
+        ptxstd::setmaxnreg_dec<kRegsCtl>();  // idle: its share of registers goes to the epilogue
     } else {
-        // ---------------- epilogue: warps 2..9 of both CTAs ----------------
-        const uint32_t q = warp & 3u;
-        const uint32_t half = (warp - 2u) >> 2;
+        // ---------------- epilogue: warps 4..11 of both CTAs ----------------
+        ptxstd::setmaxnreg_inc<kRegsEpi>();
+        const uint32_t ew = warp - kFirstEpiWarp, q = warp & 3u, half = ew >> 2;
         uint32_t acc_phase = 0;
         const uint32_t tempty_leader = ptxstd::mapa_shared(ptxstd::smem_u32(&s.tempty), 0);
         const size_t q_tiles_k = mx::tiles_k(N / 32);
+        EpiWarp w;
+        w.stg = ptxstd::smem_u32(s.cstage[ew][0]);
+        w.lane = lane;
+        w.res_full = s.res_full[ew];
+        w.M = M;
+        w.N = N;
         for (uint32_t t = pair; t < num_tiles; t += n_pairs) {
+            uint32_t mb, nb;
+            tile_coords(t, num_m, num_n, mb, nb);
+            w.row0 = static_cast<int32_t>(mb * P_BM + rank * P_HALF + 32 * q);
+            w.row = static_cast<uint32_t>(w.row0) + lane;
+            const uint32_t col0 = nb * kTileN + half * (GATED ? 64 : 128);
+            // while the accumulator is being computed: the bias to registers, residual boxes to the
+            // staging buffers
+            float bias[4] = {};
+            if (!GATED && e.bias && col0 + 4 * lane < N) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(e.bias + col0 + 4 * lane));
+                bias[0] = dt::bf16_lo(v.x);
+                bias[1] = dt::bf16_hi(v.x);
+                bias[2] = dt::bf16_lo(v.y);
+                bias[3] = dt::bf16_hi(v.y);
+            }
+            if (!GATED && e.residual) {
+                ptxstd::epi::wait_staging<0>(lane);
+                const uint32_t n = residual_buffers(e);
+                for (uint32_t b = 0; b < n; ++b) w.load_residual(&maps.residual, col0 + 32 * b, b);
+            }
+
             bool ok = !aborted(s) && mbar_wait(&s.tfull, acc_phase);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
                 if (lane == 0 && !aborted(s)) fail(s, err, kDetailEpilogue | 0x80);
+                // the residual boxes under way have to land before this block may end
+                if (!GATED && e.residual)
+                    for (uint32_t b = 0; b < residual_buffers(e); ++b)
+                        if (w.live(col0 + 32 * b))
+                            mbar_wait(&w.res_full[b], (w.res_parity >> b) & 1u);
                 break;
             }
             t5::fence_after_thread_sync();
@@ -461,43 +587,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             t5::fence_before_thread_sync();
             __syncwarp();
-            if (lane == 0) ptxstd::mbar_arrive_cluster(tempty_leader);
+            if (lane == 0) ptxstd::mbar_arrive_cluster_relaxed(tempty_leader);
             acc_phase ^= 1u;
 
-            uint32_t mb, nb;
-            tile_coords(t, num_m, num_n, mb, nb);
-            Out o;
-            o.stg = ptxstd::smem_u32(s.cstage[warp - 2u]);
-            o.lane = lane;
-            o.row0 = static_cast<int32_t>(mb * P_BM + rank * P_HALF + 32 * q);
-            o.row = static_cast<uint32_t>(o.row0) + lane;
-            o.M = M;
-            o.N = N;
-            const uint32_t col0 = nb * kTileN + half * (GATED ? 64 : 128);
-            const bool in_tiles = o.row < mx::padded_rows(M);  // a row of the scale tiles
+            const bool in_tiles = w.row < mx::padded_rows(M);  // a row of the scale tiles
             if constexpr (GATED) {
-                gated32<0>(r, o, e, maps, col0);
-                gated32<32>(r, o, e, maps, col0 + 32);
+                gated32<0>(r, w, e, maps, col0);
+                gated32<32>(r, w, e, maps, col0 + 32);
                 if (e.q) {
-                    const uint32_t codes = o.mx2<0>(&maps.q, r, col0, e.q_type);
+                    uint32_t codes = 0;
+                    if (w.live(col0)) codes = w.mx2<0>(&maps.q, r, col0, e.q_type, w.rotate());
                     // the tile's four scale columns: this warp holds two of them
                     if (in_tiles)
                         *reinterpret_cast<uint16_t*>(
-                            e.sfq + mx::word_offset(o.row, nb, q_tiles_k) + 2 * half) =
+                            e.sfq + mx::word_offset(w.row, nb, q_tiles_k) + 2 * half) =
                             static_cast<uint16_t>(codes);
                 }
             } else {
-                linear32<0>(r, o, e, maps, col0);
-                linear32<32>(r, o, e, maps, col0 + 32);
-                linear32<64>(r, o, e, maps, col0 + 64);
-                linear32<96>(r, o, e, maps, col0 + 96);
-                if (e.q) {
-                    uint32_t codes = o.mx2<0>(&maps.q, r, col0, e.q_type);
-                    codes |= o.mx2<64>(&maps.q, r, col0 + 64, e.q_type) << 16;
-                    if (in_tiles && col0 < N)
-                        *reinterpret_cast<uint32_t*>(
-                            e.sfq + mx::word_offset(o.row, nb * 2 + half, q_tiles_k)) = codes;
-                }
+                // with a residual the MX results take the last buffer, else the rotation's
+                auto mx_buffer = [&] {
+                    if (!e.residual) return w.rotate();
+                    ptxstd::epi::wait_staging<0>(lane);
+                    return w.buffer(kBuffers - 1);
+                };
+                uint32_t codes = 0;
+                ok = linear32<0>(r, w, e, maps, col0, bias);
+                ok &= linear32<1>(r, w, e, maps, col0, bias);
+                if (e.q && w.live(col0)) codes = w.mx2<0>(&maps.q, r, col0, e.q_type, mx_buffer());
+                ok &= linear32<2>(r, w, e, maps, col0, bias);
+                ok &= linear32<3>(r, w, e, maps, col0, bias);
+                if (e.q && w.live(col0 + 64))
+                    codes |= w.mx2<64>(&maps.q, r, col0 + 64, e.q_type, mx_buffer()) << 16;
+                if (e.q && in_tiles && col0 < N)
+                    *reinterpret_cast<uint32_t*>(
+                        e.sfq + mx::word_offset(w.row, nb * 2 + half, q_tiles_k)) = codes;
+                // a residual that did not arrive: recorded, and the other roles stop
+                if (__any_sync(0xffffffffu, !ok) && lane == 0)
+                    fail(s, err, kDetailEpilogue | 0x40);
             }
         }
         ptxstd::epi::drain(lane);
@@ -762,54 +888,49 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (ptxstd::elect_one()) {
-            uint32_t idesc0 = 0;
-            t5::idesc_mxf8f6f4(wtype, xtype, 128, T, idesc0);
-            uint32_t idesc[kMmas];
-#pragma unroll
-            for (uint32_t j = 0; j < kMmas; ++j) {
-                uint32_t t0 = 0;
-                t5::idesc_with_field(idesc0, 29, 2, j, t0);
-                t5::idesc_with_field(t0, 4, 2, j, idesc[j]);
-            }
-            const uint32_t slot_cols = 4 * (G + tok_tiles);
-            // a column of the copied scales holds 32 rows: a 64-token tile may start at the third
-            const uint32_t x_col = 4 * G + (tok0 % 128) / 32;
-            uint32_t stage = 0, phase = 0;
-            for (uint32_t kb = k_lo; kb < k_hi; ++kb) {
-                if (!mbar_wait(&b.full[stage], phase)) {
+        // ---------------- MMA issuer (uniform control flow, one lane issues) ----------------
+        const bool lead = ptxstd::elect_one();
+        uint32_t idesc = 0;
+        t5::idesc_mxf8f6f4(wtype, xtype, 128, T, idesc);
+        const uint32_t slot_cols = 4 * (G + tok_tiles);
+        // a column of the copied scales holds 32 rows: a 64-token tile may start at the third
+        const uint32_t x_col = 4 * G + (tok0 % 128) / 32;
+        const uint32_t st0 = ptxstd::smem_u32(base), sf0 = ptxstd::smem_u32(sf_base);
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t kb = k_lo; kb < k_hi; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&b.full[stage], phase))) {
+                if (lead) {
                     ptxstd::record_error(err, PTXSTD_ETIMEOUT, kDetailMma | stage);
                     *abort_flag = 1u;
-                    break;
                 }
-                t5::fence_after_thread_sync();
-                const uint32_t st = ptxstd::smem_u32(base + stage * stage_bytes);
-                const uint32_t sf = ptxstd::smem_u32(sf_base + stage * sf_bytes);
-                const uint32_t slot = tmem + G * T + stage * slot_cols;
+                break;
+            }
+            t5::fence_after_thread_sync();
+            const uint32_t slot = tmem + G * T + stage * slot_cols;
+            const uint64_t sfd = t5::smem_desc_nosw(sf0 + stage * sf_bytes, 0, 128);
+            const uint64_t wd = t5::smem_desc_k128(st0 + stage * stage_bytes);
+            const uint64_t xd = wd + G * (kWBytes >> 4);
+            const uint32_t live = (p.K - kb * BK) / kMmaK;
+            if (lead) {
                 for (uint32_t j = 0; j < G + tok_tiles; ++j)
-                    t5::cp_32x128b_warpx4(slot + 4 * j,
-                                          t5::smem_desc_nosw(sf + 512 * j, 0, 128));
-                const uint64_t xd = t5::smem_desc_k128(st + G * kWBytes);
-                const uint32_t live = (p.K - kb * BK) / kMmaK;
+                    t5::cp_32x128b_warpx4(slot + 4 * j, sfd + 32 * j);
 #pragma unroll
-                for (uint32_t g = 0; g < G; ++g) {
-                    const uint64_t wd = t5::smem_desc_k128(st + g * kWBytes);
+                for (uint32_t g = 0; g < G; ++g)
 #pragma unroll
                     for (uint32_t j = 0; j < kMmas; ++j)
                         if (j < live)
-                            t5::mma_mxf8f6f4_block32(tmem + g * T, wd + 2 * j, xd + 2 * j,
-                                                     idesc[j], slot + 4 * g, slot + x_col,
-                                                     kb > k_lo || j > 0);
-                }
+                            t5::mma_mxf8f6f4_block32(
+                                tmem + g * T, wd + g * (kWBytes >> 4) + 2 * j, xd + 2 * j,
+                                idesc + j * kScaleIdStep, slot + 4 * g, slot + x_col,
+                                kb > k_lo || j > 0);
                 t5::commit(&b.empty[stage]);
-                if (++stage == p.stages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
             }
-            t5::commit(&b.done);
+            if (++stage == p.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
         }
+        if (lead) t5::commit(&b.done);
     }
     __syncwarp();
 
@@ -899,6 +1020,10 @@ int launch_wide(Operand a, int a_type, Operand b, Operand b2, int b_type, const 
     if (e.c && (st = ptxstd::epi::make_store_map<kCCols>(&maps.c, e.c, M, N))) return st;
     if (e.pre && (st = ptxstd::epi::make_store_map<kCCols>(&maps.pre, e.pre, M, N))) return st;
     if (e.up && (st = ptxstd::epi::make_store_map<kCCols>(&maps.up, e.up, M, N))) return st;
+    if (e.residual &&
+        (st = ptxstd::epi::make_store_map<kCCols>(&maps.residual,
+                                                  const_cast<uint16_t*>(e.residual), M, N)))
+        return st;
     if (e.q && (st = ptxstd::make_tmap_2d(&maps.q, e.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, N, M, N, 64,
                                           ptxstd::epi::kRows, CU_TENSOR_MAP_SWIZZLE_64B)))
         return st;
