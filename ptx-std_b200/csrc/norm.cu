@@ -344,14 +344,13 @@ __device__ __forceinline__ Oct load_planes(const float4* src, uint32_t nv, uint3
     return {{pack2f(a.x, a.y), pack2f(a.z, a.w), pack2f(b.x, b.y), pack2f(b.z, b.w)}};
 }
 
-constexpr uint32_t kGroupThreads = 256, kGroups = 3;
-
-template <int V>
-__global__ void __launch_bounds__(kGroupThreads* kGroups, 1)
+template <int V, uint32_t THREADS, uint32_t GROUPS>
+__global__ void __launch_bounds__(THREADS* GROUPS, 1)
     norm_ring_kernel(const __grid_constant__ Fwd p, uint32_t stages, uint32_t* err) {
     extern __shared__ uint4 ring_smem[];
     __shared__ RingState state;
-    __shared__ float4 red[kGroups][3][2];  // eight warps' partial sums; a buffer per exchange
+    constexpr uint32_t kWarps = THREADS / 32;
+    __shared__ float4 red[GROUPS][3][kWarps / 4];  // the warps' partial sums; a buffer per exchange
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t nv = p.cols / 8;
     const size_t k_tiles = mx::tiles_k(p.cols / 32);
@@ -382,26 +381,34 @@ __global__ void __launch_bounds__(kGroupThreads* kGroups, 1)
         pad_row(p, row, tid, blockDim.x, k_tiles);
     __syncthreads();
 
-    const uint32_t g = warp / (kGroupThreads / 32);
-    const uint32_t t = tid - g * kGroupThreads, gw = t >> 5;
+    const uint32_t g = warp / kWarps;
+    const uint32_t t = tid - g * THREADS, gw = t >> 5;
     const float inv_d = 1.0f / static_cast<float>(p.cols);
     auto group_sum = [&](float v, float4* buf) {
         v = warp_sum(v);
         if (lane == 0) reinterpret_cast<float*>(buf)[gw] = v;
-        group_sync(g, kGroupThreads);
-        const float4 a = buf[0], b = buf[1];
-        return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+        group_sync(g, THREADS);
+        float4 a = buf[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kWarps / 4; ++i) {
+            const float4 b = buf[i];
+            a.x += b.x;
+            a.y += b.y;
+            a.z += b.z;
+            a.w += b.w;
+        }
+        return (a.x + a.y) + (a.z + a.w);
     };
     uint32_t stage = g % stages, parity = (g / stages) & 1u, flip = 0, k = g;
     for (uint32_t row = blockIdx.x + g * gridDim.x; row < p.rows;
-         row += kGroups * gridDim.x, k += kGroups) {
+         row += GROUPS * gridDim.x, k += GROUPS) {
         ring.wait(k, stage, parity, err, kDetailFwd);
         const uint4* const xs = stage0 + static_cast<size_t>(stage) * arrays * nv;
         const size_t base = static_cast<size_t>(row) * p.cols;
         uint4 xv[V], yv[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint32_t i = t + j * kGroupThreads;
+            const uint32_t i = t + j * THREADS;
             xv[j] = yv[j] = make_uint4(0, 0, 0, 0);
             if (i < nv) {
                 xv[j] = xs[i];
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(kGroupThreads* kGroups, 1)
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const uint32_t i = t + j * kGroupThreads;
+                const uint32_t i = t + j * THREADS;
                 if (i >= nv) continue;
                 Oct x = widen(xv[j]), y = widen(yv[j]);
                 const Oct f = load_planes(c, nv, i);
@@ -450,12 +457,12 @@ __global__ void __launch_bounds__(kGroupThreads* kGroups, 1)
         sr.pad(p, t);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint32_t i = t + j * kGroupThreads;
+            const uint32_t i = t + j * THREADS;
             const bool on = i < nv;
             finish8(p, xv[j], on ? w[i] : make_uint4(0, 0, 0, 0), rx, base, i, on, lane, sr);
         }
         flip ^= 1u;
-        stage += kGroups;
+        stage += GROUPS;
         while (stage >= stages) {
             stage -= stages;
             parity ^= 1u;
@@ -482,20 +489,24 @@ uint32_t ring_stages(size_t fixed, size_t row_bytes) {
     return static_cast<uint32_t>(n < kMaxRing ? n : kMaxRing);
 }
 
-template <int V>
-int launch_fwd_ring(const Fwd& p, uint32_t stages, size_t smem, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    const int st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(norm_ring_kernel<V>),
-                                                kRingBytes);
+// -1 where the rows are too long for a stage per group.
+template <int V, uint32_t THREADS, uint32_t GROUPS>
+int launch_fwd_ring(const Fwd& p, cudaStream_t stream) {
+    auto* kernel = norm_ring_kernel<V, THREADS, GROUPS>;
+    const size_t vec = static_cast<size_t>(p.cols) * 2, fixed = vec * (p.y ? 3 : 1);
+    const size_t row = vec * (1 + (p.y ? 1 : 0) + (p.gate && p.gate_stride ? 1 : 0));
+    const uint32_t stages = ring_stages(fixed, row);
+    if (stages < GROUPS) return -1;
+    const int st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes);
     if (st) return st;
     uint32_t* err = ptxstd::device_error_word();
     if (!err) return PTXSTD_ECUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
     const uint32_t sms = static_cast<uint32_t>(ptxstd::sm_count());
-    ptxstd::set_pdl(cfg, attr, p.rows < sms ? p.rows : sms, kGroupThreads * kGroups, stream);
-    cfg.dynamicSmemBytes = smem;
-    if (cudaLaunchKernelEx(&cfg, norm_ring_kernel<V>, p, stages, err) != cudaSuccess)
-        return PTXSTD_ECUDA;
+    ptxstd::set_pdl(cfg, attr, p.rows < sms ? p.rows : sms, THREADS * GROUPS, stream);
+    cfg.dynamicSmemBytes = fixed + stages * row;
+    if (cudaLaunchKernelEx(&cfg, kernel, p, stages, err) != cudaSuccess) return PTXSTD_ECUDA;
     return ptxstd::launch_status();
 }
 
@@ -933,25 +944,25 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
     if (nv <= 32) return launch_fwd<1, true>(p, 32, s);
     if (nv <= 64) return launch_fwd<2, true>(p, 32, s);
     if (nv <= 128) return launch_fwd<4, true>(p, 32, s);
-    // Many rows: the ring. 8192 x 8192 with everything on, E4M3 out: 80 us against 99 us for the
-    // row-per-block kernel below; with fewer rows than the GPU holds groups the latter starts
-    // sooner.
-    if (rows >= 4 * ptxstd::sm_count() && nv <= 4 * kGroupThreads) {
-        const bool per_row = d_gate && p.gate_stride;
-        const size_t vec = static_cast<size_t>(cols) * 2;
-        const size_t fixed = vec * (d_y ? 3 : 1);
-        const size_t row_bytes = vec * (1 + (d_y ? 1 : 0) + (per_row ? 1 : 0));
-        const uint32_t stages = ring_stages(fixed, row_bytes);
-        if (stages >= kGroups) {
-            const size_t smem = fixed + stages * row_bytes;
-            if (nv <= kGroupThreads) return launch_fwd_ring<1>(p, stages, smem, s);
-            if (nv <= 2 * kGroupThreads) return launch_fwd_ring<2>(p, stages, smem, s);
-            return launch_fwd_ring<4>(p, stages, smem, s);
-        }
+    // The ring pays where a row has two exchanges and there is enough to stream: with w_post,
+    // gate, E4M3 out, 8192 x 8192 takes 80 us against 95 us for a row per block, 8192 x 4096 43
+    // against 48 us, 8192 x 2048 28 against 31 us. Without w_post a row per block is at the copy
+    // rate already (8192 x 8192 in bf16: 80 us, the ring 92 us), and so it is the faster one for
+    // fewer elements (2400 x 4096: 17.9 against 18.6 us) and for rows that leave much of the long
+    // rows' groups idle (3000 x 5152: 28.3 against 29.5 us).
+    if (d_w_post && rows * cols >= 12'000'000) {
+        int st = -1;
+        if (nv <= 256) st = launch_fwd_ring<2, 128, 6>(p, s);
+        else if (nv <= 512) st = launch_fwd_ring<4, 128, 6>(p, s);
+        else if (nv > 768 && nv <= 1024) st = launch_fwd_ring<4, 256, 3>(p, s);
+        if (st >= 0) return st;
     }
-    // One row per block: one vector per thread while the block can be that large (a row's latency
-    // counts when there are few), else as many as the row needs.
-    const int v = nv > 2048 ? 4 : nv > 1024 ? 2 : 1;
+    // A row per block: one vector per thread while a block can be that large and a row's latency
+    // counts (100 x 4096: 3.4 us, 3.8 us with two); two once an SM has several rows, so that more
+    // blocks fit (300 x 8192 6.2 against 7.6 us, 1200 x 4096 8.8 against 10.4 us), but for a gate
+    // per row, whose third stream keeps enough loads in flight (1037 x 5152 10.2 against 11.1 us).
+    const bool few = rows <= ptxstd::sm_count() || (d_gate && p.gate_stride);
+    const int v = nv > 2048 ? 4 : nv > 1024 || (nv > 256 && !few) ? 2 : 1;
     const uint32_t threads = ((nv + v - 1) / v + 31) / 32 * 32;
     if (v == 1) return launch_fwd<1, false>(p, threads, s);
     if (v == 2) return launch_fwd<2, false>(p, threads, s);

@@ -357,7 +357,8 @@ def test_norm_forward(cuda, rows, cols, post, gate):
             R.check_mx(*n, ref, CHAIN * ref.abs(), fmt, padded=layout == 1, what="n")
 
 
-@pytest.mark.parametrize("rows,cols", [(592, 1056), (1037, 5152), (1500, 2048), (700, 8192)])
+@pytest.mark.parametrize("rows,cols", [(592, 1056), (1037, 5152), (1500, 2048), (3000, 4096 + 32),
+                                       (1600, 8192), (12000, 1056), (3100, 4064)])
 @pytest.mark.parametrize("post,gate", [(True, "vector"), (True, "row"), (False, "row"),
                                        (False, "none")])
 def test_norm_forward_many_rows(cuda, rows, cols, post, gate):
