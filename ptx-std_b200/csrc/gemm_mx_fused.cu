@@ -1099,16 +1099,53 @@ bool narrow_ring(NarrowPlan& p, uint32_t G, uint32_t tokens, bool two) {
     return p.smem >= part;
 }
 
-// The plan with the least estimated time. The model, fitted to sweeps of both choices over
-// 1 <= M <= 1000 on a B200 (within 15 % of the measured times at 8 to 40 us): an SM takes in about
-// 95 GB/s, a CTA's start and end cost 1.5 us that CTAs sharing an SM overlap, the exchange of
-// partial sums 1 us and 30 GB/s; a launch 2.5 us. At M = 200, N = 4128, K = 2080 it takes 64-token
-// tiles without a split: 8.2 us, against 10.5 us for one 208-token tile split in two and 9.8 us
-// for the wide kernel.
-NarrowPlan narrow_plan(int64_t M, int64_t N, int64_t K, bool gated) {
-    const uint32_t G = gated ? 2 : 1, cap = gated ? 128 : 256;
+// CTAs of a narrow launch that the GPU holds at once with one per SM, in clusters of `split`: asked
+// of the runtime once per device and kind (clusters of more than two leave SMs of their processing
+// clusters unused, how many depends on the part). 0 where a cluster does not fit.
+template <bool GATED>
+int64_t narrow_slots(uint32_t split) {
+    static std::atomic<int> cache[64][9];  // value + 1
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    std::atomic<int>& c = cache[dev][split];
+    int n = c.load(std::memory_order_relaxed);
+    if (n == 0) {
+        const void* kernel = reinterpret_cast<const void*>(narrow::narrow_kernel<GATED>);
+        if (ptxstd::set_max_dynamic_smem(kernel, kFullSmem + 1024) != PTXSTD_OK) return 0;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = split;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(split);
+        cfg.blockDim = dim3(narrow::kThreads);
+        cfg.dynamicSmemBytes = kFullSmem + 1024;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            clusters = 0;
+        }
+        n = clusters * static_cast<int>(split) + 1;
+        c.store(n, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
+
+// The plan with the least estimated time, in us. The model was fitted to sweeps of tokens, split
+// and CTAs per SM over 1 <= M <= 1000 on a B200 and is mostly within 15 % of the times there (5 to
+// 40 us): a launch 2.5; a CTA's start and end 1.5, which CTAs sharing an SM overlap; an SM takes
+// in its ring's bytes every 2.1 us, at most 95 GB/s; the partial sums' exchange 1.0 and 30 GB/s,
+// half as much again with two accumulators; and all of it no faster than HBM delivers. At M = 200,
+// N = 4128, K = 2080 it takes 64-token tiles without a split: 8.2 us, against 10.5 us for one
+// 208-token tile split in two and 9.8 us for the wide kernel.
+template <bool GATED>
+NarrowPlan narrow_plan(int64_t M, int64_t N, int64_t K) {
+    const uint32_t G = GATED ? 2 : 1, cap = GATED ? 128 : 256;
     const int64_t blocks = (N + 127) / 128, num_k = (K + BK - 1) / BK;
-    const int64_t sms = ptxstd::sm_count();
+    const double hbm = 2.5 + static_cast<double>(G) * N * K * (33.0 / 32.0) / 6.4e6;
     NarrowPlan best = {};
     best.us = 1e30;
     const int64_t whole = (M + 15) / 16 * 16;
@@ -1123,15 +1160,22 @@ NarrowPlan narrow_plan(int64_t M, int64_t N, int64_t K, bool gated) {
             for (const uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u}) {
                 if (s > 1 && num_k < 2 * s) break;
                 const int64_t ctas = blocks * ytiles * s;
-                // clusters of more than two leave SMs of a processing cluster unused
-                const int64_t slots = (s > 2 ? sms * 9 / 10 : sms) / s * s * (two ? 2 : 1);
+                const int64_t slots = narrow_slots<GATED>(s) * (two ? 2 : 1);
+                if (slots == 0) continue;
                 const int64_t waves = (ctas + slots - 1) / slots;
                 // CTAs that share an SM share its intake
-                const double sharing = two ? (ctas > sms ? 2.0 : 1.5) : 1.0;
-                const double intake =
-                    sharing * static_cast<double>((num_k + s - 1) / s) * stage / 95e3;
-                const double exchange = s > 1 ? 1.0 + t * G * 512.0 * (s - 1) / s / 30e3 : 0.0;
-                const double us = 2.5 + waves * ((two && waves > 1 ? 0.75 : 1.5) + intake + exchange);
+                const bool shared = two && ctas > slots / 2;
+                const double in_flight = (shared ? 2.0 : 1.0) * (p.stages - 0.5) * stage;
+                const double rate = in_flight / 2.1 < 95e3 ? in_flight / 2.1 : 95e3;
+                const double intake = (shared ? 2.0 : two ? 1.3 : 1.0) *
+                                      static_cast<double>((num_k + s - 1) / s) * stage / rate;
+                double exchange = s > 1 ? 1.0 + t * G * 512.0 * (s - 1) / s / 30e3 : 0.0;
+                if (GATED) exchange = exchange * 1.5 + 0.25 * (s - 1);
+                double us = 2.5 + waves * ((two && waves > 1 ? 0.75 : 1.5) + intake + exchange);
+                // bound by HBM, two CTAs per SM keep it busier over their ends (8192 x 28672 for
+                // one token: 38.5 us, 39.9 us with one)
+                const double floor = two ? hbm : 1.04 * hbm;
+                if (us < floor) us = floor + 0.02 * us;
                 if (us < best.us) {
                     best = p;
                     best.split = s;
@@ -1209,7 +1253,7 @@ template <bool GATED>
 int dispatch(Operand a, int a_type, Operand b, Operand b2, int b_type, const Epi& e, int64_t M,
              int64_t N, int64_t K, cudaStream_t stream) {
     if (M <= kNarrowRows) {
-        const NarrowPlan plan = narrow_plan(M, N, K, GATED);
+        const NarrowPlan plan = narrow_plan<GATED>(M, N, K);
         if (plan.us < 0.95 * wide_us(M, N, K, GATED))
             return launch_narrow<GATED>(plan, a, a_type, b, b2, b_type, e, M, N, K, stream);
     }
