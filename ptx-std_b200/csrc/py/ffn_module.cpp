@@ -11,10 +11,13 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
+#include <optional>
+#include <string>
 
 #include "ptxstd.h"
 
@@ -106,6 +109,7 @@ Mx operand(PyObject* q, PyObject* sf, const char* name, int64_t cols = -1) {
 struct Call {
     int device = -1;
     ptxstd_stream stream = nullptr;
+    std::optional<c10::cuda::CUDAStreamGuard> guard;
 
     template <class T>
     T* in(const at::Tensor* t) {
@@ -122,10 +126,13 @@ struct Call {
         if (!t->is_contiguous()) raise(PyExc_ValueError, "expected a contiguous tensor");
         return static_cast<T*>(t->data_ptr());
     }
-    // A torch.cuda.Stream, or None for the current stream; after the inputs.
+    // A torch.cuda.Stream, or None for the current stream; after the inputs. A stream that is given
+    // is the current one until the call returns, so that the allocator keeps what is allocated
+    // here (results, and workspaces that are dropped before the kernels end) in its order.
     void set_stream(PyObject* s) {
+        const auto dev = static_cast<c10::DeviceIndex>(device);
         if (s == Py_None) {
-            stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
+            stream = c10::cuda::getCurrentCUDAStream(dev).stream();
             return;
         }
         PyObject* h = PyObject_GetAttrString(s, "cuda_stream");
@@ -133,6 +140,7 @@ struct Call {
         stream = PyLong_AsVoidPtr(h);
         Py_DECREF(h);
         if (PyErr_Occurred()) throw PythonError();
+        guard.emplace(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream), dev));
     }
     at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) const {
         return at::detail::empty_cuda(

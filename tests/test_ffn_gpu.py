@@ -664,6 +664,32 @@ def test_two_streams_at_once(cuda):
             assert torch.equal(p, q)
 
 
+def test_stream_argument(cuda):
+    """Calls on a stream that is not the current one: right results, with the caller's own work on
+    the current stream reusing freed memory meanwhile."""
+    import ptxstd
+    rows, cols = 2000, 4096
+    g, xo, y, w, wp, gt = _norm_inputs(rows, cols, True, "vector")
+    dn = _bf(g, rows, cols)
+    rx = torch.rsqrt(xo.double().square().mean(1) + 1e-6).float()
+    ry = torch.rsqrt(y.double().square().mean(1) + 1e-6).float()
+    args = dict(y=y, w_post=wp, gate=gt, scale=0.5)
+    want = ptxstd.rmsnorm_residual_backward(dn, xo, w, (rx, ry), **args)
+    want_db = ptxstd.act_backward_mx(dn, xo, act="gelu", bias_grad=True)[2]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(10):
+        got = ptxstd.rmsnorm_residual_backward(dn, xo, w, (rx, ry), stream=s, **args)
+        db = ptxstd.act_backward_mx(dn, xo, act="gelu", bias_grad=True, stream=s)[2]
+        for _ in range(4):  # takes any block the calls gave back to the current stream
+            torch.full((8 << 20,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for p, q in zip(want, got):
+            assert torch.equal(p, q)
+        assert torch.equal(db, want_db)
+    _ok()
+
+
 def test_device_refusals(cuda):
     import ptxstd
     x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
