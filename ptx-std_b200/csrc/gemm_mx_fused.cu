@@ -18,13 +18,23 @@
 //    Ragged sizes: TMA fills rows and K elements outside the tensors with zeros and clips the
 //    stores; MMAs of a last K stage whose 32 elements lie outside are not issued, so padding
 //    scales (which may be NaN codes) never meet a product that is kept.
+//    Bound by the tensor cores: a stage takes 505 clocks (clock64 traces), where 256 x 256 x 128 at
+//    the nominal rate takes 512; between two tiles the MMAs pause for about 400 clocks, and the
+//    1 kW power cap sets the clock. 8192^3: 361 us, 3.05 PFLOP/s, 0.93 of twice the measured bf16
+//    burst. The epilogue runs beside the next tile's MMAs and shows only when K is short:
+//    4096 x 4096 x 1024 takes 19.1 us plain, 26.6 us with a residual, 33 us with bias, GELU and
+//    an E4M3 result.
 //
 // 2. narrow_kernel, for few rows (serving): weight streaming, bound by HBM. The operands swap: 128
 //    weight rows are the M side of a cta_group::1 MMA and the tokens (up to 256, a multiple of 16)
 //    the N side, so a token costs one accumulator column instead of a padded row. K is split
 //    over a cluster; the CTAs' partial accumulators meet in distributed shared memory and are
 //    added in rank order, each CTA finishing every S-th token, so the split needs no workspace,
-//    no atomics and no second kernel, and the result is reproducible.
+//    no atomics and no second kernel, and the result is reproducible. One token: N = 8192,
+//    K = 28672 with residual 38.7 us, 6.25 TB/s or 0.95 of the measured copy rate; gated
+//    F = 28672, K = 8192 78.7 us, 0.94 of it. With tens of tokens and mid-sized weights the CTAs'
+//    start and end (about 4 us) and an uneven number of blocks per SM cost more: 48 tokens,
+//    F = 10240, K = 4096 21.0 us against 13.4 us of HBM time.
 //
 // Every device-side wait is bounded; a timeout records PTXSTD_ETIMEOUT.
 #include <atomic>

@@ -22,7 +22,10 @@
 // them in f32; the partial sums go through a workspace and are added in order by a second kernel
 // (reproducible, no atomics), which applies the factors.
 //
-// Both directions are near the issue rate as well as the HBM rate, hence the packed f32 pairs.
+// Both directions are near the issue rate as well as the HBM rate (67 % and 60 % of the issue
+// slots, ncu), hence the packed f32 pairs. Forward, 8192 x 8192 with w_post, gate and E4M3 out:
+// 472 MB in 80 us, 5.9 TB/s or 0.90 of the measured copy rate; without w_post in bf16 537 MB in
+// 80 us, 1.02 of it; one row of 8192: 3.5 us. Backward, 8192 x 4096: 403 MB in 67.8 us, 0.91.
 #include "common.cuh"
 #include "data_types.cuh"
 #include "mx_block.cuh"
