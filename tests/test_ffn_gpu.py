@@ -299,6 +299,52 @@ def test_quantize_transposed(cuda, rows, cols, fmt):
         assert torch.equal(q, qt) and torch.equal(sf, sft)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_quantisers_agree_on_special_values(cuda, fmt):
+    """NaN, infinities, subnormals, zeros, saturation: the transposing quantiser and the norm's and
+    the GEMM's block quantiser give the codes of quantize_mx."""
+    import ptxstd
+    x = _bf(_gen(4), 128, 64, std=3.0)
+    x[0, 0], x[33, 1], x[40, 2] = math.nan, math.inf, -math.inf
+    x[:32, 3] = 0
+    x[:32, 4] = torch.arange(32, device="cuda").to(torch.bfloat16) * 2.0 ** -130
+    x[:32, 5] = torch.linspace(400, 500, 32, device="cuda").to(torch.bfloat16)
+    x[:32, 6] = 3.3e38
+    x[:32, 7] = 2.0 ** -126
+    x[:32, 8] = -0.0
+    qt, sft = ptxstd.quantize_mx_t(x, fmt)
+    q, sf = ptxstd.quantize_mx(x.t().contiguous(), fmt, sf_layout=2)
+    _ok()
+    assert torch.equal(sft, sf) and torch.equal(qt, q)
+    # D = dh exactly (no activation): rows quantised from registers
+    (r, rsf), (c, csf) = ptxstd.act_backward_mx(x, torch.zeros_like(x), act="none", elem_type=fmt)
+    q, sf = ptxstd.quantize_mx(x, fmt, sf_layout=2)
+    _ok()
+    assert torch.equal(rsf, sf) and torch.equal(r, q)
+    assert torch.equal(csf, sft) and torch.equal(c, qt)
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_gated_element_types(cuda, M):
+    """FP6 and FP4 weights: equal to the products of the linear kernel with the same operands."""
+    import ptxstd
+    F, K = 96, 160
+    g = _gen(M)
+    a, sfa = _mx(g, M, K, "e5m2")
+    for wt in ("e2m3", "e2m1"):
+        wg, sfg = _mx(g, F, K, wt)
+        wu, sfu = _mx(g, F, K, wt)
+        h, (gate, up) = ptxstd.gemm_mx_gated(a, "e5m2", sfa, wg, sfg, wu, sfu, wt, act="none",
+                                             save=True)
+        lg = ptxstd.gemm_mx_epilogue(a, "e5m2", sfa, wg, wt, sfg)
+        lu = ptxstd.gemm_mx_epilogue(a, "e5m2", sfa, wu, wt, sfu)
+        _ok()
+        # both accumulate the same products in f32; the tilings may differ, so one bf16 step
+        for p, q in ((gate, lg), (up, lu)):
+            assert ((p.double() - q.double()).abs() <= 2.0 ** -7 * q.double().abs() + 1e-30).all()
+        R.check_bf16(h, gate.double() * up.double(), 2.0 ** -7 * (gate.double() * up.double()).abs())
+
+
 def test_activation_extremes(cuda):
     """Saturated, tiny and infinite pre-activations: no NaN where the limit is finite."""
     import ptxstd
@@ -664,6 +710,85 @@ def test_two_streams_at_once(cuda):
             assert torch.equal(p, q)
 
 
+# ---- offsets past 32 bits -------------------------------------------------------------------------
+def _tiled(block, rows):
+    """`block` repeated over `rows` rows (contiguous)."""
+    reps = -(-rows // block.shape[0])
+    return block.repeat(reps, 1)[:rows].contiguous()
+
+
+def test_norm_offsets_past_32_bits(cuda):
+    """2.2e9 elements: the last rows (byte and element offsets past 2^32 and 2^31) against the
+    restatement, the column sums against those of the repeated block."""
+    import ptxstd
+    period, reps, cols = 1024, 262, 8192
+    rows = period * reps
+    assert rows * cols > 1 << 31
+    g = _gen(1)
+    xb, yb, dnb = (_bf(g, period, cols, std=s) for s in (2.0, 0.7, 0.3))
+    w, wp, gt = (_bf(g, cols) for _ in range(3))
+    x, y = _tiled(xb, rows), _tiled(yb, rows)
+    xo, (q, sf), st = ptxstd.rmsnorm_residual(x, w, y=y, w_post=wp, gate=gt, scale=0.5,
+                                              elem_type="e4m3")
+    _ok()
+    tail = slice(rows - 256, rows)
+    ref, mag, _ = R.norm_forward(_d(x[tail]), _d(y[tail]), _d(wp), _d(gt), 0.5, 1e-6)
+    R.check_bf16(xo[tail], ref, CHAIN * mag, "x'")
+    ref, _ = R.norm_result(_d(xo[tail]), _d(w), 1e-6)
+    R.check_mx(q[tail], sf[-2 * 64 * 512:], ref, CHAIN * ref.abs(), "e4m3", what="n")
+    del q, sf, x
+    dn = _tiled(dnb, rows)
+    dx, dw, dy, dwp, dg = ptxstd.rmsnorm_residual_backward(dn, xo, w, st, y=y, w_post=wp, gate=gt,
+                                                           scale=0.5)
+    _ok()
+    ref = R.norm_backward(_d(dn[tail]), None, _d(xo[tail]), _d(w), _d(st[0][tail]), _d(y[tail]),
+                          _d(wp), _d(st[1][tail]), _d(gt), 0.5)
+    R.check_bf16(dx[tail], ref["dx"][0], CHAIN * ref["dx"][1], "dx")
+    R.check_bf16(dy[tail], ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
+    one = R.norm_backward(_d(dnb), None, _d(xo[:period]), _d(w), _d(st[0][:period]), _d(yb), _d(wp),
+                          _d(st[1][:period]), _d(gt), 0.5)
+    terms = CHAIN + (rows / 148 + 200) * 2.0 ** -24
+    for name, got in (("dw", dw), ("dw_post", dwp), ("dgate", dg)):
+        want, mag = one[name][0] * reps, one[name][1] * reps
+        assert ((got.double() - want).abs() <= 4 * terms * mag).all(), name
+
+
+def test_act_backward_offsets_past_32_bits(cuda):
+    """The last 128 rows of 2.2e9 elements equal a call on those rows alone, bit for bit, in both
+    operands (tiles do not depend on one another)."""
+    import ptxstd
+    cols, rows = 16384, 128 * 1056
+    assert rows * cols > 1 << 31
+    g = _gen(2)
+    dh, gate = _tiled(_bf(g, 640, cols, std=0.1), rows), _tiled(_bf(g, 896, cols, std=2.0), rows)
+    (q, sf), (qt, sft) = ptxstd.act_backward_mx(dh, gate, act="silu", elem_type="e4m3")
+    a, b = dh[-128:].contiguous(), gate[-128:].contiguous()
+    (q1, sf1), (qt1, sft1) = ptxstd.act_backward_mx(a, b, act="silu", elem_type="e4m3")
+    _ok()
+    assert torch.equal(q[-128:], q1) and torch.equal(qt[:, -128:], qt1)
+    assert torch.equal(sf[-sf1.numel():], sf1)
+    # the transposed scales: the last of each row tile's 512-byte tiles
+    assert torch.equal(sft.view(cols // 128, -1, 512)[:, -1], sft1.view(cols // 128, 512))
+
+
+def test_linear_offsets_past_32_bits(cuda):
+    """A result of 2.2e9 elements with a residual: its first and last rows."""
+    import ptxstd
+    M, N, K = 270336, 8192, 64
+    assert M * N > 1 << 31
+    g = _gen(3)
+    a, sfa = _mx(g, M, K)
+    b, sfb = _mx(g, N, K, std=K ** -0.5)
+    res = _tiled(_bf(g, 1024, N), M)
+    c = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb, residual=res)
+    _ok()
+    bv = R.dequant(b, sfb, "e4m3")
+    for rows, tiles in ((slice(0, 256), slice(0, 2 * 512)), (slice(M - 256, M), slice(-2 * 512, None))):
+        ref, mag = R.gemm(R.dequant(a[rows], sfa[tiles], "e4m3"), bv)
+        r = _d(res[rows])
+        R.check_bf16(c[rows], ref + r, R.acc_bound(mag, K) + CHAIN * (ref.abs() + r.abs()), "c")
+
+
 def test_stream_argument(cuda):
     """Calls on a stream that is not the current one: right results, with the caller's own work on
     the current stream reusing freed memory meanwhile."""
@@ -688,6 +813,33 @@ def test_stream_argument(cuda):
             assert torch.equal(p, q)
         assert torch.equal(db, want_db)
     _ok()
+
+
+def test_beside_the_other_gemms(cuda):
+    """The operators on one stream while the framework's other tensor-core kernels, which take all
+    of an SM's TMEM, run on another: everything finishes with the results it has alone."""
+    import ptxstd
+    b1, b2 = Block(7, 512, 1024, seed=11), Block(400, 512, 1024, seed=12)
+    want = [[t.clone() for t in _flat(b.forward())] for b in (b1, b2)]
+    g = _gen(5)
+    a, sfa = ptxstd.quantize_mx(_bf(g, 512, 1024), "e4m3", sf_layout=1)
+    x = _bf(g, 16, 2048)
+    w4, sf4 = ptxstd.quantize_nvfp4(_bf(g, 1024, 2048, std=0.02), 0.02 / 448, sf_layout=1)
+    c0 = ptxstd.gemm_mx(a, "e4m3", sfa, a, "e4m3", sfa).clone()
+    y0 = ptxstd.gemm_decode(x, w4, sf4, 0.02 / 448).clone()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            got = [_flat(b.forward()) for b in (b1, b2)]
+        with torch.cuda.stream(s2):
+            c = ptxstd.gemm_mx(a, "e4m3", sfa, a, "e4m3", sfa)
+            y = ptxstd.gemm_decode(x, w4, sf4, 0.02 / 448)
+    _ok()
+    assert torch.equal(c, c0) and torch.equal(y, y0)
+    for p, q in zip(want, got):
+        for u, v in zip(p, q):
+            assert torch.equal(u, v)
 
 
 def test_device_refusals(cuda):
