@@ -9,13 +9,15 @@
 // bf16 before its norm is taken, because the stored value is what every later reader (the next
 // block, the backward pass) sees; n is quantised from f32 without a bf16 step between.
 //
-// Backward: with a = dn w,
-//   dx = du + rx a - x' rx^3 mean(a x'),   dw = sum_rows dn x' rx,
+// Backward: with a = dn w, the normalised rows h = x' rx and k = y ry, and their means
+// m1 = mean(a h), m2 = mean(b k),
+//   dx = du + rx (a - h m1),                 dw = sum_rows dn h,
 //   dg = scale p dx,  dp = scale g dx,  b = dp w_post,
-//   dy = ry b - y ry^3 mean(b y),          dw_post = sum_rows dp y ry.
-// mean(b y) needs dx, hence mean(a x'). Substituting dx gives, with t = scale g w_post y,
-//   sum(b y) = sum(t du) + rx sum(t a) - (rx^3 mean(a x')) sum(t x'),
-// so one exchange of four sums serves both means. With one gate for all rows both dg and dw_post
+//   dy = ry (b - k m2),                      dw_post = sum_rows dp k.
+// m2 needs dx, hence m1. Substituting dx gives, with t = scale g w_post y,
+//   m2 = ry mean(t dx) = ry (sum(t du) + rx (sum(t a) - m1 rx sum(t x'))) / D,  m1 = rx sum(a x') / D,
+// so one exchange of four sums serves both means. (No power of rx or ry stands alone: rx^3 leaves
+// f32's range for rows around 1e13 or 1e-13, where the norms themselves are still exact.) With one gate for all rows both dg and dw_post
 // are column factors times the same sum, S = sum_rows dx y ry: dg = scale w_post S,
 // dw_post = scale g S; with a gate per row dg needs no sum and S takes g inside. So there are two
 // column sums at most. Each thread keeps its columns for all rows of its group and accumulates
@@ -569,15 +571,15 @@ __device__ __forceinline__ void sums8(Sums& s, const uint4& dnv, const uint4& du
 
 // The factors of a row in the gradients, from its sums and statistics.
 struct RowFactors {
-    float rx, ry, k1, k2;
+    float rx, ry, m1, m2;
 };
 __device__ __forceinline__ RowFactors row_factors(const float4& s, float rx, float ry,
                                                   float inv_d) {
     RowFactors f;
     f.rx = rx;
     f.ry = ry;
-    f.k1 = rx * rx * rx * (s.x * inv_d);
-    f.k2 = ry * ry * ry * ((s.y + rx * s.z - f.k1 * s.w) * inv_d);
+    f.m1 = rx * s.x * inv_d;
+    f.m2 = ry * (s.y + rx * (s.z - f.m1 * (rx * s.w))) * inv_d;
     return f;
 }
 
@@ -589,18 +591,19 @@ __device__ __forceinline__ void grads8(const Bwd& p, const RowFactors& r, const 
                                        Oct& S) {
     const Oct dn = widen(dnv), x = widen(xv);
     Oct dx = widen(duv);
-    const f32x2 rx = pack2f(r.rx, r.rx), k1 = pack2f(-r.k1, -r.k1);
+    const f32x2 rx = pack2f(r.rx, r.rx), m1 = pack2f(-r.m1, -r.m1);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        dw.v[k] = fma2(mul2(x.v[k], rx), dn.v[k], dw.v[k]);
-        dx.v[k] = fma2(rx, mul2(dn.v[k], f.w.v[k]), dx.v[k]);
-        dx.v[k] = fma2(x.v[k], k1, dx.v[k]);
+        const f32x2 xh = mul2(x.v[k], rx);
+        dw.v[k] = fma2(xh, dn.v[k], dw.v[k]);
+        dx.v[k] = fma2(rx, fma2(xh, m1, mul2(dn.v[k], f.w.v[k])), dx.v[k]);
     }
     *reinterpret_cast<uint4*>(p.dx + at) = narrow(dx);
     if (!p.y) return;
-    const Oct y = widen(yv);
-    const f32x2 ry = pack2f(r.ry, r.ry), k2 = pack2f(-r.k2, -r.k2);
-    Oct b;
+    Oct y = widen(yv), b;
+    const f32x2 ry = pack2f(r.ry, r.ry), m2 = pack2f(-r.m2, -r.m2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y.v[k] = mul2(y.v[k], ry);
 #pragma unroll
     for (int k = 0; k < 4; ++k) b.v[k] = mul2(dx.v[k], f.c.v[k]);
     if (gate) {
@@ -608,18 +611,17 @@ __device__ __forceinline__ void grads8(const Bwd& p, const RowFactors& r, const 
         Oct dg;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const f32x2 yh = mul2(y.v[k], ry);
-            dg.v[k] = mul2(b.v[k], yh);
-            S.v[k] = fma2(mul2(dx.v[k], g.v[k]), yh, S.v[k]);
+            dg.v[k] = mul2(b.v[k], y.v[k]);
+            S.v[k] = fma2(mul2(dx.v[k], g.v[k]), y.v[k], S.v[k]);
             b.v[k] = mul2(b.v[k], g.v[k]);
         }
         *reinterpret_cast<uint4*>(p.dgate_rows + at) = narrow(dg);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) S.v[k] = fma2(dx.v[k], mul2(y.v[k], ry), S.v[k]);
+        for (int k = 0; k < 4; ++k) S.v[k] = fma2(dx.v[k], y.v[k], S.v[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) b.v[k] = fma2(ry, b.v[k], mul2(y.v[k], k2));
+    for (int k = 0; k < 4; ++k) b.v[k] = mul2(ry, fma2(y.v[k], m2, b.v[k]));
     *reinterpret_cast<uint4*>(p.dy + at) = narrow(b);
 }
 

@@ -247,6 +247,29 @@ def test_gated_features_of_eight(cuda, M):
     _gated_case(M, 200, 96, save=True)
 
 
+@pytest.mark.parametrize("M", [5, 300])
+def test_gated_both_results(cuda, M):
+    """d_h and d_q of one call, with the projections beside them (C ABI): as the separate calls."""
+    import ptxstd
+    F, K = 160, 224
+    g = _gen(M)
+    a, sfa = _mx(g, M, K)
+    wg, sfg = _mx(g, F, K, std=K ** -0.5)
+    wu, sfu = _mx(g, F, K, std=K ** -0.5)
+    ops = (a, "e4m3", sfa, wg, sfg, wu, sfu, "e4m3")
+    h, (gate, up) = ptxstd.gemm_mx_gated(*ops, save=True)
+    q, sf = ptxstd.gemm_mx_gated(*ops, elem_type="e5m2")
+    got = [torch.empty_like(t) for t in (h, gate, up, q, sf)]
+    p = [t.data_ptr() for t in got]
+    assert ptxstd.lib().ptxstd_gemm_mx_gated(
+        a.data_ptr(), 0, sfa.data_ptr(), wg.data_ptr(), sfg.data_ptr(), wu.data_ptr(),
+        sfu.data_ptr(), 0, 2, p[0], p[1], p[2], 1, p[3], p[4], M, F, K,
+        torch.cuda.current_stream().cuda_stream) == 0
+    _ok()
+    for u, v in zip(got, (h, gate, up, q, sf)):
+        assert torch.equal(u, v)
+
+
 # ---- gradient of the activation, transposing quantiser ------------------------------------------
 def _t(v):
     rows, cols = v.shape
@@ -488,6 +511,46 @@ def test_norm_in_place(cuda):
     assert torch.equal(x, want[0]) and torch.equal(n, want[1])
 
 
+@pytest.mark.parametrize("rows,cols", [(3100, 4064), (1600, 8192), (500, 1056)])
+def test_norm_in_place_many_rows(cuda, rows, cols):
+    """x' over x, n in both forms at once (C ABI): as the separate calls give them."""
+    import ptxstd
+    _, x, y, w, wp, gt = _norm_inputs(rows, cols, True, "row")
+    args = dict(y=y, w_post=wp, gate=gt, scale=2.0)
+    xo, n, _ = ptxstd.rmsnorm_residual(x, w, **args)
+    (q, sf) = ptxstd.rmsnorm_residual(x, w, elem_type="e4m3", **args)[1]
+    n2, q2, sf2 = torch.empty_like(n), torch.empty_like(q), torch.empty_like(sf)
+    st = ptxstd.lib().ptxstd_rmsnorm_residual(
+        x.data_ptr(), y.data_ptr(), wp.data_ptr(), gt.data_ptr(), rows, 2.0, w.data_ptr(), 1e-6,
+        rows, cols, x.data_ptr(), n2.data_ptr(), 0, q2.data_ptr(), sf2.data_ptr(), 1, None, None,
+        torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    _ok()
+    for p, r in ((x, xo), (n2, n), (q2, q), (sf2, sf)):
+        assert torch.equal(p, r)
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 480), (700, 4096), (300, 8192), (5, 8192 + 32)])
+def test_norm_backward_in_place(cuda, rows, cols):
+    """dx may be written over dx_out (C ABI)."""
+    import ptxstd
+    g, xo, y, w, wp, gt = _norm_inputs(rows, cols, True, "vector")
+    dn, du = _bf(g, rows, cols), _bf(g, rows, cols)
+    _, _, st = ptxstd.rmsnorm_residual(xo, w, y=y, w_post=wp, gate=gt)
+    want = ptxstd.rmsnorm_residual_backward(dn, xo, w, st, dx_out=du, y=y, w_post=wp, gate=gt)
+    got = [du] + [torch.empty_like(t) for t in want[1:]]
+    L = ptxstd.lib()
+    nb = L.ptxstd_rmsnorm_residual_backward_workspace_bytes(rows, cols)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    ptr = [t.data_ptr() for t in (dn, du, xo, w, st[0], y, wp, st[1], gt)]
+    assert L.ptxstd_rmsnorm_residual_backward(
+        *ptr, 1, 1.0, rows, cols, *[t.data_ptr() for t in got], ws.data_ptr(), nb,
+        torch.cuda.current_stream().cuda_stream) == 0
+    _ok()
+    for p, r in zip(got, want):
+        assert torch.equal(p, r)
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 32), (2, 40), (5, 480), (300, 1056), (1200, 256),
                                        (9, 4096 + 32), (160, 8192), (5, 8192 + 32), (3, 16384)])
 @pytest.mark.parametrize("post,gate,du", [(False, "none", True), (True, "vector", True),
@@ -529,6 +592,39 @@ def test_norm_backward(cuda, rows, cols, post, gate, du):
         assert dg is None
     for p, q in zip((dx, dw, dy, dwp, dg), again):
         assert p is q is None or torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows,cols", [(70, 480), (330, 1056), (300, 8192), (3, 8192 + 32)])
+@pytest.mark.parametrize("px,py", [(50, 50), (-50, -50), (50, -50), (-50, 50), (0, 50), (-50, 0)])
+@pytest.mark.parametrize("gate", ["vector", "row"])
+def test_norm_backward_of_large_and_tiny_rows(cuda, rows, cols, px, py, gate):
+    """Rows around 2^50 and 2^-50, whose norms are exact in f32 and whose cubed factors are not
+    representable in it. The tolerances are those of test_norm_backward: powers of two change no
+    rounding, and every product of the formulas, with the factors next to their rows, stays between
+    2^-126 and 2^127 (at most |t x'| summed: 2^(100 + 13 + 10)). A sum's terms below the others by
+    more than 2^24 only lose what CHAIN allows of the magnitudes."""
+    import ptxstd
+    g, xo, y, w, wp, gt = _norm_inputs(rows, cols, True, gate)
+    xo, y = xo * 2.0 ** px, y * 2.0 ** py
+    dn, du = _bf(g, rows, cols, std=0.3), _bf(g, rows, cols, std=0.3)
+    rx = torch.rsqrt(xo.double().square().mean(1)).float()
+    ry = torch.rsqrt(y.double().square().mean(1)).float()
+    for dxo in (None, du):
+        dx, dw, dy, dwp, dg = ptxstd.rmsnorm_residual_backward(
+            dn, xo, w, (rx, ry), dx_out=dxo, y=y, w_post=wp, gate=gt, scale=0.5)
+        _ok()
+        ref = R.norm_backward(_d(dn), _d(dxo), _d(xo), _d(w), _d(rx), _d(y), _d(wp), _d(ry),
+                              _d(gt), 0.5)
+        R.check_bf16(dx, ref["dx"][0], CHAIN * ref["dx"][1], "dx")
+        R.check_bf16(dy, ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
+        terms = CHAIN + (rows / 148 + 200) * 2.0 ** -24
+        for name, got in (("dw", dw), ("dw_post", dwp)):
+            assert ((got.double() - ref[name][0]).abs() <= 4 * terms * ref[name][1]).all(), name
+        if gate == "row":
+            R.check_bf16(dg, ref["dgate"][0], 4 * CHAIN * ref["dgate"][1], "dgate")
+        else:
+            lim = 4 * terms * ref["dgate"][1]
+            assert ((dg.double() - ref["dgate"][0]).abs() <= lim).all()
 
 
 def test_norm_gradient_against_differences(cuda):
