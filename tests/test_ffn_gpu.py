@@ -885,6 +885,62 @@ def test_linear_offsets_past_32_bits(cuda):
         R.check_bf16(c[rows], ref + r, R.acc_bound(mag, K) + CHAIN * (ref.abs() + r.abs()), "c")
 
 
+def test_two_host_threads_at_once(cuda):
+    """Concurrent calls from two threads, each on a stream of its own."""
+    import threading
+    blocks = [Block(3, 512, 1024, seed=21), Block(300, 512, 1024, seed=22)]
+    want = [_flat((f, b.backward(*f))) for b in blocks for f in [b.forward()]]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    f = blocks[i].forward()
+                    got[i] = _flat((f, blocks[i].backward(*f)))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    _ok()
+    assert not errors
+    for p, q in zip(want, got):
+        assert len(p) == len(q) and all(torch.equal(u, v) for u, v in zip(p, q))
+
+
+def test_first_calls_are_captured(cuda):
+    """In a new process the first call of every operator may be one under graph capture."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import torch
+import test_ffn_gpu as T
+b = T.Block(300, 256, 512)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    f = b.forward()
+    r = T._flat((f, b.backward(*f)))
+g.replay()
+torch.cuda.synchronize()
+f = b.forward()
+e = T._flat((f, b.backward(*f)))
+T._ok()
+assert len(r) == len(e) and all(torch.equal(p, q) for p, q in zip(r, e))
+"""
+    r = subprocess.run([sys.executable, "-c", code] + sys.path, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_stream_argument(cuda):
     """Calls on a stream that is not the current one: right results, with the caller's own work on
     the current stream reusing freed memory meanwhile."""
