@@ -9,10 +9,18 @@
 // back by columns for the transposed operand. Loads are 128-byte row segments, all of a tile
 // issued before the first use; 8 lanes hold a row segment, so a row block of 32 is four lanes. In
 // the second step a thread holds one column's 32 rows, i.e. one whole block, and stores its 32
-// codes as two 16-byte vectors.
-// 4096 x 16384, E5M2, column sums included: 407 MB in 74 us with ReLU (0.84 of the measured copy
-// rate), 77 us with SiLU, 83 us with GELU, whose polynomial takes the issue slots to 75 % (ncu).
-// Gated, SiLU, 4096 x 10240: 425 MB in 92 us (0.70); the order of the tiles makes no difference.
+// codes in one instruction; the column's other 32 rows belong to the neighbouring lane, so that a
+// pair writes 64 adjacent bytes, its two scales as one half-word, and adds its sums by a shuffle.
+// (As two 16-byte stores, with a column's halves in different warps, the requests to L2 bound the
+// kernel: ReLU 82 us instead of 71 us, the transposing quantiser of 8192 x 8192 50 us instead of
+// 41 us, gated 99 us instead of 88 us.)
+// 4096 x 16384, E5M2, column sums included, results of successive calls in different buffers, under
+// load: 407 MB in 71 us with ReLU (0.88 of the measured copy rate), 89 us with GELU, which takes 30
+// instructions per element to ReLU's 20 and so the issue slots to three quarters (ncu); at the
+// clock of an idle GPU 67 and 80 us. Gated, SiLU, 4096 x 10240: 425 MB in 88 us (0.74). The
+// transposing quantiser of 8192 x 8192: 204 MB in 41 us (0.76). Without effect or slower: other
+// orders of the tiles, prefetching a later tile to L2, a persistent form that copies the next tile
+// to shared memory meanwhile (gated 81 us instead of 84 us, GELU 106 instead of 83).
 #include "common.cuh"
 #include "data_types.cuh"
 #include "mx_block.cuh"
@@ -34,6 +42,7 @@ struct Params {
     float* partial;  // [row tiles][W] column sums, or null
     uint32_t rows, cols, W, R;  // W columns of D, R = rows rounded up to 32
     uint32_t col_tiles, act, type;
+    bool wide;  // qt is 32-byte aligned
 };
 
 using ptxstd::f32x2;
@@ -41,16 +50,30 @@ using ptxstd::mul2;
 using ptxstd::Oct;
 using ptxstd::widen;
 
-// The tile in shared memory, [row][64] f32 as 16 slots of four columns. Slot s of a row sits at
-// s ^ (s / 8): then the eight lanes of a quarter-warp, which hold slots 0, 2, .. 14 (then 1, 3, ..
-// 15) of one row, store into different banks. A column keeps its place in every row, so reading
-// 32 neighbouring columns of a row is free of conflicts too.
-__device__ __forceinline__ uint32_t slot_of(uint32_t s) { return s ^ (s >> 3); }
+// The tile in shared memory, [row][64] f32 as 16 slots of four columns. Slot s of a row in block b
+// of 32 rows sits at s ^ (s / 8) ^ 4 b: then the eight lanes of a quarter-warp, which hold slots 0,
+// 2, .. 14 (then 1, 3, .. 15) of one row, store into different banks. A column keeps its place in
+// every row of a block, and a warp that reads 16 neighbouring columns in both blocks finds one
+// block's in the other half of the banks, so reading is free of conflicts too.
+__device__ __forceinline__ uint32_t slot_of(uint32_t s, uint32_t b) { return s ^ (s >> 3) ^ (4 * b); }
 
-// Eight values (lane l of a row's eight) to the tile.
-__device__ __forceinline__ void put8(float4* row, uint32_t l, const float (&v)[8]) {
-    row[slot_of(2 * l)] = make_float4(v[0], v[1], v[2], v[3]);
-    row[slot_of(2 * l + 1)] = make_float4(v[4], v[5], v[6], v[7]);
+// Eight values (lane l of a row's eight) to the tile; b: the row's block of 32.
+__device__ __forceinline__ void put8(float4* row, uint32_t l, uint32_t b, const float (&v)[8]) {
+    row[slot_of(2 * l, b)] = make_float4(v[0], v[1], v[2], v[3]);
+    row[slot_of(2 * l + 1, b)] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// 32 codes of one column.
+__device__ __forceinline__ void store32(uint8_t* dst, const uint2 (&c)[4], bool wide) {
+    if (wide)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+                     "r"(c[0].x), "r"(c[0].y), "r"(c[1].x), "r"(c[1].y), "r"(c[2].x), "r"(c[2].y),
+                     "r"(c[3].x), "r"(c[3].y)
+                     : "memory");
+    else {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(c[2].x, c[2].y, c[3].x, c[3].y);
+    }
 }
 
 // One row block (four lanes) of D: eight codes to q, the block's scale to sf (first lane).
@@ -62,15 +85,14 @@ __device__ __forceinline__ void row_block(uint32_t type, const float (&v)[8], bo
 }
 
 // Blocks per SM asked of the compiler: enough registers that all of a tile's loads are in flight at
-// once. Gated, SiLU, 4096 x 10240: 92 us with 5 (92 registers), 119 us without a bound (80
-// registers, loads in turn with their use), 101 us with tiles of 128 rows and 256 threads.
+// once. Gated, SiLU, 4096 x 10240: 84 us with 5 (93 registers), 110 us with 6 (80 registers, loads
+// in turn with their use). Ungated, GELU, 4096 x 16384: 81 us with 9, 83 us with 8, 88 us with 10.
 template <int MODE>
-__global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
+__global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 9)
     act_backward_kernel(const __grid_constant__ Params p) {
     constexpr int kTiles = MODE == kGated ? 2 : 1;
     extern __shared__ float4 smem_raw[];
     float4* const tile = smem_raw;  // [kTiles][kRows][kCols / 4]
-    __shared__ float sums[kRows / 32][kCols];
     const uint32_t tid = threadIdx.x, lane = ptxstd::lane_id(), warp = tid >> 5;
     const uint32_t ct = blockIdx.x % p.col_tiles, rt = blockIdx.x / p.col_tiles;
     const uint32_t row0 = rt * kRows, col0 = ct * kCols;
@@ -85,14 +107,19 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
         const bool col_on = col < p.cols;
         const size_t at = static_cast<size_t>(row) * p.cols + col, step = static_cast<size_t>(kPassRows) * p.cols;
         uint4 gv[kPasses], dv[kPasses], uv[kPasses];
+        auto load = [&](uint32_t i) {
+            gv[i] = *reinterpret_cast<const uint4*>(p.gate + at + i * step);
+            if (MODE != kTranspose) dv[i] = *reinterpret_cast<const uint4*>(p.dh + at + i * step);
+            if (MODE == kGated) uv[i] = *reinterpret_cast<const uint4*>(p.up + at + i * step);
+        };
+        if (row0 + kRows <= p.rows && col0 + kCols <= p.cols) {
 #pragma unroll
-        for (uint32_t i = 0; i < kPasses; ++i) {
-            gv[i] = dv[i] = uv[i] = make_uint4(0, 0, 0, 0);
-            if (row + kPassRows * i < p.rows && col_on) {
-                gv[i] = *reinterpret_cast<const uint4*>(p.gate + at + i * step);
-                if (MODE != kTranspose)
-                    dv[i] = *reinterpret_cast<const uint4*>(p.dh + at + i * step);
-                if (MODE == kGated) uv[i] = *reinterpret_cast<const uint4*>(p.up + at + i * step);
+            for (uint32_t i = 0; i < kPasses; ++i) load(i);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                gv[i] = dv[i] = uv[i] = make_uint4(0, 0, 0, 0);
+                if (row + kPassRows * i < p.rows && col_on) load(i);
             }
         }
         float4* const dst = tile + r * (kCols / 4);
@@ -101,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
             for (uint32_t i = 0; i < kPasses; ++i) {
                 float v[8];
                 ptxstd::flatten(widen(gv[i]), v);
-                put8(dst + i * kPassRows * (kCols / 4), l, v);
+                put8(dst + i * kPassRows * (kCols / 4), l, i * kPassRows / 32, v);
             }
         } else {
             const size_t k_tiles = mx::tiles_k(p.W / 32);
@@ -135,12 +162,12 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
                     }
                     float v[8];
                     ptxstd::flatten(b, v);
-                    put8(dst + i * kPassRows * (kCols / 4), l, v);
+                    put8(dst + i * kPassRows * (kCols / 4), l, i * kPassRows / 32, v);
                     row_block(p.type, v, on, q + i * static_cast<size_t>(kPassRows) * p.W, first,
                               sf0 + at_sf);
                     if constexpr (MODE == kGated) {
                         ptxstd::flatten(a, v);
-                        put8(dst + (kRows + i * kPassRows) * (kCols / 4), l, v);
+                        put8(dst + (kRows + i * kPassRows) * (kCols / 4), l, i * kPassRows / 32, v);
                         row_block(p.type, v, on, q + i * static_cast<size_t>(kPassRows) * p.W + p.cols,
                                   first, sf1 + at_sf);
                     }
@@ -150,12 +177,14 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
     }
     __syncthreads();
 
-    // transposed: thread = (column f, row block b)
-    const uint32_t f = tid & (kCols - 1), b = tid / kCols;
+    // transposed: thread = (column f, row block b), the two blocks of a column in neighbouring lanes
+    const uint32_t f = tid >> 1, b = tid & 1u;
     const uint32_t t0 = row0 + 32 * b;
     const size_t kt = mx::tiles_k(p.R / 32);
     const uint32_t emax = mx::emax_of(p.type);
-    const float* const column = reinterpret_cast<const float*>(tile) + 4 * slot_of(f >> 2) + (f & 3u);
+    const float* const column =
+        reinterpret_cast<const float*>(tile) + 4 * slot_of(f >> 2, b) + (f & 3u);
+    const bool f_on = col0 + f < p.cols;
 #pragma unroll
     for (int h = 0; h < kTiles; ++h) {
         const float* src = column + (h * kRows + 32 * b) * kCols;
@@ -164,29 +193,24 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
         for (uint32_t i = 0; i < 32; ++i) v[i] = src[i * kCols];
         const mx::Scale sc = mx::scale_of(mx::amax_of(v), emax);
         const uint32_t feature = h * p.cols + col0 + f;
-        if (col0 + f < p.cols) {
-            if (t0 < p.R) {
-                uint4* dst = reinterpret_cast<uint4*>(p.qt + static_cast<size_t>(feature) * p.R + t0);
+        if (f_on && t0 < p.R) {
+            uint2 c[4];
 #pragma unroll
-                for (uint32_t c = 0; c < 2; ++c) {
-                    const uint2 lo = mx::pack8(p.type, v + 16 * c, sc.inv);
-                    const uint2 hi = mx::pack8(p.type, v + 16 * c + 8, sc.inv);
-                    dst[c] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                }
-            }
-            p.sft[mx::word_offset(feature, t0 >> 7, kt) + ((t0 >> 5) & 3u)] =
-                t0 < p.R ? static_cast<uint8_t>(sc.code) : 0;
+            for (uint32_t k = 0; k < 4; ++k) c[k] = mx::pack8(p.type, v + 8 * k, sc.inv);
+            store32(p.qt + static_cast<size_t>(feature) * p.R + t0, c, p.wide);
         }
+        const uint32_t code = t0 < p.R ? sc.code : 0;
+        const uint32_t other = __shfl_down_sync(0xffffffffu, code, 1);
+        if (f_on && b == 0)
+            *reinterpret_cast<uint16_t*>(p.sft + mx::word_offset(feature, t0 >> 7, kt) +
+                                         ((t0 >> 5) & 3u)) = static_cast<uint16_t>(code | other << 8);
         if (MODE != kTranspose && p.partial) {
             f32x2 sum = 0;
 #pragma unroll
             for (uint32_t i = 0; i < 32; i += 2)
                 sum = ptxstd::add2(sum, ptxstd::pack2f(v[i], v[i + 1]));
-            sums[b][f] = ptxstd::hsum2(sum);
-            __syncthreads();
-            if (b == 0 && col0 + f < p.cols)
-                p.partial[static_cast<size_t>(rt) * p.W + feature] = sums[0][f] + sums[1][f];
-            if (h + 1 < kTiles) __syncthreads();
+            const float own = ptxstd::hsum2(sum), next = __shfl_down_sync(0xffffffffu, own, 1);
+            if (f_on && b == 0) p.partial[static_cast<size_t>(rt) * p.W + feature] = own + next;
         }
     }
 
@@ -209,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 8)
 template <int MODE>
 int launch(Params& p, cudaStream_t stream) {
     p.R = (p.rows + 31) / 32 * 32;
+    p.wide = (reinterpret_cast<uintptr_t>(p.qt) & 31u) == 0;
     p.col_tiles = (p.cols + kCols - 1) / kCols;
     const uint64_t tiles = p.col_tiles * static_cast<uint64_t>(mx::padded_rows(p.rows) / kRows);
     if (tiles >= (1ull << 31)) return PTXSTD_EINVAL;

@@ -307,6 +307,31 @@ def test_act_backward(cuda, rows, cols, gated, fmt):
             assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 32), (129, 160)])
+def test_act_backward_into_given_memory(cuda, rows, cols):
+    """Outputs at 16-byte boundaries that are not 32-byte ones, with guards around (C ABI)."""
+    import ptxstd
+    g = _gen(rows)
+    dh, gate, up = _bf(g, rows, cols), _bf(g, rows, cols), _bf(g, rows, cols)
+    row, col = ptxstd.act_backward_mx(dh, gate, up, act="gelu")
+    want = [*row, *col]
+    buf = [torch.full((t.numel() + 96,), 77, dtype=torch.uint8, device="cuda") for t in want]
+    assert ptxstd.lib().ptxstd_act_backward_mx(
+        3, dh.data_ptr(), gate.data_ptr(), up.data_ptr(), rows, cols, 1,
+        *[b.data_ptr() + 48 for b in buf], None, None, 0,
+        torch.cuda.current_stream().cuda_stream) == 0
+    xt = ptxstd.quantize_mx_t(dh, "e4m3")
+    want += xt
+    buf += [torch.full((t.numel() + 96,), 77, dtype=torch.uint8, device="cuda") for t in xt]
+    assert ptxstd.lib().ptxstd_quantize_mx_t(
+        dh.data_ptr(), rows, cols, 0, buf[4].data_ptr() + 48, buf[5].data_ptr() + 48,
+        torch.cuda.current_stream().cuda_stream) == 0
+    _ok()
+    for b, t in zip(buf, want):
+        assert torch.equal(b[48:-48], t.reshape(-1))
+        assert (b[:48] == 77).all() and (b[-48:] == 77).all()
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 8), (32, 32), (33, 72), (200, 264), (1000, 136)])
 @pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
 def test_quantize_transposed(cuda, rows, cols, fmt):
