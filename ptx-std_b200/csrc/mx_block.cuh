@@ -194,13 +194,14 @@ constexpr float kC = 0.044715f;
 
 // The normal distribution: with a = |x|, phi its density and M(a) = Phi(-a) / phi(a) (Mills' ratio),
 //   Phi(x) = s + (1 - 2 s) phi M,   Phi(x) + x phi(x) = s + (1 - 2 s) phi (M - a),   s = [x > 0],
-// which keeps the lower tail's relative accuracy (1 + erf would cancel there). M is a degree-7
-// polynomial without constant term in t = 1 / (1 + 0.37 a / sqrt(2)) (the form of Abramowitz and
+// which keeps the lower tail's relative accuracy (1 + erf would cancel there). M is a degree-8
+// polynomial without constant term in t = 1 / (1 + 0.33 a / sqrt(2)) (the form of Abramowitz and
 // Stegun 7.1.26), its coefficients fitted here for the least largest relative error on 0 <= a <=
-// 13.5: 8.4e-7, a few times that of the exponential; beyond, phi is below the smallest normal
-// float. One degree more would give 8e-8, which no caller's rounding (2^-9 at the finest) shows.
-// With CUDA's erfcf instead, act_backward_mx with GELU took 192 us instead of 120 us at
-// 4096 x 16384; with erfcx, 1 - q and a choice for each element 90.7 us instead of 88.4 us.
+// 13.5: 1.3e-7, and 9e-8 of the result on average with the f32 arithmetic. (Degree 7 would save 1 %
+// of act_backward_mx's time, but its 8e-7 moves 8-bit codes off the exact value's rounding, a dozen
+// in a million.) Beyond 13.5, phi is below the smallest normal float. act_backward_mx with GELU,
+// 4096 x 16384, took 192 us with CUDA's erfcf when it took 120 us with a polynomial for erfcx, and
+// 91 us with that, 1 - q and a choice for each element where it takes 89 us in this form.
 struct Normal2 {
     f32x2 na, t, p, phi;  // -a; M = p t
     f32x2 s, sign;        // s and 1 - 2 s
@@ -209,15 +210,16 @@ __device__ __forceinline__ Normal2 normal2(f32x2 x) {
     const float2 v = unpack2(x);
     Normal2 n;
     n.na = pack2f(-fabsf(v.x), -fabsf(v.y));
-    n.t = rcp2(fma2(n.na, splat(-0.26162952f), splat(1.0f)));
+    n.t = rcp2(fma2(n.na, splat(-0.23334524f), splat(1.0f)));
     n.phi = exp2_2(fma2(mul2(x, x), splat(-0.5f * kLog2e), splat(-1.3257481f)));  // log2 phi(0)
-    f32x2 p = splat(-0.17795026f);
-    p = fma2(p, n.t, splat(0.5434346f));
-    p = fma2(p, n.t, splat(-0.22989362f));
-    p = fma2(p, n.t, splat(0.39500487f));
-    p = fma2(p, n.t, splat(0.1924486f));
-    p = fma2(p, n.t, splat(0.26908714f));
-    n.p = fma2(p, n.t, splat(0.26118386f));
+    f32x2 p = splat(-0.17008568f);
+    p = fma2(p, n.t, splat(0.57873446f));
+    p = fma2(p, n.t, splat(-0.4434476f));
+    p = fma2(p, n.t, splat(0.51513124f));
+    p = fma2(p, n.t, splat(0.05745955f));
+    p = fma2(p, n.t, splat(0.2527419f));
+    p = fma2(p, n.t, splat(0.22920893f));
+    n.p = fma2(p, n.t, splat(0.23357132f));
     float a, b;
     asm("set.gt.f32.f32 %0, %1, 0f00000000;" : "=f"(a) : "f"(v.x));
     asm("set.gt.f32.f32 %0, %1, 0f00000000;" : "=f"(b) : "f"(v.y));
