@@ -15,8 +15,8 @@
 // kernel: ReLU 82 us instead of 71 us, the transposing quantiser of 8192 x 8192 50 us instead of
 // 41 us, gated 99 us instead of 88 us.)
 // 4096 x 16384, E5M2, column sums included, results of successive calls in different buffers, under
-// load: 407 MB in 71 us with ReLU (0.88 of the measured copy rate), 89 us with GELU, which takes 30
-// instructions per element to ReLU's 20 and so the issue slots to three quarters (ncu); at the
+// load: 407 MB in 71 us with ReLU (0.88 of the measured copy rate), 89 us with GELU, which takes 31
+// instructions per element to ReLU's 21 and so the issue slots to three quarters (ncu); at the
 // clock of an idle GPU 67 and 80 us. Gated, SiLU, 4096 x 10240: 425 MB in 88 us (0.74). The
 // transposing quantiser of 8192 x 8192: 204 MB in 41 us (0.76). Without effect or slower: other
 // orders of the tiles, prefetching a later tile to L2, a persistent form that copies the next tile
@@ -85,7 +85,7 @@ __device__ __forceinline__ void row_block(uint32_t type, const float (&v)[8], bo
 }
 
 // Blocks per SM asked of the compiler: enough registers that all of a tile's loads are in flight at
-// once. Gated, SiLU, 4096 x 10240: 84 us with 5 (93 registers), 110 us with 6 (80 registers, loads
+// once. Gated, SiLU, 4096 x 10240: 84 us with 5 (96 registers), 110 us with 6 (80 registers, loads
 // in turn with their use). Ungated, GELU, 4096 x 16384: 81 us with 9, 83 us with 8, 88 us with 10.
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, MODE == kGated ? 5 : 9)
