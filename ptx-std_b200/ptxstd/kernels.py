@@ -7,6 +7,30 @@ from . import _dev, _stream, _torch, check, lib
 SF_ROWMAJOR, SF_BLOCKED, SF_PADDED = 0, 1, 2
 
 
+def _given(t, nbytes: int, device, name: str):
+    """An output that the caller gave: refused unless it holds what the call writes there (a kernel
+    would run over whatever lies behind it)."""
+    if t.device != device:
+        raise ValueError(f"{name}: on {t.device}, but the inputs are on {device}")
+    if t.numel() * t.element_size() < nbytes:
+        raise ValueError(f"{name}: too small ({t.numel() * t.element_size()} bytes, the call "
+                         f"writes {nbytes})")
+    return t
+
+
+def _given_pair(out, q_bytes: int, sf_bytes: int, device):
+    q, sf = out
+    return _given(q, q_bytes, device, "q"), _given(sf, sf_bytes, device, "sf")
+
+
+def _result(out, M: int, N: int, device):
+    """The bf16 [M, N] result of a GEMM: the caller's, or a new one."""
+    if out is not None:
+        return _given(out, 2 * M * N, device, "out")
+    torch = _torch()
+    return torch.empty((M, N), dtype=torch.bfloat16, device=device)
+
+
 def quantize_mxfp8(x, sf_layout: int = SF_ROWMAJOR, out=None, stream=None, seed=None):
     """bf16 [rows, cols] -> (E4M3 [rows, cols] uint8, UE8M0 scales uint8).
 
@@ -22,7 +46,7 @@ def quantize_mxfp8(x, sf_layout: int = SF_ROWMAJOR, out=None, stream=None, seed=
         q = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
         sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
     else:
-        q, sf = out
+        q, sf = _given_pair(out, rows * cols, rows * (cols // 32), x.device)
     if seed is None:
         check(lib().ptxstd_quantize_mxfp8_layout(_dev(x), rows, cols, _dev(q), _dev(sf),
                                                  sf_layout, _stream(stream)), "quantize_mxfp8")
@@ -42,7 +66,7 @@ def gemm_fp8(a, b, sa: float = 1.0, sb: float = 1.0, out=None, stream=None):
     N = b.shape[0]
     if b.shape[1] != K:
         raise ValueError("K mismatch")
-    c = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+    c = _result(out, M, N, a.device)
     check(lib().ptxstd_gemm_fp8(_dev(a), _dev(b), float(sa), float(sb), _dev(c), M, N, K,
                                 _stream(stream)), "gemm_fp8")
     return c
@@ -50,14 +74,13 @@ def gemm_fp8(a, b, sa: float = 1.0, sb: float = 1.0, out=None, stream=None):
 
 def gemm_mxfp8(a, sfa, b, sfb, out=None, stream=None):
     """MXFP8 a [M, K], b [N, K] (uint8, E4M3) with blocked UE8M0 scales per 32 -> bf16 [M, N]."""
-    torch = _torch()
     M, K = a.shape
     N = b.shape[0]
     if b.shape[1] != K:
         raise ValueError("K mismatch")
     if sfa.numel() != M * K // 32 or sfb.numel() != N * K // 32:
         raise ValueError("scale tensors must hold one UE8M0 per 32 elements")
-    c = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+    c = _result(out, M, N, a.device)
     check(lib().ptxstd_gemm_mxfp8(_dev(a), _dev(sfa), _dev(b), _dev(sfb), _dev(c), M, N, K,
                                   _stream(stream)), "gemm_mxfp8")
     return c
@@ -86,15 +109,14 @@ def quantize_mx(x, elem_type, sf_layout: int = 1, out=None, stream=None):
         raise TypeError("expected a 2-D bfloat16 tensor")
     t = _mx_type(elem_type)
     rows, cols = x.shape
+    padded = -(-rows // 128) * -(-cols // 128) * 512
     if out is None:
         q = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
-        if sf_layout == SF_PADDED:
-            sf = torch.empty(-(-rows // 128) * -(-cols // 128) * 512, dtype=torch.uint8,
-                             device=x.device)
-        else:
-            sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
+        sf = torch.empty(padded if sf_layout == SF_PADDED else (rows, cols // 32),
+                         dtype=torch.uint8, device=x.device)
     else:
-        q, sf = out
+        q, sf = _given_pair(out, rows * cols,
+                            padded if sf_layout == SF_PADDED else rows * (cols // 32), x.device)
     check(lib().ptxstd_quantize_mx(_dev(x), rows, cols, t, _dev(q), _dev(sf), sf_layout,
                                    _stream(stream)), "quantize_mx")
     return q, sf
@@ -103,7 +125,6 @@ def quantize_mx(x, elem_type, sf_layout: int = 1, out=None, stream=None):
 def gemm_mx(a, a_type, sfa, b, b_type, sfb, out=None, stream=None):
     """MX GEMM with any pair of element types: a [M, K], b [N, K] payloads in the operand layout
     of quantize_mx, blocked UE8M0 scales per 32 -> bf16 [M, N]."""
-    torch = _torch()
     ta, tb = _mx_type(a_type), _mx_type(b_type)
     M, K = a.shape
     N = b.shape[0]
@@ -111,7 +132,7 @@ def gemm_mx(a, a_type, sfa, b, b_type, sfb, out=None, stream=None):
         raise ValueError("K mismatch")
     if sfa.numel() != M * K // 32 or sfb.numel() != N * K // 32:
         raise ValueError("scale tensors must hold one UE8M0 per 32 elements")
-    c = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+    c = _result(out, M, N, a.device)
     check(lib().ptxstd_gemm_mx(_dev(a), ta, _dev(sfa), _dev(b), tb, _dev(sfb), _dev(c), M, N, K,
                                _stream(stream)), "gemm_mx")
     return c
@@ -151,7 +172,6 @@ def prune_24(codes, stream=None):
 def gemm_mxfp8_sparse(vals, meta, sfa, b, sfb, out=None, stream=None):
     """2:4-sparse MXFP8: A as (vals [M, K/2], meta [M, K/8]) from prune_24, b [N, K] E4M3, blocked
     UE8M0 scales per 64 logical K for both operands -> bf16 [M, N]."""
-    torch = _torch()
     M, Kh = vals.shape
     K = 2 * Kh
     N = b.shape[0]
@@ -159,7 +179,7 @@ def gemm_mxfp8_sparse(vals, meta, sfa, b, sfb, out=None, stream=None):
         raise ValueError("shape mismatch")
     if sfa.numel() != M * K // 64 or sfb.numel() != N * K // 64:
         raise ValueError("scale tensors must hold one UE8M0 per 64 logical elements")
-    c = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=vals.device)
+    c = _result(out, M, N, vals.device)
     check(lib().ptxstd_gemm_mxfp8_sparse(_dev(vals), _dev(meta), _dev(sfa), _dev(b), _dev(sfb),
                                          _dev(c), M, N, K, _stream(stream)), "gemm_mxfp8_sparse")
     return c
@@ -181,7 +201,6 @@ def get_gemm_schedule() -> int:
 
 def gemm_nvfp4(a, sfa, ga: float, b, sfb, gb: float, out=None, stream=None):
     """NVFP4 a [M, K/2], b [N, K/2] (uint8, E2M1x2) with blocked E4M3 scales -> bf16 [M, N]."""
-    torch = _torch()
     M, Kh = a.shape
     N = b.shape[0]
     if b.shape[1] != Kh:
@@ -189,7 +208,7 @@ def gemm_nvfp4(a, sfa, ga: float, b, sfb, gb: float, out=None, stream=None):
     K = 2 * Kh
     if sfa.numel() != M * K // 16 or sfb.numel() != N * K // 16:
         raise ValueError("scale tensors must hold one E4M3 per 16 elements")
-    c = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+    c = _result(out, M, N, a.device)
     check(lib().ptxstd_gemm_nvfp4(_dev(a), _dev(sfa), float(ga), _dev(b), _dev(sfb), float(gb),
                                   _dev(c), M, N, K, _stream(stream)), "gemm_nvfp4")
     return c
@@ -225,7 +244,7 @@ def gemm_decode(x, w, sfw, gw: float, out=None, workspace=None, stream=None):
     N = w.shape[0]
     if w.shape[1] * 2 != K or sfw.numel() != N * K // 16:
         raise ValueError("shape mismatch")
-    y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    y = _result(out, M, N, x.device)
     if workspace is None:
         _, ptr, nbytes = decode_workspace(M, N, K, x.device)
     else:
@@ -248,7 +267,7 @@ def quantize_nvfp4(x, global_scale: float, sf_layout: int = SF_ROWMAJOR, out=Non
         q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x.device)
         sf = torch.empty((rows, cols // 16), dtype=torch.uint8, device=x.device)
     else:
-        q, sf = out
+        q, sf = _given_pair(out, rows * (cols // 2), rows * (cols // 16), x.device)
     if seed is None:
         check(lib().ptxstd_quantize_nvfp4_layout(_dev(x), rows, cols, float(global_scale),
                                                  _dev(q), _dev(sf), sf_layout, _stream(stream)),

@@ -62,3 +62,57 @@ def test_gemm_schedule_setting(ptxstd_lib):
         assert ptxstd.get_gemm_schedule() == ptxstd.SCHEDULE_DYNAMIC
     finally:
         ptxstd.set_gemm_schedule(ptxstd.SCHEDULE_PERSISTENT)
+
+
+@pytest.mark.parametrize("rows,cols,layout,need", [(1, 32, 2, 512), (129, 160, 2, 2 * 2 * 512),
+                                                   (128, 128, 1, 512), (5, 96, 0, 15)])
+def test_quantize_mx_given_outputs_have_room(ptxstd_lib, rows, cols, layout, need):
+    """The padded layout clears and writes whole tiles, more than rows * cols / 32 bytes: a pair made
+    for another layout is refused before the call. What is large enough gets as far as the check
+    for device memory."""
+    import torch
+
+    import ptxstd
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16)
+
+    def call(nq, nsf):
+        out = (torch.zeros(nq, dtype=torch.uint8), torch.zeros(nsf, dtype=torch.uint8))
+        ptxstd.quantize_mx(x, "e4m3", sf_layout=layout, out=out)
+
+    with pytest.raises(ValueError, match="sf: too small"):
+        call(rows * cols, need - 1)
+    with pytest.raises(ValueError, match="q: too small"):
+        call(rows * cols - 1, need)
+    with pytest.raises(TypeError, match="CUDA"):
+        call(rows * cols, need)
+    with pytest.raises(ValueError, match="sf: on"):
+        ptxstd.quantize_mx(x, "e4m3", sf_layout=layout,
+                           out=(torch.zeros(rows * cols, dtype=torch.uint8),
+                                torch.zeros(need, dtype=torch.uint8, device="meta")))
+
+
+def test_given_outputs_have_room(ptxstd_lib):
+    """The same for every other call that writes into a tensor it is given."""
+    import torch
+
+    import ptxstd
+    x = torch.zeros((128, 256), dtype=torch.bfloat16)
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    c = torch.zeros(128 * 128 - 1, dtype=torch.bfloat16)
+    calls = {
+        "mxfp8": lambda: ptxstd.quantize_mxfp8(x, out=(u8(128, 256), u8(128 * 8 - 1))),
+        "nvfp4": lambda: ptxstd.quantize_nvfp4(x, 1.0, out=(u8(128, 127), u8(128, 16))),
+        "fp8": lambda: ptxstd.gemm_fp8(u8(128, 64), u8(128, 64), out=c),
+        "gemm_mxfp8": lambda: ptxstd.gemm_mxfp8(u8(128, 64), u8(256), u8(128, 64), u8(256), out=c),
+        "gemm_mx": lambda: ptxstd.gemm_mx(u8(128, 64), 0, u8(256), u8(128, 64), 0, u8(256), out=c),
+        "sparse": lambda: ptxstd.gemm_mxfp8_sparse(u8(128, 32), u8(128, 8), u8(128), u8(128, 64),
+                                                   u8(128), out=c),
+        "gemm_nvfp4": lambda: ptxstd.gemm_nvfp4(u8(128, 32), u8(512), 1.0, u8(128, 32), u8(512),
+                                                1.0, out=c),
+        "decode": lambda: ptxstd.gemm_decode(x[:16, :64], u8(128, 32), u8(512), 1.0, out=c[:2047],
+                                             workspace=(0, 0)),
+    }
+    for name, call in calls.items():
+        with pytest.raises(ValueError, match="too small"):
+            call()
+            pytest.fail(name)
