@@ -552,10 +552,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             w.row = static_cast<uint32_t>(w.row0) + lane;
             const uint32_t col0 = nb * kTileN + half * (GATED ? 64 : 128);
             // while the accumulator is being computed: the bias to registers, residual boxes to the
-            // staging buffers
+            // staging buffers (the bias by an ordinary load: under programmatic launch the kernel before
+            // may write it while this grid is resident, which ld.global.nc does not allow for)
             float bias[4] = {};
             if (!GATED && e.bias && col0 + 4 * lane < N) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(e.bias + col0 + 4 * lane));
+                const uint2 v = *reinterpret_cast<const uint2*>(e.bias + col0 + 4 * lane);
                 bias[0] = dt::bf16_lo(v.x);
                 bias[1] = dt::bf16_hi(v.x);
                 bias[2] = dt::bf16_lo(v.y);
@@ -846,8 +847,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     ptxstd::pdl_wait();
     float bias[8] = {};
     if (!GATED && e.bias && block * 128 + (tid & 15u) * 8 < p.N) {
-        const uint4 w =
-            __ldg(reinterpret_cast<const uint4*>(e.bias + block * 128 + (tid & 15u) * 8));
+        const uint4 w = *reinterpret_cast<const uint4*>(e.bias + block * 128 + (tid & 15u) * 8);
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {

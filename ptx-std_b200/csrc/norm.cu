@@ -17,12 +17,12 @@
 // m2 needs dx, hence m1. Substituting dx gives, with t = scale g w_post y,
 //   m2 = ry mean(t dx) = ry (sum(t du) + rx (sum(t a) - m1 rx sum(t x'))) / D,  m1 = rx sum(a x') / D,
 // so one exchange of four sums serves both means. (No power of rx or ry stands alone: rx^3 leaves
-// f32's range for rows around 1e13 or 1e-13, where the norms themselves are still exact.) With one gate for all rows both dg and dw_post
-// are column factors times the same sum, S = sum_rows dx y ry: dg = scale w_post S,
-// dw_post = scale g S; with a gate per row dg needs no sum and S takes g inside. So there are two
-// column sums at most. Each thread keeps its columns for all rows of its group and accumulates
-// them in f32; the partial sums go through a workspace and are added in order by a second kernel
-// (reproducible, no atomics), which applies the factors.
+// f32's range for rows around 1e13 or 1e-13, where the norms themselves are still exact.) With one
+// gate for all rows both dg and dw_post are column factors times the same sum, S = sum_rows dx y ry:
+// dg = scale w_post S, dw_post = scale g S; with a gate per row dg needs no sum and S takes g inside.
+// So there are two column sums at most. Each thread keeps its columns for all rows of its group and
+// accumulates them in f32; the partial sums go through a workspace and are added in order by a second
+// kernel (reproducible, no atomics), which applies the factors.
 //
 // Both directions are near the issue rate as well as the HBM rate (67 % and 60 % of the issue
 // slots, ncu), hence the packed f32 pairs. Forward, 8192 x 8192 with w_post, gate and E4M3 out:
@@ -76,6 +76,13 @@ struct Fwd {
     uint32_t rows, cols, q_type, blocked;
     size_t gate_stride;  // 0: one gate for all rows
 };
+
+// Vector i (eight columns) of a bf16 array. An ordinary load, not ld.global.nc: under programmatic
+// launch the kernel before may write the array while this grid is already resident, and a load
+// that takes the memory for constant may be moved above the wait or served from an old L1 line.
+__device__ __forceinline__ uint4 load16(const uint16_t* p, uint32_t i) {
+    return reinterpret_cast<const uint4*>(p)[i];
+}
 
 __device__ __forceinline__ f32x2 square_sum(const uint4& v, f32x2 s) {
     const Oct a = widen(v);
@@ -165,12 +172,12 @@ __device__ __forceinline__ Oct branch_factor(const uint16_t* w_post, const uint1
 #pragma unroll
     for (int k = 0; k < 4; ++k) f.v[k] = pack2f(scale, scale);
     if (w_post) {
-        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(w_post) + i));
+        const Oct o = widen(load16(w_post, i));
 #pragma unroll
         for (int k = 0; k < 4; ++k) f.v[k] = mul2(f.v[k], o.v[k]);
     }
     if (gate) {
-        const Oct o = widen(__ldg(reinterpret_cast<const uint4*>(gate) + i));
+        const Oct o = widen(load16(gate, i));
 #pragma unroll
         for (int k = 0; k < 4; ++k) f.v[k] = mul2(f.v[k], o.v[k]);
     }
@@ -232,8 +239,13 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
         }
     }
     f32x2 s = 0;
+    uint4 w[V];  // loaded before the exchange, which hides them
 #pragma unroll
-    for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
+    for (int j = 0; j < V; ++j) {
+        const uint32_t i = tid + j * stride;
+        w[j] = i < nv ? load16(p.w, i) : make_uint4(0, 0, 0, 0);
+        s = square_sum(xv[j], s);
+    }
     const float rx = rsqrtf(row_sum<WARP_ROW>(hsum2(s), red[1]) * inv_d + p.eps);
     if (p.rstd && tid == 0) p.rstd[row] = rx;
     const ScaleRow sr(p, row, k_tiles);
@@ -241,9 +253,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const uint32_t i = tid + j * stride;
-        const bool on = i < nv;
-        const uint4 w = on ? __ldg(reinterpret_cast<const uint4*>(p.w) + i) : make_uint4(0, 0, 0, 0);
-        finish8(p, xv[j], w, rx, base, i, on, lane, sr);
+        finish8(p, xv[j], w[j], rx, base, i, i < nv, lane, sr);
     }
 }
 
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(THREADS* GROUPS, 1)
     if (tid == 0)
         for (uint32_t k = 0; k < stages; ++k) ring.load(k, k);
     for (uint32_t i = tid; i < nv; i += blockDim.x) {
-        w[i] = __ldg(reinterpret_cast<const uint4*>(p.w) + i);
+        w[i] = load16(p.w, i);
         if (p.y)
             store_planes(c, nv, i,
                          branch_factor(p.w_post, gate_rows ? nullptr : p.gate, p.scale, i));
@@ -533,7 +543,7 @@ struct Factors {
     Oct w, c;
 };
 __device__ __forceinline__ Factors column_factors(const Bwd& p, uint32_t i) {
-    return {widen(__ldg(reinterpret_cast<const uint4*>(p.w) + i)),
+    return {widen(load16(p.w, i)),
             branch_factor(p.w_post, p.gate_stride ? nullptr : p.gate, p.scale, i)};
 }
 

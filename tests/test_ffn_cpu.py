@@ -192,3 +192,19 @@ def test_rounding_restatement():
         x = torch.cat([v, (v[1:] + v[:-1]) / 2, (v[1:] * 0.7 + v[:-1] * 0.3)])
         assert torch.equal(R._round(x.double(), fmt).float(), x.to(R.F8[fmt]).float())
     assert C.sizeof(C.c_void_p) == 8
+
+
+def test_no_non_coherent_loads_under_programmatic_launch():
+    """A kernel launched with programmatic stream serialisation runs beside the one before it, which
+    may still be writing what this one reads after griddepcontrol.wait (a bias, a gate, a weight
+    vector). ld.global.nc asks for memory that nothing writes while the kernel runs, and the compiler
+    may move such a load above the wait."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "ptx-std_b200", "csrc")
+    for name in ("norm.cu", "act_backward.cu", "gemm_mx_fused.cu", "reduce.cuh", "mx_block.cuh",
+                 "epilogue.cuh", "common.cuh"):
+        with open(os.path.join(csrc, name)) as f:
+            code = re.sub(r"//.*", "", f.read())
+        assert not re.search(r"__ldg|global\.nc|__restrict__", code), name

@@ -1019,6 +1019,62 @@ def test_beside_the_other_gemms(cuda):
             assert torch.equal(u, v)
 
 
+def test_vectors_written_by_the_call_before(cuda):
+    """Weight, gate and bias vectors that the previous call of the stream writes, into the buffer that
+    the calls before it read: with programmatic launch all of them may be resident at once. Without a
+    wait in between, every result is that of calls which are waited for."""
+    import ptxstd
+    D, K = 8192, 64
+    g = _gen(17)
+    b, sfb = _mx(g, D, K, std=K ** -0.5)
+    tokens = [_mx(g, 1, K) for _ in range(2)]
+    buf = torch.zeros(D, dtype=torch.bfloat16, device="cuda")
+    rows = (1600, 300, 3)  # the ring, a row per block with two vectors per thread and with one
+    x, y = _bf(g, rows[0], D, std=2.0), _bf(g, rows[0], D, std=0.7)
+    dn = _bf(g, rows[0], D, std=0.3)
+    rx = torch.rsqrt(x.double().square().mean(1) + 1e-6).float()
+    ry = torch.rsqrt(y.double().square().mean(1) + 1e-6).float()
+    wide, narrow = _mx(g, 2048, K), _mx(g, 5, K)
+    L = ptxstd.lib()
+
+    def write(i):
+        a, sfa = tokens[i]
+        assert L.ptxstd_gemm_mx_epilogue(
+            a.data_ptr(), 0, sfa.data_ptr(), b.data_ptr(), 0, sfb.data_ptr(), None, 0, None,
+            buf.data_ptr(), None, 0, None, None, 1, D, K,
+            torch.cuda.current_stream().cuda_stream) == 0
+
+    def reads():
+        for r in rows:
+            yield lambda r=r: ptxstd.rmsnorm_residual(x[:r], buf, y=y[:r], w_post=buf, gate=buf)[:2]
+        for r in rows[1:]:
+            for c in (1024, 4096, D):  # registers, the ring
+                part = [t[:r, :c].contiguous() for t in (dn, x, y)]
+                yield lambda r=r, c=c, part=part: ptxstd.rmsnorm_residual_backward(
+                    part[0], part[1], buf[:c], (rx[:r], ry[:r]), y=part[2], w_post=buf[:c],
+                    gate=buf[:c])
+        for a, sfa in (wide, narrow):
+            yield lambda a=a, sfa=sfa: ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb,
+                                                               bias=buf)
+
+    for read in reads():
+        want = []
+        for i in range(2):
+            write(i)
+            torch.cuda.synchronize()
+            want.append(read())
+            torch.cuda.synchronize()
+        got = []
+        for k in range(20):
+            write(k % 2)
+            got.append(read())
+        _ok()
+        assert not torch.equal(_flat([want[0]])[0], _flat([want[1]])[0])
+        for k, r in enumerate(got):
+            for p, q in zip(_flat([want[k % 2]]), _flat([r])):
+                assert torch.equal(p, q), k
+
+
 def test_device_refusals(cuda):
     import ptxstd
     x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
