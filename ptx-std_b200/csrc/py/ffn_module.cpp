@@ -5,7 +5,8 @@
 // (include/ptxstd.h), which check sizes, alignment and types again.
 //
 // Functions take positional arguments only (ptxstd/ffn.py has the public signatures). Type errors
-// raise TypeError, shapes and devices ValueError, a status of the library ptxstd.PtxStdError.
+// raise TypeError, shapes and devices ValueError, a status of the library ptxstd.PtxStdError, and
+// what torch throws meanwhile is raised as torch raises it.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -13,6 +14,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -407,8 +409,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return F(args);
     } catch (const PythonError&) {
         return nullptr;
-    } catch (const std::exception& e) {  // an allocation failure, say
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {  // torch's own errors as torch raises them (torch.OutOfMemoryError, say)
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
 }

@@ -1075,6 +1075,24 @@ def test_vectors_written_by_the_call_before(cuda):
                 assert torch.equal(p, q), k
 
 
+def test_out_of_memory_is_torchs_error(cuda):
+    """A result that does not fit raises torch.OutOfMemoryError, as every torch allocation does (here
+    under a limit of this process's own, well below the 8.6 GB asked for), and the next call works."""
+    import ptxstd
+    rows = 65536
+    g = _gen(1)
+    a, sfa = _mx(g, rows, 32)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.02)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, a, "e4m3", sfa)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    ptxstd.gemm_mx_epilogue(a[:128], "e4m3", sfa[:512], a[:256], "e4m3", sfa[:1024])
+    _ok()
+
+
 def test_device_refusals(cuda):
     import ptxstd
     x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
