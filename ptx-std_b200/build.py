@@ -88,15 +88,20 @@ MODULE_SRC = os.path.join(CSRC, "py", "ffn_module.cpp")
 MODULE = os.path.join(HERE, "ptxstd", "_ffn.so")
 
 
-def build_module(force: bool = False) -> str:
-    """ptxstd/_ffn.so, rebuilt when its source, the C header or this file is newer."""
+def build_module(force: bool = False) -> str | None:
+    """ptxstd/_ffn.so, rebuilt when its source, the C header or this file is newer. None where torch
+    is not installed: the library itself does not need it, only the Python calls do."""
     inputs = [MODULE_SRC, os.path.join(ROOT, "include", "ptxstd.h"), __file__]
     if not force and os.path.exists(MODULE) and \
             os.path.getmtime(MODULE) > max(os.path.getmtime(f) for f in inputs):
         return MODULE
     import importlib.util
     import sysconfig
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        print("torch is not installed: ptxstd/_ffn.so is not built", file=sys.stderr)
+        return None
+    torch = os.path.dirname(spec.origin)
     cuda = os.path.dirname(os.path.dirname(NVCC))
     inc = [os.path.join(torch, "include"), os.path.join(cuda, "include"),
            sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]

@@ -208,3 +208,22 @@ def test_no_non_coherent_loads_under_programmatic_launch():
         with open(os.path.join(csrc, name)) as f:
             code = re.sub(r"//.*", "", f.read())
         assert not re.search(r"__ldg|global\.nc|__restrict__", code), name
+
+
+def test_the_library_builds_without_torch(ptxstd_lib, monkeypatch, capsys):
+    """The C library needs nvcc only; where torch is not installed the Python extension module is left
+    out, with a word, and the build of the library still succeeds."""
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location(
+        "ptxstd_build_test", os.path.join(root, "ptx-std_b200", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    before = os.path.getmtime(build.MODULE)
+    find = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec",
+                        lambda name, *a: None if name == "torch" else find(name, *a))
+    assert build.build_module(force=True) is None
+    assert "torch" in capsys.readouterr().err
+    assert os.path.getmtime(build.MODULE) == before
