@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(WARP_ROW ? 32 * kWarpRows : 1024)
 // row's sums, another's stores and the loads of later rows overlap. A group copies its row to
 // registers first; once it has met in the row's first sum, the stage is free and its first thread
 // sends the row `stages` further on into it. The ring is thus in flight nearly all of the time,
-// whatever the groups wait for. Column weights sit in shared memory for the CTA's life.
+// whatever the groups wait for. Column weights sit in shared memory for the CTA's life. The forward
+// ring is for rows with both norms (y and w_post given).
 constexpr uint32_t kRingBytes = 222 * 1024;
 constexpr uint32_t kMaxRing = 12;
 enum : uint32_t { kDetailFwd = 0x4200, kDetailBwd = 0x4400 };
@@ -370,12 +371,12 @@ __global__ void __launch_bounds__(THREADS* GROUPS, 1)
     const uint32_t nv = p.cols / 8;
     const size_t k_tiles = mx::tiles_k(p.cols / 32);
     const bool gate_rows = p.gate && p.gate_stride;
-    // shared memory: w (bf16) | with y, c = scale w_post gate in f32 (the gate of all rows; 1 where
-    // there is none) | stages of x | y | gate row
+    // shared memory: w (bf16) | c = scale w_post gate in f32 (the gate of all rows; 1 where there is
+    // none) | stages of x | y | gate row
     uint4* const w = ring_smem;
     float4* const c = reinterpret_cast<float4*>(w + nv);
-    uint4* const stage0 = w + (p.y ? 3 : 1) * nv;
-    const uint32_t arrays = 1 + (p.y ? 1 : 0) + (gate_rows ? 1 : 0);
+    uint4* const stage0 = w + 3 * nv;
+    const uint32_t arrays = 2 + (gate_rows ? 1 : 0);
     Ring ring = {state,
                  reinterpret_cast<uint8_t*>(stage0),
                  {p.x, p.y, gate_rows ? p.gate : nullptr, nullptr, nullptr},
@@ -388,9 +389,8 @@ __global__ void __launch_bounds__(THREADS* GROUPS, 1)
         for (uint32_t k = 0; k < stages; ++k) ring.load(k, k);
     for (uint32_t i = tid; i < nv; i += blockDim.x) {
         w[i] = load16(p.w, i);
-        if (p.y)
-            store_planes(c, nv, i,
-                         branch_factor(p.w_post, gate_rows ? nullptr : p.gate, p.scale, i));
+        store_planes(c, nv, i,
+                     branch_factor(p.w_post, gate_rows ? nullptr : p.gate, p.scale, i));
     }
     for (uint32_t row = p.rows + blockIdx.x; row < mx::padded_rows(p.rows); row += gridDim.x)
         pad_row(p, row, tid, blockDim.x, k_tiles);
@@ -421,52 +421,45 @@ __global__ void __launch_bounds__(THREADS* GROUPS, 1)
         const uint4* const xs = stage0 + static_cast<size_t>(stage) * arrays * nv;
         const size_t base = static_cast<size_t>(row) * p.cols;
         uint4 xv[V], yv[V];
+        f32x2 s = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t i = t + j * THREADS;
             xv[j] = yv[j] = make_uint4(0, 0, 0, 0);
             if (i < nv) {
                 xv[j] = xs[i];
-                if (p.y) yv[j] = xs[nv + i];
+                yv[j] = xs[nv + i];
             }
+            s = square_sum(yv[j], s);
         }
-        if (p.y) {
-            float ry = 1.0f;
-            if (p.w_post) {
-                f32x2 s = 0;
-#pragma unroll
-                for (int j = 0; j < V; ++j) s = square_sum(yv[j], s);
-                ry = rsqrtf(group_sum(hsum2(s), red[g][0]) * inv_d + p.eps);
-                if (t == 0) {
-                    if (p.rstd_post) p.rstd_post[row] = ry;
-                    if (!gate_rows) ring.load(k + stages, stage);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t i = t + j * THREADS;
-                if (i >= nv) continue;
-                Oct x = widen(xv[j]), y = widen(yv[j]);
-                const Oct f = load_planes(c, nv, i);
-                const f32x2 r = pack2f(ry, ry);
-                if (gate_rows) {
-                    const Oct g = widen(xs[2 * nv + i]);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) y.v[q] = mul2(y.v[q], g.v[q]);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) x.v[q] = fma2(mul2(y.v[q], r), f.v[q], x.v[q]);
-                xv[j] = narrow(x);
-                *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
-            }
+        const float ry = rsqrtf(group_sum(hsum2(s), red[g][0]) * inv_d + p.eps);
+        if (t == 0) {
+            if (p.rstd_post) p.rstd_post[row] = ry;
+            if (!gate_rows) ring.load(k + stages, stage);
         }
-        f32x2 s = 0;
+        s = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) s = square_sum(xv[j], s);
+        for (int j = 0; j < V; ++j) {
+            const uint32_t i = t + j * THREADS;
+            if (i >= nv) continue;
+            Oct x = widen(xv[j]), y = widen(yv[j]);
+            const Oct f = load_planes(c, nv, i);
+            const f32x2 r = pack2f(ry, ry);
+            if (gate_rows) {
+                const Oct g = widen(xs[2 * nv + i]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) y.v[q] = mul2(y.v[q], g.v[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x.v[q] = fma2(mul2(y.v[q], r), f.v[q], x.v[q]);
+            xv[j] = narrow(x);
+            *reinterpret_cast<uint4*>(p.x_out + base + 8 * i) = xv[j];
+            s = square_sum(xv[j], s);
+        }
         const float rx = rsqrtf(group_sum(hsum2(s), red[g][1 + flip]) * inv_d + p.eps);
         if (t == 0) {
             if (p.rstd) p.rstd[row] = rx;
-            if (!p.w_post || gate_rows) ring.load(k + stages, stage);
+            if (gate_rows) ring.load(k + stages, stage);  // the gate row was read until here
         }
         const ScaleRow sr(p, row, k_tiles);
         sr.pad(p, t);
@@ -504,14 +497,14 @@ uint32_t ring_stages(size_t fixed, size_t row_bytes) {
     return static_cast<uint32_t>(n < kMaxRing ? n : kMaxRing);
 }
 
-// -1 where the rows are too long for a stage per group.
 template <int V, uint32_t THREADS, uint32_t GROUPS>
 int launch_fwd_ring(const Fwd& p, cudaStream_t stream) {
     auto* kernel = norm_ring_kernel<V, THREADS, GROUPS>;
-    const size_t vec = static_cast<size_t>(p.cols) * 2, fixed = vec * (p.y ? 3 : 1);
-    const size_t row = vec * (1 + (p.y ? 1 : 0) + (p.gate && p.gate_stride ? 1 : 0));
+    const size_t vec = static_cast<size_t>(p.cols) * 2, fixed = 3 * vec;
+    const size_t row = vec * (2 + (p.gate && p.gate_stride ? 1 : 0));
+    // at most 8192 columns: beside 48 KB of weights, three rows of 48 KB; with 4096, eight of 24 KB
     const uint32_t stages = ring_stages(fixed, row);
-    if (stages < GROUPS) return -1;
+    if (stages < GROUPS) return PTXSTD_EINVAL;
     const int st = ptxstd::set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes);
     if (st) return st;
     uint32_t* err = ptxstd::device_error_word();
@@ -966,11 +959,9 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
     // fewer elements (2400 x 4096: 17.9 against 18.6 us) and for rows that leave much of the long
     // rows' groups idle (3000 x 5152: 28.3 against 29.5 us).
     if (d_w_post && rows * cols >= 12'000'000) {
-        int st = -1;
-        if (nv <= 256) st = launch_fwd_ring<2, 128, 6>(p, s);
-        else if (nv <= 512) st = launch_fwd_ring<4, 128, 6>(p, s);
-        else if (nv > 768 && nv <= 1024) st = launch_fwd_ring<4, 256, 3>(p, s);
-        if (st >= 0) return st;
+        if (nv <= 256) return launch_fwd_ring<2, 128, 6>(p, s);
+        if (nv <= 512) return launch_fwd_ring<4, 128, 6>(p, s);
+        if (nv > 768 && nv <= 1024) return launch_fwd_ring<4, 256, 3>(p, s);
     }
     // A row per block: one vector per thread while a block can be that large and a row's latency
     // counts (100 x 4096: 3.4 us, 3.8 us with two); two once an SM has several rows, so that more
