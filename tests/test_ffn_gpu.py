@@ -1106,3 +1106,80 @@ def test_device_refusals(cuda):
     with pytest.raises(ptxstd.PtxStdError):  # 2-byte offset: not 16-byte aligned
         ptxstd.rmsnorm_residual(flat[1:257].view(4, 64), w.cuda())
     assert C.sizeof(C.c_void_p) == 8
+
+
+# ---- the activations over all of bf16 -----------------------------------------------------------
+def _every_bf16():
+    """Every finite bf16 value, in order."""
+    x = torch.arange(1 << 16, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    return x[x.float().isfinite()].float().sort().values.to(torch.bfloat16)
+
+
+def _value_bounds(x, act):
+    """(f, f', bound of f, bound of f') in f64, the bounds relative to the values' own terms.
+
+    The exponential's argument z, at most 128 in size where its result is in range, passes at most
+    eight roundings to f32, those of the constants included: 8 * 128 * 2^-24 * ln 2 < 4.3e-5 of the
+    result. The exponential, the reciprocal, the polynomial and at most eight further operations
+    add less than 2^-19: 2^-14 = 6.1e-5 in all. Where the logistic function is below 2^-128, or the
+    density below 2^-126, zero may stand for it (asked a factor of two before). 2^-148: f32's
+    subnormals."""
+    rel, a, zero = 2.0 ** -14, x.abs(), torch.zeros_like(x)
+    if act in ("none", "relu"):
+        return R.act(x, act), torch.ones_like(x) if act == "none" else (x > 0).double(), zero, zero
+    if act == "gelu":
+        phi = torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+        cdf = 0.5 * torch.erfc(-x / math.sqrt(2))
+        f, df = x * cdf, cdf + x * phi
+        terms, out_of_range, sharp = cdf + a * phi, phi < 2.0 ** -125, zero
+        lost, lost_f = torch.minimum(cdf, 1 - cdf) + a * phi, torch.where(x < 0, f.abs(), zero)
+    else:
+        k, c = (math.sqrt(8 / math.pi), 0.044715) if act == "gelu_tanh" else (1.0, 0.0)
+        u, du = k * (x + c * x ** 3), k * (1 + 3 * c * x * x)
+        t, s = torch.sigmoid(u), torch.sigmoid(-u)
+        inner = torch.where(t * s == 0, zero, a * t * s * du)
+        f, df = x * t, t + x.sign() * inner
+        terms, out_of_range = t + inner, t < 2.0 ** -127
+        lost, lost_f = terms, f.abs()
+        # above zero the factor 1 - t has the absolute rounding of a value next to 1, at most 2^-22
+        # with the reciprocal's; below 2^-24 it is zero
+        sharp = torch.where((x > 0) & (s > 2.0 ** -26), a * du * 2.0 ** -22, zero) + \
+            torch.where((x > 0) & (s < 2.0 ** -22), inner, zero)
+    return f, df, rel * f.abs() + torch.where(out_of_range, lost_f, zero) + 2.0 ** -148, \
+        rel * terms + sharp + torch.where(out_of_range, lost, zero) + 2.0 ** -148
+
+
+@pytest.mark.parametrize("M", [1, 1100])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_activation_of_every_bf16(cuda, act, M):
+    """Zero operands, so that the bias is the pre-activation exactly: act(x) for every finite bf16,
+    held to its own size and not to x's. M: the kernel for few rows and the one for many."""
+    import ptxstd
+    x = _every_bf16()
+    N = x.numel()
+    a, sfa = ptxstd.quantize_mx(torch.zeros(M, 32, dtype=torch.bfloat16, device="cuda"), "e4m3",
+                                sf_layout=2)
+    b, sfb = ptxstd.quantize_mx(torch.zeros(N, 32, dtype=torch.bfloat16, device="cuda"), "e4m3",
+                                sf_layout=2)
+    c = ptxstd.gemm_mx_epilogue(a, "e4m3", sfa, b, "e4m3", sfb, bias=x, act=act)
+    _ok()
+    f, _, d, _ = _value_bounds(x.double(), act)
+    R.check_bf16(c[0], f, d, act)
+    assert (c == c[0]).all()
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_activation_gradient_of_every_bf16(cuda, act):
+    """One row with dh = 1: the f32 column sums are act'(x) itself; and the products' 8-bit blocks of
+    32 neighbouring values."""
+    import ptxstd
+    x = _every_bf16()
+    gate = x.view(1, -1)
+    row, _, db = ptxstd.act_backward_mx(torch.ones_like(gate), gate, act=act, elem_type="e4m3",
+                                        bias_grad=True)
+    _ok()
+    _, df, _, d = _value_bounds(x.double(), act)
+    bad = (db.double() - df).abs() > d
+    assert not bad.any(), (act, x[bad][:5].tolist(), db[bad][:5].tolist(), df[bad][:5].tolist(),
+                           d[bad][:5].tolist())
+    R.check_mx(*row, df.view(1, -1), d.view(1, -1), "e4m3", what=act)
