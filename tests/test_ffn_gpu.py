@@ -756,6 +756,39 @@ def test_block_stage_by_stage(cuda, M):
     R.check_bf16(dy, ref["dy"][0], 4 * CHAIN * ref["dy"][1], "dy")
 
 
+@pytest.mark.parametrize("M", [1, 40, 333])
+def test_training_step_as_documented(cuda, M):
+    """The calls of the documented training step (n and h in bf16, then both quantisers), with the down
+    projection's weight gradient; that one and dh held to their restatement on the stored operands."""
+    import ptxstd
+    b = Block(M, 256, 416, seed=31)
+    x1, n, stats = ptxstd.rmsnorm_residual(b.x, b.w, y=b.y, w_post=b.wp, gate=b.gate, scale=0.5)
+    q, sf = ptxstd.quantize_mx(n, "e4m3", sf_layout=2)
+    h, kept = ptxstd.gemm_mx_gated(q, "e4m3", sf, *b.qg, *b.qu, "e4m3", save=True)
+    hq, hsf = ptxstd.quantize_mx(h, "e4m3", sf_layout=2)
+    out = ptxstd.gemm_mx_epilogue(hq, "e4m3", hsf, b.qd[0], "e4m3", b.qd[1], residual=x1)
+    dq, dsf = ptxstd.quantize_mx(b.dout, "e5m2", sf_layout=2)
+    dh = ptxstd.gemm_mx_epilogue(dq, "e5m2", dsf, b.dt[0], "e4m3", b.dt[1])
+    dqt, dsft = ptxstd.quantize_mx_t(b.dout, "e5m2")
+    ht, hsft = ptxstd.quantize_mx_t(h, "e4m3")
+    dwd = ptxstd.gemm_mx_epilogue(dqt, "e5m2", dsft, ht, "e4m3", hsft)
+    nt, sfnt = ptxstd.quantize_mx_t(n, "e4m3")
+    dn, dwgu = ptxstd.gemm_mx_gated_backward(dh, *kept, nt, "e4m3", sfnt, b.gut[0], "e4m3",
+                                             b.gut[1])
+    dx, dw, dy, dwp, dg = ptxstd.rmsnorm_residual_backward(
+        dn, x1, b.w, stats, dx_out=b.dout, y=b.y, w_post=b.wp, gate=b.gate, scale=0.5)
+    _ok()
+    assert out.shape == dx.shape == dy.shape == (M, b.D) and dwd.shape == (b.D, b.F)
+    assert dwgu.shape == (2 * b.F, b.D) and dw.shape == dwp.shape == dg.shape == (b.D,)
+    R.check_mx(dqt, dsft, _t(_d(b.dout)), 0.0, "e5m2", what="dout^T")
+    R.check_mx(ht, hsft, _t(_d(h)), 0.0, "e4m3", what="h^T")
+    rows = dqt.shape[1]
+    c, cm = R.gemm(R.dequant(dqt, dsft, "e5m2"), R.dequant(ht, hsft, "e4m3"))
+    R.check_bf16(dwd, c, R.acc_bound(cm, rows), "dwd")
+    c, cm = R.gemm(R.dequant(dq, dsf, "e5m2"), R.dequant(*b.dt, "e4m3"))
+    R.check_bf16(dh, c, R.acc_bound(cm, b.D), "dh")
+
+
 def test_block_gradients_follow_the_exact_ones(cuda):
     """End to end against autograd of the unquantised block in 64 bits. A check of signs and factors,
     not of rounding: E4M3 / E5M2 operands carry up to 2^-4 and 2^-3 of relative rounding each
