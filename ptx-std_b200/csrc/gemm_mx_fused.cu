@@ -18,12 +18,14 @@
 //    Ragged sizes: TMA fills rows and K elements outside the tensors with zeros and clips the
 //    stores; MMAs of a last K stage whose 32 elements lie outside are not issued, so padding
 //    scales (which may be NaN codes) never meet a product that is kept.
-//    Bound by the tensor cores: a stage takes 505 clocks (clock64 traces), where 256 x 256 x 128 at
-//    the nominal rate takes 512; between two tiles the MMAs pause for about 400 clocks, and the
-//    1 kW power cap sets the clock. 8192^3: 361 us, 3.05 PFLOP/s, 0.93 of twice the measured bf16
-//    burst. The epilogue runs beside the next tile's MMAs and shows only when K is short:
-//    4096 x 4096 x 1024 takes 19.1 us plain, 26.6 us with a residual, 33 us with bias, GELU and
-//    an E4M3 result.
+//    Bound by the tensor cores: a stage (256 x 256 x 128) keeps a pair's pipes busy for 512 clocks
+//    and takes 602 clocks of the SMs' active time at 4096 x 8192 x 8192, 591 in the gated
+//    2048 x 14336 x 4096 (ncu, cold caches; the pipes are active 85 and 87 % of the time). Of the
+//    remainder only the pause between two tiles, about 400 clocks or 6 to 13 per stage, is accounted
+//    for. The 1 kW power cap sets the clock: 8192^3 takes 361 us (3.05 PFLOP/s, 0.93 of twice the
+//    measured bf16 burst) on a cool GPU and 377 to 415 us under load. The epilogue runs beside the
+//    next tile's MMAs and shows only when K is short: 4096 x 4096 x 1024 takes 19.1 us plain, 24.8 us
+//    with a residual, 31.7 us with bias, GELU and an E4M3 result.
 //
 // 2. narrow_kernel, for few rows (serving): weight streaming, bound by HBM. The operands swap: 128
 //    weight rows are the M side of a cta_group::1 MMA and the tokens (up to 256, a multiple of 16)
@@ -31,10 +33,10 @@
 //    over a cluster; the CTAs' partial accumulators meet in distributed shared memory and are
 //    added in rank order, each CTA finishing every S-th token, so the split needs no workspace,
 //    no atomics and no second kernel, and the result is reproducible. One token: N = 8192,
-//    K = 28672 with residual 38.7 us, 6.25 TB/s or 0.95 of the measured copy rate; gated
-//    F = 28672, K = 8192 78.7 us, 0.94 of it. With tens of tokens and mid-sized weights the CTAs'
+//    K = 28672 with residual 38.0 us, 6.4 TB/s or 0.97 of the measured copy rate; gated
+//    F = 28672, K = 8192 77.6 us, 0.95 of it. With tens of tokens and mid-sized weights the CTAs'
 //    start and end (about 4 us) and an uneven number of blocks per SM cost more: 48 tokens,
-//    F = 10240, K = 4096 18.7 us against 13.4 us of HBM time.
+//    F = 10240, K = 4096 18.4 us against 13.4 us of HBM time.
 //
 // Every device-side wait is bounded; a timeout records PTXSTD_ETIMEOUT.
 #include <atomic>
@@ -81,10 +83,10 @@ __device__ __forceinline__ float f(uint32_t r) { return __uint_as_float(r); }
 namespace wide {
 
 constexpr uint32_t P_BM = 256, P_BN = 256, P_HALF = 128;
-// Five stages, not the six that would fit: the mainloop runs as fast (8192^3: 372.6 us with five,
-// 372.2 us with six, 389 us with four), and the epilogue warps get three staging buffers each:
-// with a residual, 4096 x 4096 x 1024 takes 26.6 us instead of 40.6 us with one buffer and the
-// residual read by each lane from its own row.
+// Five stages, not the six that would fit: the mainloop runs as fast (8192^3 on a cool GPU, with
+// raster groups of 8: 372.6 us with five, 372.2 us with six, 389 us with four), and the epilogue
+// warps get three staging buffers each: with a residual, 4096 x 4096 x 1024 takes 24.8 us, and took
+// 40.6 us with one buffer and the residual read by each lane from its own row.
 constexpr uint32_t STAGES = 5;
 constexpr uint32_t kEpiWarps = 8;
 // Warpgroup 0 holds the producer and MMA warps and needs few registers; the two epilogue
@@ -103,7 +105,7 @@ constexpr uint32_t kSlotCols = 4 + 4 * (P_BN / 128);
 constexpr uint32_t kSfBase = P_BN;
 constexpr uint32_t kTmemCols = 512;
 static_assert(kSfBase + STAGES * kSlotCols <= kTmemCols, "TMEM budget");
-constexpr uint32_t kGroupM = 16;  // 8192^3: 363 us, against 372 us with 8 and 381 us with 4
+constexpr uint32_t kGroupM = 16;  // 8192^3, cool: 361 us, against 372 us with 8 and 381 us with 4
 constexpr uint32_t kCCols = 32;   // bf16 columns (or 64 MX bytes) per epilogue store
 using StageBox = ptxstd::epi::Box<kCCols>;
 constexpr uint32_t kBuffers = 3;  // staging buffers of an epilogue warp
@@ -1149,8 +1151,9 @@ int64_t narrow_slots(uint32_t split) {
 // 40 us): a launch 2.5; a CTA's start and end 1.5, which CTAs sharing an SM overlap; an SM takes
 // in its ring's bytes every 2.1 us, at most 95 GB/s; the partial sums' exchange 1.0 and 30 GB/s,
 // half as much again with two accumulators; and all of it no faster than HBM delivers. At M = 200,
-// N = 4128, K = 2080 it takes 64-token tiles without a split: 8.2 us, against 10.5 us for one
-// 208-token tile split in two and 9.8 us for the wide kernel.
+// N = 4128, K = 2080 it takes 64-token tiles without a split: 8.0 us, against 10.5 us for one
+// 208-token tile split in two and 9.8 us for the wide kernel (all for a plain bf16 result; with bias,
+// GELU and an E4M3 result the first takes 9.6 us).
 template <bool GATED>
 NarrowPlan narrow_plan(int64_t M, int64_t N, int64_t K) {
     const uint32_t G = GATED ? 2 : 1, cap = GATED ? 128 : 256;
@@ -1255,8 +1258,14 @@ double wide_us(int64_t M, int64_t N, int64_t K, bool gated) {
     return 2.5 + waves * (2.0 + num_k * (tiles > pairs ? 0.41 : 0.31));
 }
 
-// The narrow kernel where its estimate is clearly the better one. Above 1024 rows the wide kernel's
-// 256-row tiles fill the GPU at every size that matters and the narrow plan is not considered.
+// The narrow kernel where its estimate is clearly the better one, up to the 1024 rows that the
+// estimate was fitted over. Above, always the wide kernel. Both sides there, wide and narrow in us:
+// with enough columns the 256-row tiles fill the GPU, and the wide kernel is the faster one
+// (2048 x 2048 x 4096 15.9 and 19.0; 2048 x 4096 x 4096 27.9 and 38.1; 4096 x 576 x 7168 24.0 and
+// 36.3; gated 2048 x 512 x 4096 14.6 and 15.9). With few columns they do not, and as the wide kernel
+// has no split of K a long K is slow (1040 x 128 x 16384 40.4 and 12.2, just above the limit;
+// 2048 x 128 x 16384 41.8 and 15.3; 4096 x 128 x 16384 42.7 and 19.6; 2048 x 512 x 16384 43.3 and
+// 25.4; 2048 x 1024 x 1024 7.5 and 6.7).
 constexpr int64_t kNarrowRows = 1024;
 
 template <bool GATED>

@@ -24,10 +24,11 @@
 // accumulates them in f32; the partial sums go through a workspace and are added in order by a second
 // kernel (reproducible, no atomics), which applies the factors.
 //
-// Both directions are near the issue rate as well as the HBM rate (67 % and 60 % of the issue
+// Both directions are near the issue rate as well as the HBM rate (68 % and 59 % of the issue
 // slots, ncu), hence the packed f32 pairs. Forward, 8192 x 8192 with w_post, gate and E4M3 out:
-// 472 MB in 80 us, 5.9 TB/s or 0.90 of the measured copy rate; without w_post in bf16 537 MB in
-// 80 us, 1.02 of it; one row of 8192: 3.5 us. Backward, 8192 x 4096: 403 MB in 67.8 us, 0.91.
+// 472 MB in 77 to 80 us, 6.0 TB/s or 0.92 of the measured copy rate; without w_post in bf16 537 MB
+// in 80 us, 1.02 of it; one row of 8192: 3.3 us. Backward, 8192 x 4096: 403 MB in 68 us, 0.91 (72 us
+// after a second of load); 2000 x 16384: 393 MB in 137 us, 0.44 (column factors from L2 twice a row).
 #include "common.cuh"
 #include "data_types.cuh"
 #include "mx_block.cuh"
@@ -38,7 +39,6 @@ namespace {
 namespace dt = ptxstd::data_types;
 namespace mx = ptxstd::mx;
 
-using ptxstd::add2;
 using ptxstd::f32x2;
 using ptxstd::fma2;
 using ptxstd::hsum2;
@@ -953,11 +953,12 @@ extern "C" int ptxstd_rmsnorm_residual(const uint16_t* d_x, const uint16_t* d_y,
     if (nv <= 64) return launch_fwd<2, true>(p, 32, s);
     if (nv <= 128) return launch_fwd<4, true>(p, 32, s);
     // The ring pays where a row has two exchanges and there is enough to stream: with w_post,
-    // gate, E4M3 out, 8192 x 8192 takes 80 us against 95 us for a row per block, 8192 x 4096 43
-    // against 48 us, 8192 x 2048 28 against 31 us. Without w_post a row per block is at the copy
-    // rate already (8192 x 8192 in bf16: 80 us, the ring 92 us), and so it is the faster one for
-    // fewer elements (2400 x 4096: 17.9 against 18.6 us) and for rows that leave much of the long
-    // rows' groups idle (3000 x 5152: 28.3 against 29.5 us).
+    // gate, E4M3 out, 8192 x 8192 takes 77 to 80 us against 92 us for a row per block, 8192 x 4096
+    // 42.0 against 47.1 us, 8192 x 2048 25.8 against 30.0 us, 6000 x 2048 19.9 against 23.1 us. Below
+    // the limit the two come together (4000 x 2048 15.3 against 16.8 us, 2400 x 4096 17.3 against
+    // 17.7 us, 1200 x 8192 18.3 against 18.7 us), and a row per block is the faster one for rows that
+    // leave much of the long rows' groups idle (3000 x 5152: 26.9 us, the ring 28.1 us). Without
+    // w_post it is at the copy rate already (8192 x 8192 in bf16: 80 us).
     if (d_w_post && rows * cols >= 12'000'000) {
         if (nv <= 256) return launch_fwd_ring<2, 128, 6>(p, s);
         if (nv <= 512) return launch_fwd_ring<4, 128, 6>(p, s);
