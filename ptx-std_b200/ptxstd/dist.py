@@ -19,6 +19,7 @@ import ctypes as C
 import numpy as np
 
 from . import _dev, _stream, _torch, check, lib
+from .kernels import _given, _result
 
 _SIGS = {
     "ptxstd_dist_unique_id": (C.c_int, [C.c_void_p]),
@@ -109,11 +110,9 @@ class Dist:
             self.handle = None
 
     def gemm_nvfp4(self, a, sfa, ga, b_shard, sfb_shard, gb, n_total, out=None, stream=None):
-        torch = _torch()
         M, Kh = a.shape
         ns = n_total // self.world
-        c = out if out is not None else torch.empty((M, ns), dtype=torch.bfloat16,
-                                                    device=a.device)
+        c = _result(out, M, ns, a.device)
         check(_lib().ptxstd_gemm_nvfp4_sharded(self.handle, _dev(a), _dev(sfa), float(ga),
                                                _dev(b_shard), _dev(sfb_shard), float(gb),
                                                _dev(c), M, n_total, 2 * Kh, _stream(stream)),
@@ -122,15 +121,13 @@ class Dist:
 
     def gemm_decode(self, x, w_shard, sfw_shard, gw, n_total, out=None, stream=None):
         """y [M, n_total] (every rank) = MXFP8(x) * NVFP4(W)^T * gw, W split along N."""
-        torch = _torch()
         M, K = x.shape
+        y = _result(out, M, n_total, x.device)
         nbytes = int(_lib().ptxstd_gemm_decode_sharded_workspace_bytes(self.handle, M, n_total,
                                                                         K))
         if nbytes == 0:
             raise ValueError("bad decode shape for this communicator")
         ptr = self._workspace(nbytes, x.device)
-        y = out if out is not None else torch.empty((M, n_total), dtype=torch.bfloat16,
-                                                    device=x.device)
         check(_lib().ptxstd_gemm_decode_sharded(self.handle, _dev(x), _dev(w_shard),
                                                 _dev(sfw_shard), float(gw), _dev(y), M, n_total,
                                                 K, ptr, nbytes, _stream(stream)),
@@ -165,6 +162,8 @@ class Dist:
         fused into the GEMM. Returns rows [:M] of the library-owned output (valid until the next
         call), or `out` filled with a copy of them."""
         M, K = x.shape
+        if out is not None:
+            _given(out, 2 * M * n_total, x.device, "out")
         y = self.decode_p2p_output(n_total)
         ns = n_total // self.world
         nbytes = int(lib().ptxstd_gemm_decode_workspace_bytes(M, ns, K))

@@ -116,3 +116,22 @@ def test_given_outputs_have_room(ptxstd_lib):
         with pytest.raises(ValueError, match="too small"):
             call()
             pytest.fail(name)
+
+
+def test_given_outputs_of_the_sharded_gemms_have_room(ptxstd_lib):
+    """A communicator that was never set up: the refusals come before any call on it."""
+    import torch
+
+    from ptxstd.dist import Dist
+    d = Dist.__new__(Dist)
+    d.world, d.rank, d.handle, d._p2p, d._ws = 2, 0, None, None, {}
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)
+    a, w = torch.zeros((256, 32), dtype=torch.uint8), torch.zeros((128, 32), dtype=torch.uint8)
+    sf = torch.zeros(1024, dtype=torch.uint8)
+    c = torch.zeros(256 * 128 - 1, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="too small"):
+        d.gemm_nvfp4(a, sf, 1.0, w, sf, 1.0, 256, out=c)
+    with pytest.raises(ValueError, match="too small"):
+        d.gemm_decode(x, w, sf, 1.0, 256, out=c[:4 * 256 - 1])
+    with pytest.raises(ValueError, match="too small"):
+        d.gemm_decode_p2p(x, w, sf, 1.0, 256, out=c[:4 * 256 - 1])
